@@ -406,6 +406,114 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
                                     int64_t* ge_dev, int64_t* total_dev, void* stream);
 
 /*
+ * Sequence operators: layer norm, linear attention with a decay per head, attention with a sliding window and sinks.
+ * No counterpart in the reference, whose sequence models are torch.nn's GRU and LSTM (core/models.py:19-25); these are the
+ * mixers that a frame-by-frame model is built from, each over whole recordings (with its backward pass) and for one
+ * live frame at a time.  Common to all of them:
+ *   dtype        VAD_DTYPE_F32 or VAD_DTYPE_BF16, the element type of every void* tensor of a call.  Products of float32
+ *                are formed in float32; of bfloat16 exactly, summed in float32.  Sums, states, softmax and norm statistics
+ *                are float32.
+ *   rows         q, k, v and the gradients of outputs are read through strides in ELEMENTS given on the host: {sequence,
+ *                row, head} (steps: {batch, head}, caches: {batch, slot, head}); the head dimension is dense.  Any alignment
+ *                works; rows that start 16-byte aligned with a head dimension of whole 16-byte pieces take the wide path.
+ *                Outputs are dense (rows, heads, dim).
+ *   sequences    starts_dev == NULL: n_seq sequences of max_len rows each.  Otherwise the rows of all sequences are packed
+ *                behind one another in n_tokens rows and starts_dev holds n_seq + 1 ascending int64 on the device, sequence s
+ *                being rows starts[s] .. starts[s+1] - 1 (empty ones allowed).  The table is NOT validated: entries are clamped
+ *                into 0 .. n_tokens.  Output rows before the first and behind the last sequence are set to zero.  max_len is
+ *                then a hint that sizes the launch; longer sequences are still computed in full.
+ *   masked rows  what lies outside a row's mask -- later rows, rows beyond the window, unfilled cache slots, rows of no
+ *                sequence -- has no influence on it, also where it holds infinities or NaN.
+ *   repeatability  no atomics: the same call gives the same bits.
+ */
+#define VAD_DTYPE_F32 0
+#define VAD_DTYPE_BF16 1
+#define VAD_MAX_HEAD_DIM 128
+#define VAD_MAX_SINKS 64
+
+/*
+ * Layer norm: y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (var: mean squared deviation).
+ *   x_dev           (rows, cols), rows x_stride elements apart (cols dense)
+ *   weight_dev, bias_dev   cols values of weight_dtype (VAD_DTYPE_F32 or dtype), each may be NULL
+ *   y_dev           (rows, cols) dense
+ *   stats_dev       (rows, 2) mean and 1 / sqrt(var + eps) for the backward pass; may be NULL
+ * Backward: dx_dev (rows, cols) dense, dweight_dev / dbias_dev cols values of weight_dtype; each of the three may be NULL.
+ * workspace_dev: vad_layer_norm_workspace_bytes(rows, cols), needed for dweight / dbias.
+ */
+size_t vad_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+int vad_layer_norm_forward(const void* x_dev, int64_t rows, int64_t cols, int64_t x_stride,
+                           const void* weight_dev, const void* bias_dev, int dtype, int weight_dtype, float eps,
+                           void* y_dev, float* stats_dev, void* stream);
+int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, int64_t rows, int64_t cols, int64_t x_stride,
+                            int64_t dy_stride, const void* weight_dev, int dtype, int weight_dtype,
+                            const float* stats_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
+                            void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/*
+ * Linear attention with a decay per head:  S_t = exp(log_decay) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t.
+ *   log_decay_dev   heads float32, <= 0.  Not validated: values are clamped into -87 .. 0.
+ *   state_in_dev    (n_seq, heads, dim, dim) float32, S before the first row ([key dim][value dim]); NULL = zero
+ *   state_out_dev   S behind the last row (state_in for an empty sequence); may be NULL, must not be state_in_dev
+ * Backward: do_dev the gradient of o, dstate_out_dev that of state_out (NULL = zero); dq_dev / dk_dev / dv_dev dense,
+ * dstate_in_dev (may be NULL) that of state_in.  The decay is a constant of the model: it gets no gradient.
+ * workspace_dev: vad_linear_attention_workspace_bytes(n_seq, max_len, heads, dim, backward).
+ *
+ * Step: one row per sequence; state_dev (batch, heads, dim, dim) is updated in place.
+ */
+size_t vad_linear_attention_workspace_bytes(int64_t n_seq, int64_t max_len, int heads, int dim, int backward);
+int vad_linear_attention_forward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                 const void* v_dev, const int64_t* v_strides, const int64_t* starts_dev, int64_t n_seq,
+                                 int64_t n_tokens, int64_t max_len, int heads, int dim, int dtype,
+                                 const float* log_decay_dev, float scale, const float* state_in_dev, void* o_dev,
+                                 float* state_out_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+int vad_linear_attention_backward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                  const void* v_dev, const int64_t* v_strides, const void* do_dev, const int64_t* do_strides,
+                                  const int64_t* starts_dev, int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads,
+                                  int dim, int dtype, const float* log_decay_dev, float scale, const float* state_in_dev,
+                                  const float* dstate_out_dev, void* dq_dev, void* dk_dev, void* dv_dev,
+                                  float* dstate_in_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+int vad_linear_attention_step(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                              const void* v_dev, const int64_t* v_strides, int64_t batch, int heads, int dim, int dtype,
+                              const float* log_decay_dev, float scale, float* state_dev, void* o_dev, void* stream);
+
+/*
+ * Attention with a sliding window and sinks: row i sees key j when j <= i and (i - j < window or j < sinks);
+ * o_i = softmax over the visible keys of (scale q_i . k_j) v_j.  heads query heads share kv_heads key heads: query head h
+ * reads key head h / (heads / kv_heads).  sinks <= VAD_MAX_SINKS, scale > 0, at most 2^30 rows.
+ *   stats_dev       (rows, heads, 2) float32 softmax statistics for the backward pass; may be NULL in the forward call
+ * Backward: o_dev the forward call's output; dk_dev / dv_dev (rows, kv_heads, dim).
+ * workspace_dev: vad_window_attention_workspace_bytes(..., n_rows = rows of q, ...).
+ *
+ * Step: one row per sequence against a rolling cache (batch, sinks + window, kv_heads, dim) of the same dtype.  Row pos
+ * goes to slot pos while pos < sinks, then to sinks + (pos - sinks) % window.  pos_dev[b] is the number of rows that
+ * sequence b has had before; a negative one gives zeros and leaves the cache alone.  Slots beyond pos are not read.
+ * vad_window_cache_fill brings whole sequences into their caches (and, where pos_dev is given, sets it to their lengths);
+ * slots that no row belongs to stay as they are.
+ */
+size_t vad_window_attention_workspace_bytes(int64_t n_seq, int64_t n_rows, int64_t max_len, int heads, int kv_heads,
+                                            int dim, int64_t window, int sinks);
+int vad_window_attention_forward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                 const void* v_dev, const int64_t* v_strides, const int64_t* starts_dev, int64_t n_seq,
+                                 int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype,
+                                 int64_t window, int sinks, float scale, void* o_dev, float* stats_dev, void* stream);
+int vad_window_attention_backward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                  const void* v_dev, const int64_t* v_strides, const void* o_dev, const void* do_dev,
+                                  const int64_t* do_strides, const float* stats_dev, const int64_t* starts_dev, int64_t n_seq,
+                                  int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype,
+                                  int64_t window, int sinks, float scale, void* dq_dev, void* dk_dev, void* dv_dev,
+                                  void* workspace_dev, size_t workspace_bytes, void* stream);
+size_t vad_window_step_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int64_t window, int sinks);
+int vad_window_attention_step(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                              const void* v_dev, const int64_t* v_strides, void* cache_k_dev, const int64_t* cache_k_strides,
+                              void* cache_v_dev, const int64_t* cache_v_strides, const int64_t* pos_dev, int64_t batch,
+                              int heads, int kv_heads, int dim, int dtype, int64_t window, int sinks, float scale,
+                              void* o_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+int vad_window_cache_fill(const void* k_dev, const int64_t* k_strides, const void* v_dev, const int64_t* v_strides,
+                          const int64_t* starts_dev, int64_t n_seq, int64_t n_tokens, int64_t max_len, int kv_heads, int dim,
+                          int dtype, int64_t window, int sinks, void* cache_k_dev, const int64_t* cache_k_strides,
+                          void* cache_v_dev, const int64_t* cache_v_strides, int64_t* pos_dev, void* stream);
+
+/*
  * Deterministic synthetic 16 kHz int16 audio, written on the device: sample n
  * of stream `seed` is a pure integer function of (seed, n), reproducible on
  * the host.  No counterpart in the reference (its audio comes from datasets

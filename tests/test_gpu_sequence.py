@@ -1,0 +1,629 @@
+"""Layer norm, linear attention with a decay per head and attention with a sliding window and sinks, on the GPU, against
+their float64 forms (oracle/sequence_ref.py).
+
+Tolerances, derived before the first run.  u = half a step of the element type (bf16 2^-8; float32 products and sums are
+counted in 2^-24).  An output is rounded once: u |ref|.  Inside, bfloat16 kernels round the weights (and the copy of the
+state that q meets) once, each error at most u of its term, so at most u `mag`, mag being the sum of the terms' absolute
+values; the softmax's dS carries two (the weight itself, and rowsum(dO O) formed from the rounded o).  A float32 sum of n
+terms is off by at most n 2^-24 mag.  A softmax weight inherits the absolute error of its score, (dim + 4) 2^-24 `size`, once
+from itself and once from the sum it is divided by; powers of the decay are exponentials of at most 87 (larger ones vanish):
+90 2^-24."""
+import math
+
+import pytest
+import torch
+
+from oracle import sequence_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8}
+ULP = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def _rand(gen, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=gen, device='cuda') * scale).to(dtype)
+
+
+def _gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def _close(got, want, mag, inner, dtype, what):
+    """|got - want| <= inner * mag + (u + 2^-24) |want|, elementwise; NaN nowhere."""
+    err = (got.double() - want).abs()
+    tol = inner * mag + (U[dtype] + ULP) * want.abs() + 1e-38
+    worst = float((err / tol).max()) if err.numel() else 0.0
+    assert worst <= 1.0, '%s: %.2f of the tolerance' % (what, worst)
+
+
+# ---- layer norm ----
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,cols', [(1, 1), (3, 2), (1, 7), (1000, 24), (333, 30), (65, 64), (2048, 900), (5, 1025), (700, 1024), (17, 2047),
+                                       (9, 4096), (3, 16384), (4, 20001), (2, 40000)])
+def test_layer_norm(vad, dtype, rows, cols):
+    g = _gen(rows * 7 + cols)
+    x = (_rand(g, rows, cols) * 2 + 3).to(dtype).requires_grad_()
+    w = (1 + _rand(g, cols, scale=0.3)).requires_grad_()
+    b = _rand(g, cols).requires_grad_()
+    dy = _rand(g, rows, cols, dtype=dtype)
+    y = vad.layer_norm(x, w, b)
+    assert y.dtype == dtype and y.shape == x.shape
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    want = ref.layer_norm(x.detach(), w.detach(), b.detach(), 1e-5, dy)
+    xd = x.detach().double()
+    r = 1 / torch.sqrt(xd.var(1, unbiased=False, keepdim=True) + 1e-5)
+    # a row's sum: at most 160 values down a lane (256 lanes, 40000 columns) and 9 levels across; one deviation from the mean
+    # is off by that of the largest value, then a few roundings
+    n = 180 * ULP
+    xh = ((xd - xd.mean(1, keepdim=True)) * r).abs()
+    size = xd.abs().amax(1, keepdim=True) * r                     # what an error of the mean, relative to x, does to xh
+    mag_xh = size + xh * (1 + size * size)                        # and through the variance
+    _close(y.detach(), want[0], mag_xh * w.detach().abs() + b.detach().abs(), n, dtype, 'y')
+    gw = (dy.double() * w.detach()).abs()
+    mag = r * (gw + gw.mean(1, keepdim=True) + (xh + mag_xh) * (gw * (xh + mag_xh)).mean(1, keepdim=True)) * (1 + size * size)
+    _close(grads[0], want[1], mag, n, dtype, 'dx')
+    rows_n = (rows + 64) * ULP
+    _close(grads[1], want[2], (dy.double().abs() * (xh + mag_xh)).sum(0), rows_n + n, torch.float32, 'dw')
+    _close(grads[2], want[3], dy.double().abs().sum(0), rows_n, torch.float32, 'db')
+
+
+def test_layer_norm_parameters_shapes_and_strides(vad):
+    g = _gen(5)
+    x = _rand(g, 4, 6, 48)
+    w16, b16 = (1 + _rand(g, 48)).bfloat16(), _rand(g, 48).bfloat16()
+    plain = ref.layer_norm(x, None, None, 1e-5)
+    assert float((vad.layer_norm(x).double() - plain).abs().max()) < 1e-5
+    assert float((vad.layer_norm(x, bias=b16.float()).double() - plain - b16.double()).abs().max()) < 1e-5
+    y16 = vad.layer_norm(x.bfloat16(), w16, b16)
+    want = ref.layer_norm(x.bfloat16(), w16, b16, 1e-5)
+    assert float(((y16.double() - want).abs() / (want.abs() + 1e-2)).max()) < 2.0 ** -8 + 1e-4
+    # bfloat16 parameters get bfloat16 gradients
+    leaf = [t.clone().requires_grad_() for t in (x.bfloat16(), w16, b16)]
+    dy = _rand(g, 4, 6, 48, dtype=torch.bfloat16)
+    grads = torch.autograd.grad(vad.layer_norm(*leaf), leaf, dy)
+    exact = ref.layer_norm(leaf[0].detach(), w16, b16, 1e-5, dy)
+    for got, e in zip(grads, exact[1:]):
+        assert got.dtype == torch.bfloat16
+        assert float(((got.double() - e).abs() / (e.abs() + 1e-2)).max()) < 2.0 ** -8 + 1e-3
+    # only some of the gradients, and every stride: the same bits as dense rows
+    wide = _rand(g, 40, 100)
+    for view in (wide[:, 3:51], wide[::2, :48], wide[:, :48].T.contiguous().T, wide[:1, :48].expand(40, 48), wide[:, ::2]):
+        leaf = view.detach().requires_grad_()
+        w = torch.ones(view.size(1), device='cuda')
+        y = vad.layer_norm(leaf, w)
+        dense = view.contiguous().requires_grad_()
+        yd = vad.layer_norm(dense, w)
+        assert torch.allclose(y, yd, rtol=1e-6, atol=1e-6)
+        ones = torch.ones((), device='cuda').expand(y.shape)
+        assert torch.allclose(torch.autograd.grad(y, leaf, ones)[0], torch.autograd.grad(yd, dense, ones)[0], atol=1e-5)
+    # no rows; a row with a NaN leaves the others alone; huge offsets keep their variance
+    empty = torch.empty(0, 24, device='cuda', requires_grad=True)
+    we = torch.ones(24, device='cuda', requires_grad=True)
+    ge = torch.autograd.grad(vad.layer_norm(empty, we), (empty, we), torch.empty(0, 24, device='cuda'))
+    assert ge[0].shape == (0, 24) and not ge[1].any()
+    x = _rand(g, 64, 24)
+    clean = vad.layer_norm(x)
+    x[10, 3] = math.nan
+    dirty = vad.layer_norm(x)
+    assert dirty[10].isnan().all() and torch.equal(dirty[:10], clean[:10]) and torch.equal(dirty[11:], clean[11:])
+    far = torch.arange(24, device='cuda').float().repeat(8, 1) + 2.0 ** 20
+    assert float((vad.layer_norm(far).double() - ref.layer_norm(far, None, None, 1e-5)).abs().max()) < 1e-5
+
+
+# ---- linear attention ----
+
+def _decays(heads):
+    # forgetting within 2, 4, ... rows, never, and at once
+    vals = [math.log1p(-2.0 ** -(1 + i)) for i in range(8)] + [0.0, -200.0]
+    return torch.tensor([vals[(3 * i + 2) % len(vals)] for i in range(heads)], device='cuda')
+
+
+def _decay_reference(q, k, v, log_decay, scale, starts, state, do, dstate):
+    """Results and magnitudes laid out as the operator lays them out."""
+    a = log_decay.clamp(-87.0, 0.0).double().tolist()
+    seqs = [ref.sequences(t.detach().double(), starts) for t in (q, k, v, do)]
+    out = {n: [] for n in ('o', 'dq', 'dk', 'dv', 'state', 'dstate')}
+    out.update({'mag_' + n: [] for n in list(out)})
+    for s, (qs, ks, vs, gs) in enumerate(zip(*seqs)):
+        heads = [ref.decay_sequence(qs[:, h], ks[:, h], vs[:, h], a[h], scale, None if state is None else state[s, h].detach().double(),
+                                    gs[:, h], None if dstate is None else dstate[s, h].double()) for h in range(len(a))]
+        for n in out:
+            out[n].append(torch.stack([x[n] for x in heads], 0 if 'state' in n else 1))
+    join = torch.stack if starts is None else torch.cat
+    return {n: torch.stack(x) if 'state' in n else join(x) for n, x in out.items()}
+
+
+DECAY_CASES = [   # lengths, heads, dim, packed
+    ([1], 1, 1, False), ([1, 1, 1], 2, 30, False), ([64], 2, 64, False), ([65, 65], 3, 33, False), ([63], 1, 128, False), ([166] * 3, 3, 30, False),
+    ([700], 2, 64, False), ([1500], 1, 128, False), ([0, 5, 0, 131, 64, 1], 2, 64, True), ([300, 1100, 0], 3, 30, True), ([900, 20], 1, 96, True),
+    ([1300], 2, 16, True),
+]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths,heads,dim,packed', DECAY_CASES)
+def test_linear_attention(vad, dtype, lengths, heads, dim, packed):
+    g = _gen(sum(lengths) + dim)
+    lead = (sum(lengths),) if packed else (len(lengths), lengths[0])
+    starts = torch.tensor([0] + lengths, device='cuda').cumsum(0) if packed else None
+    q, k, v, do = (_rand(g, *lead, heads, dim, dtype=dtype) for _ in range(4))
+    state, dstate = (_rand(g, len(lengths), heads, dim, dim) for _ in range(2))
+    log_decay, scale = _decays(heads), 0.3
+    leaf = [t.requires_grad_() for t in (q, k, v, state)]
+    o, last = vad.linear_attention(*leaf[:3], log_decay, scale=scale, state=leaf[3], starts=starts, max_len=max(lengths))
+    assert o.dtype == dtype and o.shape == q.shape and last.dtype == torch.float32
+    grads = torch.autograd.grad((o, last), leaf, (do, dstate))
+    want = _decay_reference(q, k, v, log_decay, scale, starts, state, do, dstate)
+    pieces = -(-max(lengths) // 64)
+    n = (2 * dim + 2 * 64 + 4 * pieces + 100) * ULP
+    for name, got in (('o', o.detach()), ('dq', grads[0]), ('dk', grads[1]), ('dv', grads[2])):
+        _close(got, want[name], want['mag_' + name], U[dtype] + n, dtype, name)
+    for name, got in (('state', last.detach()), ('dstate', grads[3])):        # the state is exact to float32 in either type
+        _close(got, want[name], want['mag_' + name], n, torch.float32, name)
+    # without a state, and only the state's gradient
+    o2, last2 = vad.linear_attention(q.detach(), k.detach(), v.detach(), log_decay, scale=scale, starts=starts)
+    want = _decay_reference(q, k, v, log_decay, scale, starts, None, do, None)
+    _close(o2, want['o'], want['mag_o'], U[dtype] + n, dtype, 'o from zero')
+    _close(last2, want['state'], want['mag_state'], n, torch.float32, 'state from zero')
+    again = vad.linear_attention(q.detach(), k.detach(), v.detach(), log_decay, scale=scale, starts=starts)
+    assert torch.equal(o2, again[0]) and torch.equal(last2, again[1])
+
+
+def test_linear_attention_gradients_against_differences(vad):
+    g = _gen(3)
+    q, k, v = (_rand(g, 2, 150, 2, 30) for _ in range(3))
+    state = _rand(g, 2, 2, 30, 30)
+    wo, ws = _rand(g, 2, 150, 2, 30), _rand(g, 2, 2, 30, 30)
+    log_decay = torch.tensor([-0.05, 0.0], device='cuda')
+
+    def loss(*t):
+        o, s = vad.linear_attention(*t[:3], log_decay, state=t[3])
+        return (o.double() * wo).sum() + (s.double() * ws).sum()
+
+    leaf = [t.requires_grad_() for t in (q, k, v, state)]
+    grads = torch.autograd.grad(loss(*leaf), leaf)
+    # the loss is linear in each input by itself: a central difference of any length is exact but for rounding
+    for i, got in enumerate(grads):
+        d = _rand(g, *leaf[i].shape)
+        with torch.no_grad():
+            moved = [[t + s * d if j == i else t for j, t in enumerate(leaf)] for s in (0.5, -0.5)]
+            slope = float(loss(*moved[0]) - loss(*moved[1]))
+        assert slope == pytest.approx(float((got.double() * d).sum()), rel=2e-4, abs=2e-2)
+
+
+def test_linear_attention_step_goes_on_from_a_recording(vad):
+    for dtype in DTYPES:
+        for heads, dim in ((3, 30), (2, 64), (1, 1), (4, 128), (2, 33)):
+            g = _gen(dim)
+            q, k, v = (_rand(g, 5, 80, heads, dim, dtype=dtype) for _ in range(3))
+            log_decay = _decays(heads)
+            whole, last = vad.linear_attention(q, k, v, log_decay)
+            _, state = vad.linear_attention(q[:, :70], k[:, :70], v[:, :70], log_decay)
+            want = _decay_reference(q, k, v, log_decay, dim ** -0.5, None, None, q, None)
+            for t in range(70, 80):
+                o = vad.linear_attention_step(q[:, t], k[:, t], v[:, t], log_decay, state)
+                _close(o, want['o'][:, t], want['mag_o'][:, t], (dim + 150) * ULP, dtype, 'step %d' % t)
+            _close(state, want['state'], want['mag_state'], (dim + 250) * ULP, torch.float32, 'state')
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_linear_attention_later_rows_do_not_reach_earlier_ones(vad, dtype):
+    """Infinities and NaN from row 100 on leave rows 0 .. 99 as they were, and the gradients the other way round; other
+    sequences and heads feel nothing."""
+    g = _gen(9)
+    q, k, v, do = (_rand(g, 2, 200, 2, 64, dtype=dtype) for _ in range(4))
+    log_decay = _decays(2)
+    clean = vad.linear_attention(q, k, v, log_decay)[0]
+    for which in range(3):
+        t = [x.clone() for x in (q, k, v)]
+        t[which][0, 100:, 0] = math.nan if which else math.inf
+        o = vad.linear_attention(*t, log_decay)[0]
+        assert torch.isfinite(o[0, :100]).all() and torch.isfinite(o[1]).all() and torch.isfinite(o[0, :, 1]).all()
+        assert torch.allclose(o[0, :100].float(), clean[0, :100].float(), rtol=2 * U[dtype] + 1e-4, atol=1e-3)
+        assert torch.equal(o[1], clean[1])
+    leaf = [x.clone().requires_grad_() for x in (q, k, v)]
+    bad = do.clone()
+    bad[0, :100, 0] = math.nan
+    grads = torch.autograd.grad(vad.linear_attention(*leaf, log_decay)[0], leaf, bad)
+    for x in grads[1:]:
+        assert torch.isfinite(x[0, 100:]).all() and torch.isfinite(x[1]).all()
+    assert torch.isfinite(grads[0][0, 100:]).all()
+
+
+# ---- window attention ----
+
+def _window_reference(q, k, v, window, sinks, scale, starts, do):
+    heads, group = q.size(-2), q.size(-2) // k.size(-2)
+    seqs = [ref.sequences(t.detach().double(), starts) for t in (q, k, v, do)]
+    out = {n: [] for n in ('o', 'dq', 'dk', 'dv', 'mag_o', 'mag_dq', 'mag_dk', 'mag_dv')}
+    size = 0.0
+    for qs, ks, vs, gs in zip(*seqs):
+        per = [ref.window_sequence(qs[:, h], ks[:, h // group], vs[:, h // group], window, sinks, scale, gs[:, h]) for h in range(heads)]
+        size = max([size] + [x['size'] for x in per])
+        for n in out:
+            t = torch.stack([x[n] for x in per], 1)
+            out[n].append(t.unflatten(1, (heads // group, group)).sum(2) if n[-2:] in ('dk', 'dv') else t)
+    join = torch.stack if starts is None else torch.cat
+    return {n: join(x) for n, x in out.items()}, size
+
+
+WINDOW_CASES = [   # lengths, heads, kv heads, dim, window, sinks, packed
+    ([1], 1, 1, 1, 1, 0, False), ([1, 1], 2, 1, 30, 5, 3, False), ([64], 2, 2, 64, 64, 0, False), ([65], 3, 3, 33, 1, 0, False),
+    ([200], 2, 1, 64, 30, 0, False), ([200] * 2, 4, 2, 64, 17, 4, False), ([300], 2, 1, 128, 100, 64, False), ([700], 3, 3, 30, 30, 0, False),
+    ([500], 2, 1, 16, 1, 1, False), ([450], 1, 1, 96, 1000, 7, False), ([0, 3, 129, 0, 65, 256, 1], 4, 2, 64, 63, 2, True),
+    ([700, 40], 6, 2, 30, 129, 20, True), ([1200, 0], 2, 1, 128, 256, 33, True), ([1700], 4, 1, 64, 40, 5, True),
+]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lengths,heads,kv_heads,dim,window,sinks,packed', WINDOW_CASES)
+def test_window_attention(vad, dtype, lengths, heads, kv_heads, dim, window, sinks, packed):
+    g = _gen(sum(lengths) + dim + window)
+    lead = (sum(lengths),) if packed else (len(lengths), lengths[0])
+    starts = torch.tensor([0] + lengths, device='cuda').cumsum(0) if packed else None
+    q, do = (_rand(g, *lead, heads, dim, dtype=dtype) for _ in range(2))
+    k, v = (_rand(g, *lead, kv_heads, dim, dtype=dtype) for _ in range(2))
+    scale = 1.5 * dim ** -0.5
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    o = vad.window_attention(*leaf, window, sinks, scale=scale, starts=starts, max_len=max(lengths))
+    assert o.dtype == dtype and o.shape == q.shape
+    grads = torch.autograd.grad(o, leaf, do)
+    want, size = _window_reference(q, k, v, window, sinks, scale, starts, do)
+    n = (2 * (dim + 8) * max(size, 1.0) + max(lengths) + dim) * ULP
+    _close(o.detach(), want['o'], want['mag_o'], U[dtype] + n, dtype, 'o')
+    _close(grads[2], want['dv'], want['mag_dv'], U[dtype] + n * (heads // kv_heads), dtype, 'dv')
+    _close(grads[0], want['dq'], want['mag_dq'], 2 * U[dtype] + 2 * n, dtype, 'dq')
+    _close(grads[1], want['dk'], want['mag_dk'], 2 * U[dtype] + 2 * n * (heads // kv_heads), dtype, 'dk')
+    with torch.no_grad():
+        assert torch.equal(vad.window_attention(q, k, v, window, sinks, scale=scale, starts=starts), o)
+    grads2 = torch.autograd.grad(vad.window_attention(*leaf, window, sinks, scale=scale, starts=starts, max_len=max(lengths)), leaf, do)
+    assert all(torch.equal(a, b) for a, b in zip(grads, grads2))
+
+
+def test_window_attention_gradients_against_differences(vad):
+    g = _gen(4)
+    q = _rand(g, 1, 150, 4, 30)
+    k, v = (_rand(g, 1, 150, 2, 30) for _ in range(2))
+    w = _rand(g, 1, 150, 4, 30)
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad((vad.window_attention(*leaf, 20, 3).double() * w).sum(), leaf)
+    for i, got in enumerate(grads):
+        d = _rand(g, *leaf[i].shape)
+        h = 2.0 ** -6
+        with torch.no_grad():
+            ends = [float((vad.window_attention(*[t + s * h * d if j == i else t for j, t in enumerate(leaf)], 20, 3).double() * w).sum())
+                    for s in (1, -1)]
+        slope = (ends[0] - ends[1]) / (2 * h)
+        # the third derivative's h^2 / 6 and the rounding of the two sums over 2 h
+        assert slope == pytest.approx(float((got.double() * d).sum()), rel=2e-3, abs=5e-2)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_window_attention_masked_rows_have_no_influence(vad, dtype):
+    """Infinities and NaN in keys and values that a row does not see -- later ones and those its window has left -- leave it
+    as it was; so do NaN queries and output gradients of rows that do not see a key, for that key's gradients."""
+    g = _gen(8)
+    window, sinks, n = 40, 4, 300
+    q, do = (_rand(g, 1, n, 2, 64, dtype=dtype) for _ in range(2))
+    k, v = (_rand(g, 1, n, 1, 64, dtype=dtype) for _ in range(2))
+    clean = vad.window_attention(q, k, v, window, sinks)
+    at = 130
+    rows = torch.arange(n, device='cuda')
+    blind = (rows < at) | (rows >= at + window)
+    for which, value in ((0, math.nan), (1, math.nan), (1, math.inf)):
+        t = [k.clone(), v.clone()]
+        t[which][0, at] = value
+        o = vad.window_attention(q, *t, window, sinks)
+        assert torch.isfinite(o[0, blind]).all() and not torch.isfinite(o[0, ~blind]).all()
+        assert torch.allclose(o[0, blind].float(), clean[0, blind].float(), rtol=2 * U[dtype] + 1e-4, atol=2 * U[dtype] + 1e-4)
+    keys = rows
+    unseen = (keys > at) | ((keys <= at - window) & (keys >= sinks))
+    for which in range(2):
+        t = [q.clone(), do.clone()]
+        t[which][0, at, 0] = math.nan
+        leaf = [x.requires_grad_() for x in (t[0], k.clone(), v.clone())]
+        grads = torch.autograd.grad(vad.window_attention(*leaf, window, sinks), leaf, t[1])
+        for x in grads[1:]:
+            assert torch.isfinite(x[0, unseen]).all() and not torch.isfinite(x[0, ~unseen]).all()
+        assert torch.isfinite(grads[0][0, rows != at]).all() and torch.isfinite(grads[0][0, :, 1]).all()
+
+
+STEP_CASES = [(1, 1, 1, 1, 1, 0), (3, 4, 2, 64, 30, 0), (2, 6, 2, 30, 100, 3), (2, 8, 1, 128, 700, 64), (1, 5, 5, 33, 257, 1), (4, 16, 4, 96, 64, 2)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('batch,heads,kv_heads,dim,window,sinks', STEP_CASES)
+def test_window_attention_step(vad, dtype, batch, heads, kv_heads, dim, window, sinks):
+    """Caches full of NaN, filled by recordings shorter and longer than they hold, then steps: every output is that of the
+    whole recording's row."""
+    g = _gen(window + dim)
+    slots = sinks + window
+    for length in (0, 1, sinks + 1, slots - 1 if slots > 1 else 1, slots, 2 * slots + 3):
+        total = length + 3
+        q = _rand(g, batch, total, heads, dim, dtype=dtype)
+        k, v = (_rand(g, batch, total, kv_heads, dim, dtype=dtype) for _ in range(2))
+        ck, cv = (torch.full((batch, slots, kv_heads, dim), math.nan, dtype=dtype, device='cuda') for _ in range(2))
+        pos = vad.window_cache_fill(k[:, :length], v[:, :length], ck, cv, window, sinks)
+        assert pos.tolist() == [length] * batch
+        want, size = _window_reference(q, k, v, window, sinks, dim ** -0.5, None, q)
+        tol = (2 * (dim + 8) * max(size, 1.0) + slots + dim) * ULP
+        for t in range(length, total):
+            o = vad.window_attention_step(q[:, t], k[:, t], v[:, t], ck, cv, pos, window, sinks)
+            _close(o, want['o'][:, t], want['mag_o'][:, t], tol, dtype, 'length %d row %d' % (length, t))
+            slot = ref.window_slot(t, window, sinks)
+            assert torch.equal(ck[:, slot], k[:, t]) and torch.equal(cv[:, slot], v[:, t])
+            pos += 1
+
+
+def test_window_step_rows_at_different_places(vad):
+    g = _gen(2)
+    window, sinks, dim = 50, 2, 64
+    pos = torch.tensor([0, -1, 1, 51, 2 ** 33 + 5, -7, 60], device='cuda')
+    b = pos.numel()
+    q, k, v = _rand(g, b, 4, dim), _rand(g, b, 2, dim), _rand(g, b, 2, dim)
+    ck, cv = _rand(g, b, 52, 2, dim), _rand(g, b, 52, 2, dim)
+    before = ck.clone(), cv.clone()
+    o = vad.window_attention_step(q, k, v, ck, cv, pos, window, sinks)
+    for i, p in enumerate(pos.tolist()):
+        if p < 0:
+            assert not o[i].any() and torch.equal(ck[i], before[0][i]) and torch.equal(cv[i], before[1][i])
+            continue
+        kk, vv = before[0][i].clone(), before[1][i].clone()
+        slot = ref.window_slot(p, window, sinks)
+        kk[slot], vv[slot] = k[i], v[i]
+        assert torch.equal(ck[i], kk) and torch.equal(cv[i], vv)
+        n = min(p + 1, 52)
+        for h in range(4):
+            w = torch.softmax(kk[:n, h // 2].double() @ q[i, h].double() * dim ** -0.5, 0)
+            assert float((o[i, h].double() - w @ vv[:n, h // 2].double()).abs().max()) < 1e-5
+
+
+# ---- what all share ----
+
+def _packed_views(t):
+    """The same values at other strides: a slice of a wider tensor, heads first, and one element off alignment."""
+    yield torch.cat([t, t, t], -2)[..., t.size(-2):2 * t.size(-2), :]
+    yield t.transpose(-3, -2).contiguous().transpose(-3, -2)
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.flatten()
+    yield flat[1:].view(t.shape)
+    yield t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_strides_and_alignment(vad, dtype):
+    g = _gen(6)
+    q, k, v, do = (_rand(g, 2, 130, 2, 64, dtype=dtype) for _ in range(4))
+    log_decay = _decays(2)
+
+    def everything(q, k, v, do):
+        leaf = [t.detach().requires_grad_() for t in (q, k, v)]
+        o, s = vad.linear_attention(*leaf, log_decay)
+        w = vad.window_attention(*leaf, 50, 2)
+        return [o, s, w, *torch.autograd.grad(o, leaf, do), *torch.autograd.grad(w, leaf, do)]
+
+    want = everything(q, k, v, do)
+    for views in zip(*(_packed_views(t) for t in (q, k, v, do))):
+        for a, b in zip(everything(*views), want):
+            assert torch.equal(a, b)
+    # an expanded gradient, as sum().backward() gives
+    leaf = [t.clone().requires_grad_() for t in (q, k, v)]
+    vad.window_attention(*leaf, 50, 2).sum().backward()
+    ones = torch.autograd.grad(vad.window_attention(*leaf, 50, 2), leaf, torch.ones_like(q))
+    assert all(torch.equal(a.grad, b) for a, b in zip(leaf, ones))
+    # steps on slices of a fused projection
+    x = _rand(g, 3, 3, 2, 64, dtype=dtype)
+    state = _rand(g, 3, 2, 64, 64)
+    a = vad.linear_attention_step(x[:, 0], x[:, 1], x[:, 2], log_decay, state.clone())
+    b = vad.linear_attention_step(*[x[:, i].contiguous() for i in range(3)], log_decay, state.clone())
+    assert torch.equal(a, b)
+    cache = _rand(g, 3, 2, 20, 2, 64, dtype=dtype)
+    pos = torch.tensor([3, 19, 100], device='cuda')
+    a = vad.window_attention_step(x[:, 0], x[:, 1], x[:, 2], cache[:, 0], cache[:, 1], pos, 20)
+    cc = cache.clone()
+    b = vad.window_attention_step(*[x[:, i].contiguous() for i in range(3)], cc[:, 0].contiguous(), cc[:, 1].contiguous(), pos, 20)
+    assert torch.equal(a, b)
+
+
+def test_rows_of_no_sequence(vad):
+    """Rows before the first and behind the last sequence: NaN there reaches nothing, outputs and gradients there are zero; a
+    table that reaches outside is cut off."""
+    g = _gen(7)
+    n, lo, hi = 300, 17, 260
+    q, k, v, do = (_rand(g, n, 2, 64) for _ in range(4))
+    for t in (q, k, v, do):
+        t[:lo] = math.nan
+        t[hi:] = math.nan
+    starts = torch.tensor([lo, 100, 100, hi], device='cuda')
+    log_decay = _decays(2)
+    inner = torch.tensor([0, 100 - lo, 100 - lo, hi - lo], device='cuda')
+    for call in (lambda *t, s: vad.linear_attention(*t, log_decay, starts=s)[0], lambda *t, s: vad.window_attention(*t, 30, 4, starts=s, max_len=200)):
+        leaf = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = call(*leaf, s=starts)
+        cut = [t[lo:hi].clone().requires_grad_() for t in (q, k, v)]
+        oc = call(*cut, s=inner)
+        grads, grads_c = torch.autograd.grad(o, leaf, do), torch.autograd.grad(oc, cut, do[lo:hi])
+        for a, b in zip((o, *grads), (oc, *grads_c)):
+            assert torch.allclose(a[lo:hi], b, rtol=1e-4, atol=1e-4) and not a[:lo].any() and not a[hi:].any()
+        o = call(*[t.nan_to_num() for t in (q, k, v)], s=torch.tensor([-5, 100, 10 ** 12], device='cuda'))
+        assert torch.isfinite(o).all()
+        none = call(q, k, v, s=torch.tensor([5], device='cuda'))
+        assert not none.any()
+
+
+def test_empty_calls(vad):
+    for lead in ((0, 10), (3, 0)):
+        q, k, v = (torch.empty(*lead, 2, 32, device='cuda', requires_grad=True) for _ in range(3))
+        state = torch.randn(lead[0], 2, 32, 32, device='cuda', requires_grad=True)
+        o, s = vad.linear_attention(q, k, v, _decays(2), state=state)
+        assert o.shape == q.shape and torch.equal(s, state)
+        ds = torch.randn_like(s)
+        assert torch.equal(torch.autograd.grad(s, state, ds)[0], ds)
+        w = vad.window_attention(q, k, v, 5)
+        assert torch.autograd.grad(w, q, torch.empty_like(w))[0].shape == q.shape
+    z = torch.empty(0, 2, 32, device='cuda')
+    assert vad.linear_attention_step(z, z, z, _decays(2), torch.empty(0, 2, 32, 32, device='cuda')).shape == (0, 2, 32)
+    c = torch.empty(0, 6, 2, 32, device='cuda')
+    assert vad.window_attention_step(z, z, z, c, c.clone(), torch.empty(0, dtype=torch.int64, device='cuda'), 6).shape == (0, 2, 32)
+
+
+def test_other_streams_and_graphs(vad):
+    vad.init()
+    g = _gen(11)
+    x = _rand(g, 2, 400, 192, dtype=torch.bfloat16)
+    w, b = torch.ones(192, device='cuda'), torch.zeros(192, device='cuda')
+    log_decay = _decays(3)
+    state, cache = _rand(g, 2, 3, 64, 64), _rand(g, 2, 2, 34, 3, 64, dtype=torch.bfloat16)
+    pos = torch.tensor([5, 70], device='cuda')
+
+    def forward():
+        h = vad.layer_norm(x, w, b).view(2, 400, 3, 64)
+        o, s = vad.linear_attention(h, h, h, log_decay)
+        y = vad.window_attention(h, o, h, 30, 4)
+        st = vad.linear_attention_step(h[:, 0], h[:, 1], h[:, 2], log_decay, s)
+        ct = vad.window_attention_step(h[:, 0], h[:, 1], h[:, 2], cache[:, 0], cache[:, 1], pos, 30, 4)
+        return o, s, y, st, ct
+
+    want = [t.clone() for t in forward()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = forward()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, r) for p, r in zip(got, want))
+
+    leaf = x.view(2, 400, 3, 64).clone().requires_grad_()
+
+    def train():
+        h = vad.layer_norm(leaf)
+        o, _ = vad.linear_attention(h, h, h, log_decay)
+        y = vad.window_attention(o, h, o, 30, 4)
+        return torch.autograd.grad(y, leaf, leaf.detach())[0]
+
+    want_grad = train().clone()
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            forward(), train()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                                     # two graphs alive at once keep to their own scratch
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = forward(), train()
+        graphs.append((graph, out))
+    for turn in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        (torch.randn(1000, device='cuda') * 2).sum().item()
+        for graph, (out, grad) in graphs:
+            assert all(torch.equal(p, r) for p, r in zip(out, want)) and torch.equal(grad, want_grad)
+    torch.cuda.synchronize()
+
+
+def test_a_streaming_model_scores_frames_as_it_scores_the_recording(vad):
+    """The operators together: norm -> linear attention -> norm -> window attention over features of synthetic audio, trained
+    for a gradient over the whole recording, then run frame by frame from where the recording stopped."""
+    torch.manual_seed(0)
+    frames, heads, dim, window, sinks = 160, 3, 30, 30, 2
+    feat = vad.mfcc_delta_stream(vad.synth_stream(0, frames, seed=5), frames)
+    width = heads * dim
+    shapes = [(24, 3 * width), (width, 3 * width), (width, 2)]
+    params = [(torch.randn(s, device='cuda') / s[0] ** 0.5).requires_grad_() for s in shapes]
+    gains = [torch.ones(n, device='cuda', requires_grad=True) for n in (24, width)]
+    shifts = [torch.zeros(n, device='cuda', requires_grad=True) for n in (24, width)]
+    log_decay = _decays(heads)
+
+    def split(x, p):
+        return (x @ p).unflatten(-1, (3, heads, dim)).unbind(-3)
+
+    def model(x, layer_norm, mix, look):
+        h = mix(*split(layer_norm(x, gains[0], shifts[0]), params[0])).flatten(-2)
+        h = h + look(*split(layer_norm(h, gains[1], shifts[1]), params[1])).flatten(-2)
+        return h @ params[2]
+
+    def plain_mix(q, k, v):
+        return torch.stack([ref.decay_sequence(q[0, :, i], k[0, :, i], v[0, :, i], float(a), dim ** -0.5)['o']
+                            for i, a in enumerate(log_decay.clamp(-87.0, 0.0).double())], 1)[None]
+
+    def plain_look(q, k, v):
+        return torch.stack([ref.window_sequence(q[0, :, i], k[0, :, i], v[0, :, i], window, sinks, dim ** -0.5)['o'] for i in range(heads)], 1)[None]
+
+    leaves = params + gains + shifts
+    scores = model(feat[None], vad.layer_norm, lambda *t: vad.linear_attention(*t, log_decay)[0], lambda *t: vad.window_attention(*t, window, sinks))
+    grads = torch.autograd.grad(torch.logsumexp(scores, -1).sum() - scores[..., 1].sum(), leaves)
+    saved = [p.data for p in leaves]
+    for p in leaves:
+        p.data = p.data.double()
+    want = model(feat[None].double(), lambda x, w, b: ref.layer_norm(x, w, b, 1e-5), plain_mix, plain_look)
+    wants = torch.autograd.grad(torch.logsumexp(want, -1).sum() - want[..., 1].sum(), leaves)
+    for p, d in zip(leaves, saved):
+        p.data = d
+    # float32 through two mixers and two norms: thousands of roundings of 2^-24 against the largest value
+    assert float((scores.double() - want).abs().max()) < 1e-3 * float(want.abs().max())
+    for a, b in zip(grads, wants):
+        assert float((a.double() - b).abs().max()) < 1e-3 * float(b.abs().max())
+
+    live, state, cache = 130, {}, {}
+    with torch.no_grad():
+        def start_mix(q, k, v):
+            o, state['s'] = vad.linear_attention(q, k, v, log_decay)
+            return o
+
+        def start_look(q, k, v):
+            cache['k'], cache['v'] = (torch.empty(1, sinks + window, heads, dim, device='cuda') for _ in range(2))
+            cache['pos'] = vad.window_cache_fill(k, v, cache['k'], cache['v'], window, sinks)
+            return vad.window_attention(q, k, v, window, sinks)
+
+        head = model(feat[None, :live], vad.layer_norm, start_mix, start_look)
+        assert torch.allclose(head[0], scores[0, :live], rtol=1e-4, atol=1e-4)
+        for t in range(live, frames):
+            step = model(feat[t:t + 1], vad.layer_norm, lambda *x: vad.linear_attention_step(*x, log_decay, state['s']),
+                         lambda *x: vad.window_attention_step(*x, cache['k'], cache['v'], cache['pos'], window, sinks))
+            cache['pos'] += 1
+            assert torch.allclose(step[0], scores[0, t], rtol=1e-3, atol=1e-3)
+
+
+def test_device_refusals(vad):
+    """Refusals that need device tensors to reach: nothing is launched."""
+    q = torch.zeros(1, 10, 4, 32, device='cuda')
+    ld = torch.zeros(4, device='cuda')
+    bad = [
+        (lambda: vad.layer_norm(q.double()), 'float32 or bfloat16'),
+        (lambda: vad.layer_norm(q, torch.ones(31, device='cuda')), 'shape'),
+        (lambda: vad.layer_norm(q, torch.ones(32, device='cuda'), torch.ones(32, device='cuda').bfloat16()), 'float32'),
+        (lambda: vad.layer_norm(q, eps=float('nan')), 'eps'),
+        (lambda: vad.layer_norm(torch.zeros((), device='cuda')), 'last dimension'),
+        (lambda: vad.linear_attention(q, q, q[:, :9], ld), 'go together'),
+        (lambda: vad.linear_attention(q, q.bfloat16(), q, ld), 'k must be'),
+        (lambda: vad.linear_attention(q, q[:, :, :2], q[:, :, :2], ld), 'query heads'),
+        (lambda: vad.linear_attention(q, q, q, ld[:3]), 'log_decay'),
+        (lambda: vad.linear_attention(q, q, q, ld.requires_grad_()), 'no gradient'),
+        (lambda: vad.linear_attention(q, q, q, torch.zeros(4, device='cuda'), state=torch.zeros(1, 4, 32, 31, device='cuda')), 'state'),
+        (lambda: vad.linear_attention(q, q, q, torch.zeros(4, device='cuda'), scale=float('inf')), 'scale'),
+        (lambda: vad.linear_attention(q, q, q, torch.zeros(4, device='cuda'), starts=torch.zeros(2, dtype=torch.int64, device='cuda')), 'rows, heads'),
+        (lambda: vad.linear_attention(q[0], q[0], q[0], torch.zeros(4, device='cuda'), starts=torch.zeros(2, device='cuda')), 'starts'),
+        (lambda: vad.linear_attention(q[0], q[0], q[0], torch.zeros(4, device='cuda'), starts=torch.zeros(0, dtype=torch.int64, device='cuda')), 'starts'),
+        (lambda: vad.linear_attention_step(q[0], q[0], q[0], torch.zeros(4, device='cuda'), torch.zeros(10, 4, 32, 32, device='cuda').mT), 'contiguous'),
+        (lambda: vad.window_attention(q, q, q, 0), 'window'),
+        (lambda: vad.window_attention(q, q, q, 5, 65), 'sinks'),
+        (lambda: vad.window_attention(q, q, q, 5, scale=-1.0), 'scale'),
+        (lambda: vad.window_attention(q, q[:, :, :3], q[:, :, :3], 5), 'query heads'),
+        (lambda: vad.window_attention(torch.zeros(1, 2, 1, 129, device='cuda'), *[torch.zeros(1, 2, 1, 129, device='cuda')] * 2, 5), 'dim'),
+        (lambda: vad.window_attention_step(q[0], q[0], q[0], *[torch.zeros(10, 6, 4, 32, device='cuda')] * 2, torch.zeros(10, device='cuda'), 5, 1), 'pos'),
+        (lambda: vad.window_attention_step(q[0], q[0], q[0], *[torch.zeros(10, 5, 4, 32, device='cuda')] * 2, torch.zeros(10, dtype=torch.int64, device='cuda'), 5, 1), 'cache_k'),
+        (lambda: vad.window_attention_step(q[0], q[0], q[0], torch.zeros(10, 6, 4, 32, device='cuda'), torch.zeros(1, 6, 4, 32, device='cuda').expand(10, 6, 4, 32),
+                                           torch.zeros(10, dtype=torch.int64, device='cuda'), 5, 1), 'broadcast'),
+    ]
+    for call, needle in bad:
+        with pytest.raises(ValueError, match=needle):
+            call()
+    with pytest.raises(ValueError, match='no gradient'):
+        vad.linear_attention_step(q[0].clone().requires_grad_(), q[0], q[0], torch.zeros(4, device='cuda'), torch.zeros(10, 4, 32, 32, device='cuda'))
+    leaf = q.clone().requires_grad_()
+    first = torch.autograd.grad(vad.layer_norm(leaf).square().sum(), leaf, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), leaf)

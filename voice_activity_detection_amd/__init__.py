@@ -17,10 +17,13 @@ from .generator import DataGenerator
 from .metrics import fix_frr, roc_curve, threshold_sweep
 from .stream import StreamWorkspace, vad_stream
 from .sharding import HALO_FRAMES, all_gather_posteriors, gather_posteriors, shard_plan, shard_range, window_owner_ranges
+from .sequence import (layer_norm, linear_attention, linear_attention_step, window_attention, window_attention_step,
+                       window_cache_fill)
 from .synth import synth_audio, synth_stream
 
 __all__ = ['VadError', 'build', 'init', 'lib', 'Net', 'DenseNet', 'NickNet', 'MODEL_STACK', 'set_matrix_mode', 'process_test_frames', 'process_test_data', 'recording_slices', 'add_noise',
            'overlay', 'overlay_device', 'mfcc_delta_slices', 'mfcc_delta_stream', 'mfcc_delta_ragged', 'process_training_data', 'training_slices', 'vad_stream', 'StreamWorkspace',
            'synth_audio', 'metrics', 'train', 'DataGenerator', 'fix_frr', 'roc_curve', 'threshold_sweep',
+           'layer_norm', 'linear_attention', 'linear_attention_step', 'window_attention', 'window_attention_step', 'window_cache_fill',
            'synth_stream', 'SAMPLE_RATE', 'FRAME_SIZE', 'FRAMES', 'FEATURES', 'BATCH_SIZE', 'SLICE_MAX',
            'ALIGN_FRAMES', 'STEP_SIZE']

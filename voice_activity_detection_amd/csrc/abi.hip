@@ -74,6 +74,10 @@ extern "C" int vad_init(void) {
     if (rc != VAD_OK) return rc;
     rc = vad::ensure_nicknet_attrs();
     if (rc != VAD_OK) return rc;
+    rc = vad::ensure_linear_attention_attrs();
+    if (rc != VAD_OK) return rc;
+    rc = vad::ensure_window_attention_attrs();
+    if (rc != VAD_OK) return rc;
     return vad::ensure_sweep_scratch();
 }
 

@@ -1,0 +1,602 @@
+// Linear attention with a decay per head: the recurrent layer S_t = a S_{t-1} + k_t v_t^T, o_t = s q_t S_t with
+// a = exp(log_decay[head]), over whole sequences in pieces of 64 rows, its backward pass, and one step of it.
+//
+// Within a piece (rows i, j counted from its first row) with H = a S, S the state behind the row before it,
+//   o_i = s a^i q_i H + s sum_{j <= i} a^(i-j) (q_i . k_j) v_j,      H' = a^n H + sum_j a^(n-j) k_j v_j^T
+// so a piece is four small matrix products and the state crosses from piece to piece in the registers of the block
+// that walks along a sequence and head.  The backward pass is the same walk three times over:
+//   dq: (q,k,v) = (do, v, k) forwards, with S transposed;  dk: (v, do, q) backwards;  dv: (k, q, do) backwards
+// the backward walks starting from the gradient of the final state and ending at a times that of the initial state.
+//
+// Where sequences and heads alone do not fill the chip, a sequence is cut into spans walked by blocks of their own: a
+// first launch computes each span's state from k and v alone, a second one joins them along the sequence, and the
+// walk of every span starts from its joined state.
+//
+// Wave w of a block owns columns 16 w .. 16 w + 15 of the state and of the outputs.  The state stays in float32; for
+// bfloat16 inputs its update multiplies v by the decay in float32 and splits the product exactly into three bfloat16
+// terms, so the state has float32's accuracy; the weights a^(i-j) (q . k) and the copy of the state that q is
+// multiplied with are rounded to bfloat16 once.
+
+#include <mutex>
+
+#include "sequence_device.h"
+
+namespace vad {
+namespace {
+using namespace sq;
+
+constexpr int kPiece = 64;
+
+template <typename T>
+struct Walk {
+    Heads<const T> q, k, v;
+    T* o;                              // rows of heads * dim
+    const float* s0;                   // initial state (n_seq, heads, dim, dim) or null
+    float* s1;                         // final state or null
+    float within, across, update;      // factors of the piece's own products, of q H, and of k v^T
+    bool s0_transposed, reverse;
+};
+
+template <typename T>
+struct WalkArgs {
+    Walk<T> walk[3];
+    Sequences seq;
+    const float* log_decay;
+    float* spans;                      // [walk][seq][head][span][dim][dim]
+    int n_seq, heads, dim, n_spans;
+    bool wide, wide_out;
+};
+
+__device__ __forceinline__ float log2_decay(float ld) {
+    // not validated on the host (it lives on the device): a growing state or one past float32 is cut off, NaN stays
+    ld = ld > 0.0f ? 0.0f : (ld < -87.0f ? -87.0f : ld);
+    return ld * kLog2e;
+}
+__device__ __forceinline__ float power(float l2, float n) { return __builtin_amdgcn_exp2f(l2 * n); }
+
+// rows of a span: sequences shorter than the hint are cut just as evenly
+__device__ __forceinline__ int64_t span_rows(int64_t len, int n_spans) {
+    const int64_t per = (len + n_spans - 1) / n_spans;
+    return per <= kPiece ? kPiece : (per + kPiece - 1) / kPiece * kPiece;
+}
+
+template <typename T, int DP>
+struct WalkShape {
+    static constexpr int kWaves = DP / 16;
+    static constexpr int kThreads = kWaves * 64;
+    static constexpr int kLd = DP + Elem<T>::kPer16B;
+    static constexpr int kLdP = kPiece + Elem<T>::kPer16B;
+    static constexpr int kPieces = kPiece * DP / Elem<T>::kPer16B / kThreads;       // 16-byte pieces a thread stages
+    static constexpr size_t kLds = (size_t)(3 * kPiece * kLd + kPiece * kLdP) * sizeof(T) + 16;
+};
+
+// The (row block, key block) pairs of a piece's weights: the lower triangle, and the two blocks above it that share a
+// contraction of 32 keys with a diagonal block and must read as zero.
+__device__ const signed char kPairs[12][2] = {{0, 0}, {1, 0}, {1, 1}, {2, 0}, {2, 1}, {2, 2}, {3, 0}, {3, 1}, {3, 2}, {3, 3}, {0, 1}, {2, 3}};
+
+// float32 values as the sum of three bfloat16 (24 bits); not-finite values in the first term alone
+__device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&f)[3]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const __bf16 hi = (__bf16)x[j];
+        const float r = fabsf(x[j]) < INFINITY ? x[j] - (float)hi : 0.0f;
+        const __bf16 mid = (__bf16)r;
+        f[0][j] = hi;
+        f[1][j] = mid;
+        f[2][j] = (__bf16)(r - (float)mid);
+    }
+}
+
+template <typename T, int DP, bool STATE>
+__global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
+    using C = WalkShape<T, DP>;
+    extern __shared__ char lds_raw[];
+    T* sk = reinterpret_cast<T*>(lds_raw);
+    T* sv = sk + kPiece * C::kLd;
+    T* sq_ = sv + kPiece * C::kLd;
+    T* sp = sq_ + kPiece * C::kLd;
+    int* flags = reinterpret_cast<int*>(sp + kPiece * C::kLdP);
+
+    const int h = blockIdx.x % a.heads;
+    const int span = (blockIdx.x / a.heads) % a.n_spans;
+    const int s = blockIdx.x / a.heads / a.n_spans;
+    const Walk<T> w = a.walk[blockIdx.y];
+    int64_t first, len;
+    sequence_rows(a.seq, s, first, len);
+    const int dim = a.dim;
+    if (!STATE) zero_outside(w.o, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, span, a.n_spans);
+    const int64_t per = span_rows(len, a.n_spans);
+    const int64_t t0 = span * per, t1 = t0 + per < len ? t0 + per : len;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int64_t head = (int64_t)s * a.heads + h, elems = (int64_t)dim * dim;
+    float* spans = a.spans ? a.spans + (((int64_t)blockIdx.y * a.n_seq * a.heads + head) * a.n_spans + span) * elems : nullptr;
+    if (STATE) {
+        if (t0 >= len || t1 == len) return;        // the last span's own state is not needed
+    } else if (len == 0 && span == 0) {
+        if (w.s1)
+            for (int64_t i = threadIdx.x; i < elems; i += C::kThreads) w.s1[head * elems + i] = w.s0 ? w.s0[head * elems + i] : 0.0f;
+        return;
+    } else if (t0 >= len) {
+        return;
+    }
+    const float l2 = log2_decay(a.log_decay[h]);
+
+    // H: block b holds rows 16 b + 4 g + i, column 16 wave + c
+    f32x4 H[DP / 16];
+    const int col = 16 * wave + c;
+#pragma unroll
+    for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * b + 4 * g + i;
+            float x = 0.0f;
+            if (!STATE && row < dim && col < dim) {
+                if (a.n_spans > 1)
+                    x = spans[row * dim + col];
+                else if (w.s0)
+                    x = w.s0[head * elems + (w.s0_transposed ? col * dim + row : row * dim + col)] * (w.reverse ? 1.0f : power(l2, 1.0f));
+            }
+            H[b][i] = x;
+        }
+
+    const T* kp = head_ptr(w.k, a.seq, s, first, h);
+    const T* vp = head_ptr(w.v, a.seq, s, first, h);
+    const T* qp = STATE ? nullptr : head_ptr(w.q, a.seq, s, first, h);
+    T* op = w.o + ((a.seq.starts ? first : (int64_t)s * a.seq.max_len) * a.heads + h) * dim;
+    constexpr int PPR = DP / Elem<T>::kPer16B;
+    u32x4 rk[C::kPieces], rv[C::kPieces], rq[C::kPieces];
+    auto fetch = [&](int64_t tc) {
+#pragma unroll
+        for (int n = 0; n < C::kPieces; ++n) {
+            const int p = threadIdx.x + n * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B;
+            rk[n] = rv[n] = rq[n] = u32x4{0, 0, 0, 0};
+            if (tc + row < t1) {
+                const int64_t at = w.reverse ? len - 1 - (tc + row) : tc + row;
+                rk[n] = load_piece(kp + at * w.k.st, pc, dim, a.wide);
+                rv[n] = load_piece(vp + at * w.v.st, pc, dim, a.wide);
+                if (!STATE) rq[n] = load_piece(qp + at * w.q.st, pc, dim, a.wide);
+            }
+        }
+    };
+    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+    fetch(t0);
+    __syncthreads();
+    int turn = 0;
+    for (int64_t tc = t0; tc < t1; tc += kPiece, turn ^= 1) {
+        const int n = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < C::kPieces; ++i) {
+            const int p = threadIdx.x + i * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B;
+            *reinterpret_cast<u32x4*>(sk + row * C::kLd + pc) = rk[i];
+            *reinterpret_cast<u32x4*>(sv + row * C::kLd + pc) = rv[i];
+            if (!STATE) {
+                *reinterpret_cast<u32x4*>(sq_ + row * C::kLd + pc) = rq[i];
+                bad |= piece_not_finite<T>(rv[i]);
+            }
+        }
+        if (bad) flags[turn] = 1;
+        __syncthreads();
+        const bool careful = !STATE && flags[turn];
+        if (threadIdx.x == 0) flags[turn ^ 1] = 0;
+        if (tc + kPiece < t1) fetch(tc + kPiece);
+
+        f32x4 o[4];
+        if (!STATE) {
+            // weights of the piece: rows in columns of the tile, keys 16 kb + 4 g + i down its lanes
+            for (int t = wave; t < 12; t += C::kWaves) {
+                const int rb = kPairs[t][0], kb = kPairs[t][1];
+                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (kb <= rb) {
+#pragma unroll
+                    for (int d = 0; d < DP; d += 32)
+                        acc = mma(frag_natural(sk, C::kLd, 16 * kb, d), frag_natural(sq_, C::kLd, 16 * rb, d), acc);
+                    const int gap = 16 * (rb - kb) + c - 4 * g;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[i] = gap >= i ? acc[i] * (w.within * power(l2, (float)(gap - i))) : 0.0f;
+                }
+                Quad<T> p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = (T)acc[i];
+                *reinterpret_cast<Quad<T>*>(sp + (16 * rb + c) * C::kLdP + 16 * kb + 4 * g) = p;
+            }
+            // q H, transposed: outputs 16 wave + 4 g + i of row 16 rb + c
+            Frag<T> hf[DP / 32];
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) to_frag(H[2 * d], H[2 * d + 1], hf[d]);
+#pragma unroll
+            for (int rb = 0; rb < 4; ++rb) {
+                o[rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) o[rb] = mma(hf[d], frag_split(sq_, C::kLd, 16 * rb, 32 * d), o[rb]);
+                o[rb] *= w.across * power(l2, (float)(16 * rb + c));
+            }
+        }
+        Frag<T> vf[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) vf[t] = frag_columns(sv, C::kLd, 32 * t, 16 * wave);
+
+        // the state behind the piece
+        const bool last = tc + kPiece >= t1;
+        const bool finish = !STATE && last && t1 == len && w.s1;
+        if (!last || STATE || finish) {
+            const float less = finish && !w.reverse ? 1.0f : 0.0f;       // the forward walk hands out S, not a S
+            const float keep = power(l2, (float)n - less);
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) H[b] *= keep;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int row = 32 * t + 4 * g + (j < 4 ? j : 12 + j);
+                    x[j] = row < n ? (float)vf[t][j] * (w.update * power(l2, (float)(n - row) - less)) : 0.0f;
+                }
+                if constexpr (sizeof(T) == 2) {
+                    bf16x8 f[3];
+                    split3(x, f);
+#pragma unroll
+                    for (int b = 0; b < DP / 16; ++b) {
+                        const bf16x8 kf = frag_columns(sk, C::kLd, 32 * t, 16 * b);
+#pragma unroll
+                        for (int m = 2; m >= 0; --m) H[b] = mma(kf, f[m], H[b]);
+                    }
+                } else {
+                    f32x8 f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[j] = x[j];
+#pragma unroll
+                    for (int b = 0; b < DP / 16; ++b) H[b] = mma(frag_columns(sk, C::kLd, 32 * t, 16 * b), f, H[b]);
+                }
+            }
+        }
+        if (!STATE) {
+            __syncthreads();
+            if (!careful) {
+#pragma unroll
+                for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+                    for (int t = 0; t <= rb / 2; ++t) o[rb] = mma(vf[t], frag_split(sp, C::kLdP, 16 * rb, 32 * t), o[rb]);
+            } else {
+                // an infinity or NaN among the piece's v: a matrix product would carry it (0 * inf) to the rows before it
+#pragma unroll
+                for (int rb = 0; rb < 4; ++rb)
+                    for (int key = 0; key <= 16 * rb + c && key < n; ++key)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o[rb][i] = fmaf((float)sp[(16 * rb + c) * C::kLdP + key], (float)sv[key * C::kLd + 16 * wave + 4 * g + i], o[rb][i]);
+            }
+#pragma unroll
+            for (int rb = 0; rb < 4; ++rb) {
+                const int row = 16 * rb + c;
+                if (row < n) {
+                    const int64_t at = w.reverse ? len - 1 - (tc + row) : tc + row;
+                    store_quad(op + at * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], a.wide_out);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    float* out = STATE ? spans : (t1 == len && w.s1 ? w.s1 + head * elems : nullptr);
+    if (out) {
+#pragma unroll
+        for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * b + 4 * g + i;
+                if (row < dim && col < dim) out[row * dim + col] = H[b][i];
+            }
+    }
+}
+
+// spans[u] on entry: the state that span u alone leaves; on return: the state that span u starts from.
+template <typename T>
+__global__ __launch_bounds__(256) void decay_join_kernel(WalkArgs<T> a) {
+    const int64_t elems = (int64_t)a.dim * a.dim, blocks = (elems + 255) / 256;
+    const int64_t head = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
+    const int h = head % a.heads, s = head / a.heads;
+    const Walk<T> w = a.walk[blockIdx.y];
+    int64_t first, len;
+    sequence_rows(a.seq, s, first, len);
+    if (e >= elems || len == 0) return;
+    const int64_t per = span_rows(len, a.n_spans), used = (len + per - 1) / per;
+    const float l2 = log2_decay(a.log_decay[h]), keep = power(l2, (float)per);
+    float x = 0.0f;
+    if (w.s0) x = w.s0[head * elems + (w.s0_transposed ? e % a.dim * a.dim + e / a.dim : e)] * (w.reverse ? 1.0f : power(l2, 1.0f));
+    float* p = a.spans + (((int64_t)blockIdx.y * a.n_seq * a.heads + head) * a.n_spans) * elems + e;
+    for (int64_t u = 0; u < used; ++u, p += elems) {
+        const float own = u + 1 < used ? *p : 0.0f;
+        *p = x;
+        x = fmaf(x, keep, own);
+    }
+}
+
+// One step: the state is read, updated and written once.  A block owns 32 columns of one state, VE of them per thread,
+// the rows dealt to 8 VE groups of threads.
+template <typename T, int VE>
+__global__ __launch_bounds__(256) void decay_step_kernel(Heads<const T> q, Heads<const T> k, Heads<const T> v, const float* __restrict__ log_decay,
+                                                         float scale, int heads, int dim, int slices, float* __restrict__ state, T* __restrict__ o) {
+    typedef float vec __attribute__((ext_vector_type(VE == 1 ? 2 : VE)));
+    constexpr int kLanes = 32 / VE, kGroups = 256 / kLanes;
+    __shared__ float sums[4][32];
+    const int64_t head = blockIdx.x / slices;
+    const int h = head % heads, b = head / heads;
+    const int c = blockIdx.x % slices * 32 + threadIdx.x % kLanes * VE, group = threadIdx.x / kLanes;
+    const float a = __builtin_amdgcn_exp2f(log2_decay(log_decay[h]));
+    const T* qp = q.p + b * q.sb + h * q.sh;
+    const T* kp = k.p + b * k.sb + h * k.sh;
+    const T* vp = v.p + b * v.sb + h * v.sh;
+    float vv[VE], acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        vv[e] = c + e < dim ? (float)vp[c + e] : 0.0f;
+        acc[e] = 0.0f;
+    }
+    float* sp = state + head * dim * dim + c;
+    if (c < dim) {
+#pragma unroll 4
+        for (int row = group; row < dim; row += kGroups) {
+            const float kk = (float)kp[row], qq = (float)qp[row];
+            float x[VE];
+            if (VE == 1) {
+                x[0] = sp[row * dim];
+            } else {
+                const vec r = *reinterpret_cast<const vec*>(sp + row * dim);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) x[e] = r[e];
+            }
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                x[e] = fmaf(x[e], a, kk * vv[e]);
+                acc[e] = fmaf(qq, x[e], acc[e]);
+            }
+            if (VE == 1) {
+                sp[row * dim] = x[0];
+            } else {
+                vec r;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) r[e] = x[e];
+                *reinterpret_cast<vec*>(sp + row * dim) = r;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        for (int d = kLanes; d < 64; d <<= 1) acc[e] += __shfl_xor(acc[e], d);
+        if ((int)(threadIdx.x & 63) < kLanes) sums[threadIdx.x >> 6][threadIdx.x % kLanes * VE + e] = acc[e];
+    }
+    __syncthreads();
+    const int t = threadIdx.x, oc = blockIdx.x % slices * 32 + t;
+    if (t < 32 && oc < dim) o[head * dim + oc] = (T)(scale * ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])));
+}
+
+// Spans per sequence: enough blocks to fill the chip, spans of at least four pieces.
+int span_count(int64_t n_seq, int64_t max_len, int64_t heads, int walks) {
+    const int64_t blocks = n_seq * heads * walks, want = 768;
+    int64_t n = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    const int64_t most = max_len / (4 * kPiece);
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n);
+}
+
+template <typename T>
+int allow_walks() {
+    const void* f[] = {reinterpret_cast<const void*>(&decay_walk_kernel<T, 32, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 32, true>),
+                       reinterpret_cast<const void*>(&decay_walk_kernel<T, 64, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 64, true>),
+                       reinterpret_cast<const void*>(&decay_walk_kernel<T, 128, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 128, true>)};
+    const size_t lds[] = {WalkShape<T, 32>::kLds, WalkShape<T, 64>::kLds, WalkShape<T, 128>::kLds};
+    for (int i = 0; i < 6; ++i) VAD_HIP_CHECK(hipFuncSetAttribute(f[i], hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds[i / 2]));
+    return VAD_OK;
+}
+
+template <typename T, int DP, bool STATE>
+void launch_walk(const WalkArgs<T>& a, int walks, hipStream_t st) {
+    hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE>), dim3((unsigned)(a.n_seq * a.heads * a.n_spans), (unsigned)walks),
+                       dim3((WalkShape<T, DP>::kThreads)), (WalkShape<T, DP>::kLds), st, a);
+}
+template <typename T, bool STATE>
+void launch_walk(const WalkArgs<T>& a, int walks, hipStream_t st) {
+    if (a.dim <= 32)
+        launch_walk<T, 32, STATE>(a, walks, st);
+    else if (a.dim <= 64)
+        launch_walk<T, 64, STATE>(a, walks, st);
+    else
+        launch_walk<T, 128, STATE>(a, walks, st);
+}
+
+template <typename T>
+int run_walks(const WalkArgs<T>& a, int walks, hipStream_t st) {
+    if (a.n_spans > 1) {
+        launch_walk<T, true>(a, walks, st);
+        VAD_HIP_CHECK(hipGetLastError());
+        const int64_t blocks = ((int64_t)a.dim * a.dim + 255) / 256 * a.n_seq * a.heads;
+        hipLaunchKernelGGL((decay_join_kernel<T>), dim3((unsigned)blocks, (unsigned)walks), dim3(256), 0, st, a);
+        VAD_HIP_CHECK(hipGetLastError());
+    }
+    launch_walk<T, false>(a, walks, st);
+    VAD_HIP_CHECK(hipGetLastError());
+    return VAD_OK;
+}
+
+template <typename T>
+Heads<const T> heads_of(const void* p, const int64_t* strides) {
+    return {static_cast<const T*>(p), strides[0], strides[1], strides[2]};
+}
+template <typename T>
+bool wide_rows(const Heads<const T>& x, int dim) {
+    constexpr int VE = Elem<T>::kPer16B;
+    return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.sb % VE == 0 && x.st % VE == 0 && x.sh % VE == 0 && dim % VE == 0;
+}
+template <typename T>
+bool wide_quads(const T* p, int dim) {
+    return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && dim % 4 == 0;
+}
+
+template <typename T>
+int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, Sequences seq,
+                int n_seq, int heads, int dim, const float* log_decay, float scale, const float* s0, void* o, float* s1, int n_spans,
+                float* ws, hipStream_t st) {
+    WalkArgs<T> a = {};
+    a.walk[0] = {heads_of<T>(q, qs), heads_of<T>(k, ks), heads_of<T>(v, vs), static_cast<T*>(o), s0, s1, scale, scale, 1.0f, false, false};
+    a.seq = seq;
+    a.log_decay = log_decay;
+    a.spans = n_spans > 1 ? ws : nullptr;
+    a.n_seq = n_seq;
+    a.heads = heads;
+    a.dim = dim;
+    a.n_spans = n_spans;
+    a.wide = wide_rows(a.walk[0].q, dim) && wide_rows(a.walk[0].k, dim) && wide_rows(a.walk[0].v, dim);
+    a.wide_out = wide_quads(static_cast<const T*>(o), dim);
+    return run_walks(a, 1, st);
+}
+
+template <typename T>
+int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* g,
+                 const int64_t* gs, Sequences seq, int n_seq, int heads, int dim, const float* log_decay, float scale, const float* s0,
+                 const float* ds1, void* dq, void* dk, void* dv, float* ds0, int n_spans, float* ws, hipStream_t st) {
+    const Heads<const T> Q = heads_of<T>(q, qs), K = heads_of<T>(k, ks), V = heads_of<T>(v, vs), G = heads_of<T>(g, gs);
+    WalkArgs<T> a = {};
+    a.walk[0] = {G, V, K, static_cast<T*>(dq), s0, nullptr, scale, scale, 1.0f, true, false};
+    a.walk[1] = {V, G, Q, static_cast<T*>(dk), ds1, nullptr, scale, 1.0f, scale, true, true};
+    a.walk[2] = {K, Q, G, static_cast<T*>(dv), ds1, ds0, scale, 1.0f, scale, false, true};
+    a.seq = seq;
+    a.log_decay = log_decay;
+    a.spans = n_spans > 1 ? ws : nullptr;
+    a.n_seq = n_seq;
+    a.heads = heads;
+    a.dim = dim;
+    a.n_spans = n_spans;
+    a.wide = wide_rows(Q, dim) && wide_rows(K, dim) && wide_rows(V, dim) && wide_rows(G, dim);
+    a.wide_out = wide_quads(static_cast<const T*>(dq), dim) && wide_quads(static_cast<const T*>(dk), dim) && wide_quads(static_cast<const T*>(dv), dim);
+    return run_walks(a, 3, st);
+}
+
+int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int dim, int dtype) {
+    VAD_REQUIRE(dtype == VAD_DTYPE_F32 || dtype == VAD_DTYPE_BF16, "dtype must be VAD_DTYPE_F32 or VAD_DTYPE_BF16, got %d", dtype);
+    VAD_REQUIRE(dim >= 1 && dim <= VAD_MAX_HEAD_DIM, "head dimension %d out of range 1..%d", dim, VAD_MAX_HEAD_DIM);
+    VAD_REQUIRE(heads >= 1, "heads must be positive, got %d", heads);
+    VAD_REQUIRE(n_seq >= 0 && n_tokens >= 0 && max_len >= 0, "negative sequence count or length");
+    VAD_REQUIRE(n_seq <= 0x7FFFFFFF / heads / 64, "too many sequences for one launch");
+    return VAD_OK;
+}
+
+}  // namespace
+
+// The float32 walks of 33 and more columns use more than 64 KB of LDS: opt in once per device.
+int ensure_linear_attention_attrs() {
+    static std::mutex mu;
+    static bool done[64] = {false};
+    int dev = 0;
+    VAD_HIP_CHECK(hipGetDevice(&dev));
+    VAD_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev]) return VAD_OK;
+    int rc = allow_walks<float>();
+    if (rc != VAD_OK) return rc;
+    rc = allow_walks<__bf16>();
+    if (rc != VAD_OK) return rc;
+    done[dev] = true;
+    return VAD_OK;
+}
+}  // namespace vad
+
+extern "C" size_t vad_linear_attention_workspace_bytes(int64_t n_seq, int64_t max_len, int heads, int dim, int backward) {
+    using namespace vad;
+    if (n_seq <= 0 || max_len <= 0 || heads <= 0 || dim <= 0) return 0;
+    const int walks = backward ? 3 : 1, spans = span_count(n_seq, max_len, heads, walks);
+    return spans > 1 ? (size_t)walks * n_seq * heads * spans * dim * dim * sizeof(float) : 0;
+}
+
+extern "C" int vad_linear_attention_forward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                            const void* v_dev, const int64_t* v_strides, const int64_t* starts_dev, int64_t n_seq,
+                                            int64_t n_tokens, int64_t max_len, int heads, int dim, int dtype,
+                                            const float* log_decay_dev, float scale, const float* state_in_dev, void* o_dev,
+                                            float* state_out_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+    using namespace vad;
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype);
+    if (rc != VAD_OK) return rc;
+    VAD_REQUIRE(q_strides && k_strides && v_strides && log_decay_dev, "null pointer argument");
+    if (n_seq == 0) return VAD_OK;
+    const bool empty = starts_dev ? n_tokens == 0 : max_len == 0;
+    VAD_REQUIRE(empty || (q_dev && k_dev && v_dev && o_dev), "null pointer argument");
+    VAD_REQUIRE(!state_in_dev || state_in_dev != state_out_dev, "state_out must not be state_in");
+    const size_t need = vad_linear_attention_workspace_bytes(n_seq, max_len, heads, dim, 0);
+    VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
+    rc = ensure_linear_attention_attrs();
+    if (rc != VAD_OK) return rc;
+    const int spans = span_count(n_seq, max_len, heads, 1);
+    const Sequences seq = {starts_dev, n_tokens, max_len};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float* ws = static_cast<float*>(workspace_dev);
+    return dtype == VAD_DTYPE_F32
+               ? run_forward<float>(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, seq, (int)n_seq, heads, dim, log_decay_dev,
+                                    scale, state_in_dev, o_dev, state_out_dev, spans, ws, st)
+               : run_forward<__bf16>(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, seq, (int)n_seq, heads, dim, log_decay_dev,
+                                     scale, state_in_dev, o_dev, state_out_dev, spans, ws, st);
+}
+
+extern "C" int vad_linear_attention_backward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                             const void* v_dev, const int64_t* v_strides, const void* do_dev, const int64_t* do_strides,
+                                             const int64_t* starts_dev, int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads,
+                                             int dim, int dtype, const float* log_decay_dev, float scale, const float* state_in_dev,
+                                             const float* dstate_out_dev, void* dq_dev, void* dk_dev, void* dv_dev,
+                                             float* dstate_in_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+    using namespace vad;
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype);
+    if (rc != VAD_OK) return rc;
+    VAD_REQUIRE(q_strides && k_strides && v_strides && do_strides && log_decay_dev, "null pointer argument");
+    if (n_seq == 0) return VAD_OK;
+    const bool empty = starts_dev ? n_tokens == 0 : max_len == 0;
+    VAD_REQUIRE(empty || (q_dev && k_dev && v_dev && do_dev && dq_dev && dk_dev && dv_dev), "null pointer argument");
+    VAD_REQUIRE(!dstate_out_dev || dstate_out_dev != dstate_in_dev, "dstate_in must not be dstate_out");
+    const size_t need = vad_linear_attention_workspace_bytes(n_seq, max_len, heads, dim, 1);
+    VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
+    rc = ensure_linear_attention_attrs();
+    if (rc != VAD_OK) return rc;
+    const int spans = span_count(n_seq, max_len, heads, 3);
+    const Sequences seq = {starts_dev, n_tokens, max_len};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float* ws = static_cast<float*>(workspace_dev);
+    return dtype == VAD_DTYPE_F32
+               ? run_backward<float>(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, do_dev, do_strides, seq, (int)n_seq, heads,
+                                     dim, log_decay_dev, scale, state_in_dev, dstate_out_dev, dq_dev, dk_dev, dv_dev, dstate_in_dev,
+                                     spans, ws, st)
+               : run_backward<__bf16>(q_dev, q_strides, k_dev, k_strides, v_dev, v_strides, do_dev, do_strides, seq, (int)n_seq, heads,
+                                      dim, log_decay_dev, scale, state_in_dev, dstate_out_dev, dq_dev, dk_dev, dv_dev, dstate_in_dev,
+                                      spans, ws, st);
+}
+
+extern "C" int vad_linear_attention_step(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                         const void* v_dev, const int64_t* v_strides, int64_t batch, int heads, int dim, int dtype,
+                                         const float* log_decay_dev, float scale, float* state_dev, void* o_dev, void* stream) {
+    using namespace vad;
+    int rc = check_heads(batch, 0, 0, heads, dim, dtype);
+    if (rc != VAD_OK) return rc;
+    if (batch == 0) return VAD_OK;
+    VAD_REQUIRE(q_dev && k_dev && v_dev && q_strides && k_strides && v_strides && log_decay_dev && state_dev && o_dev, "null pointer argument");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int slices = (dim + 31) / 32;
+    const dim3 grid((unsigned)(batch * heads * slices));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(state_dev);
+    const int ve = dim % 4 == 0 && at % 16 == 0 ? 4 : (dim % 2 == 0 && at % 8 == 0 ? 2 : 1);
+    // strides here are (batch, head): Heads' row stride is not used
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) T;
+        const Heads<const T> q = {static_cast<const T*>(q_dev), q_strides[0], 0, q_strides[1]};
+        const Heads<const T> k = {static_cast<const T*>(k_dev), k_strides[0], 0, k_strides[1]};
+        const Heads<const T> v = {static_cast<const T*>(v_dev), v_strides[0], 0, v_strides[1]};
+        T* o = static_cast<T*>(o_dev);
+        if (ve == 4)
+            hipLaunchKernelGGL((decay_step_kernel<T, 4>), grid, dim3(256), 0, st, q, k, v, log_decay_dev, scale, heads, dim, slices, state_dev, o);
+        else if (ve == 2)
+            hipLaunchKernelGGL((decay_step_kernel<T, 2>), grid, dim3(256), 0, st, q, k, v, log_decay_dev, scale, heads, dim, slices, state_dev, o);
+        else
+            hipLaunchKernelGGL((decay_step_kernel<T, 1>), grid, dim3(256), 0, st, q, k, v, log_decay_dev, scale, heads, dim, slices, state_dev, o);
+    };
+    if (dtype == VAD_DTYPE_F32)
+        run(0.0f);
+    else
+        run((__bf16)0.0f);
+    VAD_HIP_CHECK(hipGetLastError());
+    return VAD_OK;
+}

@@ -1,0 +1,249 @@
+// Shared device code of the sequence operators (layer norm, linear attention, window attention): element types,
+// 16x16 matrix tiles, and the staging of rows into LDS.
+//
+// One fragment type serves both element types.  A fragment is a lane's eight values of a 16 x 32 operand: lane 16 g + c
+// holds row (or column) c and eight of the 32 contraction indices.  bfloat16 takes it in one v_mfma_f32_16x16x32_bf16;
+// float32 in eight v_mfma_f32_16x16x4_f32, the j-th of which contracts the j-th value of every lane.  A product only
+// needs both operands to use the same order of the contraction indices, and there are two:
+//   natural   lane group g holds indices 8 g + j
+//   split     lane group g holds 4 g + j (j < 4) and 16 + 4 g + j - 4 (j >= 4): the order in which two 16x16 result
+//             tiles stacked along the contraction leave their values in the lanes, so that a result becomes the next
+//             product's operand without leaving its registers.
+// A result tile (float4 per lane) holds column c and rows 4 g + i.
+#pragma once
+#include <math.h>
+
+#include "vad_internal.h"
+
+namespace vad {
+namespace sq {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    typedef f32x8 Frag;
+    typedef f32x4 Quad;
+    static constexpr int kPer16B = 4;
+};
+template <>
+struct Elem<__bf16> {
+    typedef bf16x8 Frag;
+    typedef bf16x4 Quad;
+    static constexpr int kPer16B = 8;
+};
+template <typename T>
+using Frag = typename Elem<T>::Frag;
+template <typename T>
+using Quad = typename Elem<T>::Quad;
+
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 63); }
+
+// ---- rows in global memory ----
+
+// A tensor of heads over packed or padded sequences; strides in elements, the last dimension is dense.
+template <typename T>
+struct Heads {
+    T* p;
+    int64_t sb, st, sh;
+};
+
+// The rows of sequence s: row t at p + t * st, t < len.  starts == nullptr: len = max_len rows at s * sb.  Otherwise rows
+// starts[s] .. starts[s + 1] - 1 of a packed tensor of n_tokens rows; the table is not trusted: both ends are clamped.
+struct Sequences {
+    const int64_t* starts;
+    int64_t n_tokens, max_len;
+};
+__device__ __forceinline__ void sequence_rows(const Sequences& q, int s, int64_t& first, int64_t& len) {
+    if (!q.starts) {
+        first = 0;
+        len = q.max_len;
+        return;
+    }
+    int64_t lo = q.starts[s], hi = q.starts[s + 1];
+    lo = lo < 0 ? 0 : (lo > q.n_tokens ? q.n_tokens : lo);
+    hi = hi < lo ? lo : (hi > q.n_tokens ? q.n_tokens : hi);
+    first = lo;
+    len = hi - lo;
+}
+// Rows of a packed output of `width` elements a row that lie before the first sequence or behind the last one become
+// zero: columns c0 .. c0 + cols - 1, by the blocks of the first and the last sequence; `part` of `parts` blocks of each.
+template <typename T>
+__device__ __forceinline__ void zero_outside(T* out, int64_t width, int c0, int cols, const Sequences& q, int s, int n_seq, int part, int parts) {
+    if (!q.starts || (s != 0 && s != n_seq - 1)) return;
+    int64_t lo = q.starts[0], hi = q.starts[n_seq];
+    lo = lo < 0 ? 0 : (lo > q.n_tokens ? q.n_tokens : lo);
+    hi = hi < lo ? lo : (hi > q.n_tokens ? q.n_tokens : hi);
+    if (s == 0)
+        for (int64_t i = (int64_t)part * blockDim.x + threadIdx.x; i < lo * cols; i += (int64_t)parts * blockDim.x)
+            out[i / cols * width + c0 + i % cols] = (T)0.0f;
+    if (s == n_seq - 1)
+        for (int64_t i = (int64_t)part * blockDim.x + threadIdx.x; i < (q.n_tokens - hi) * cols; i += (int64_t)parts * blockDim.x)
+            out[(hi + i / cols) * width + c0 + i % cols] = (T)0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ T* head_ptr(const Heads<T>& x, const Sequences& q, int s, int64_t first, int h) {
+    return x.p + (q.starts ? first * x.st : (int64_t)s * x.sb) + (int64_t)h * x.sh;
+}
+
+// 16 bytes of a row from column c; columns from `cols` on read as zero.  `wide`: rows start 16-byte aligned and cols is
+// a multiple of a 16-byte piece (uniform over the launch).
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, bool wide) {
+    constexpr int VE = Elem<T>::kPer16B;
+    u32x4 r = {0, 0, 0, 0};
+    if (wide) {
+        if (c < cols) r = *reinterpret_cast<const u32x4*>(row + c);
+    } else {
+        T v[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
+        __builtin_memcpy(&r, v, 16);
+    }
+    return r;
+}
+
+// Whether any of the values in a 16-byte piece is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool piece_not_finite(u32x4 v) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4)
+            bad |= (v[i] & 0x7F800000u) == 0x7F800000u;
+        else
+            bad |= (v[i] & 0x7F800000u) == 0x7F800000u || (v[i] & 0x7F80u) == 0x7F80u;
+    }
+    return bad;
+}
+
+// A natural-order fragment straight from global memory: this lane's row, columns c .. c + 7.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_row_frag(const T* row, bool live, int c, int cols, bool wide) {
+    Frag<T> f;
+    u32x4 v[sizeof(Frag<T>) / 16];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Frag<T>) / 16); ++i) {
+        v[i] = u32x4{0, 0, 0, 0};
+        if (live) v[i] = load_piece(row, c + i * Elem<T>::kPer16B, cols, wide);
+    }
+    __builtin_memcpy(&f, v, sizeof(f));
+    return f;
+}
+
+// ---- fragments from LDS ----
+
+// Lane c: row r0 + c, columns c0 + 8 g + j.
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_natural(const T* tile, int ld, int r0, int c0) {
+    const int l = lane_id();
+    const T* p = tile + (r0 + (l & 15)) * ld + c0 + 8 * (l >> 4);
+    Frag<T> f;
+    if (sizeof(T) == 2) {
+        f = *reinterpret_cast<const Frag<T>*>(p);
+    } else {
+        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f[j] = a[j];
+            f[j + 4] = b[j];
+        }
+    }
+    return f;
+}
+
+// Lane c: row r0 + c, columns c0 + (4 g + j | 16 + 4 g + j - 4).
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_split(const T* tile, int ld, int r0, int c0) {
+    const int l = lane_id();
+    const T* p = tile + (r0 + (l & 15)) * ld + c0 + 4 * (l >> 4);
+    const Quad<T> a = *reinterpret_cast<const Quad<T>*>(p), b = *reinterpret_cast<const Quad<T>*>(p + 16);
+    Frag<T> f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[j] = a[j];
+        f[j + 4] = b[j];
+    }
+    return f;
+}
+
+// Transposed: lane c: column c0 + c, rows r0 + (4 g + j | 16 + 4 g + j - 4).  The 16-bit form uses the LDS read that
+// transposes a 4 x 16 block within each group of 16 lanes (lane i supplies the address of row i >> 2, columns
+// 4 (i & 3) .. + 3 and receives column i of the four rows).
+__device__ __forceinline__ bf16x8 frag_columns(const __bf16* tile, int ld, int r0, int c0) {
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    const int l = lane_id();
+    const __bf16* p = tile + (r0 + 4 * (l >> 4) + ((l >> 2) & 3)) * ld + c0 + 4 * (l & 3);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 16 * ld));
+    bf16x8 f;
+    __builtin_memcpy(&f, &a, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &b, 8);
+    return f;
+}
+__device__ __forceinline__ f32x8 frag_columns(const float* tile, int ld, int r0, int c0) {
+    const int l = lane_id();
+    const float* p = tile + (r0 + 4 * (l >> 4)) * ld + c0 + (l & 15);
+    f32x8 f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[j] = p[j * ld];
+        f[j + 4] = p[(16 + j) * ld];
+    }
+    return f;
+}
+
+// Two stacked result tiles as an operand in split order.
+__device__ __forceinline__ void to_frag(f32x4 a, f32x4 b, bf16x8& f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[j] = (__bf16)a[j];
+        f[j + 4] = (__bf16)b[j];
+    }
+}
+__device__ __forceinline__ void to_frag(f32x4 a, f32x4 b, f32x8& f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[j] = a[j];
+        f[j + 4] = b[j];
+    }
+}
+
+// Four consecutive values of an output row; `wide`: the row and its columns allow one store.
+template <typename T>
+__device__ __forceinline__ void store_quad(T* row, int c, int cols, f32x4 v, bool wide) {
+    if (wide) {
+        if (c < cols) {
+            Quad<T> q;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+            *reinterpret_cast<Quad<T>*>(row + c) = q;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < cols) row[c + i] = (T)v[i];
+    }
+}
+
+}  // namespace sq
+}  // namespace vad

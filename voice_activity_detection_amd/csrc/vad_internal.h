@@ -37,6 +37,8 @@ int ensure_mfcc_tables();
 int ensure_rnn_attrs();
 int ensure_densenet_attrs();   // the same for the stride-1 DenseNet kernels; defined in densenet.hip
 int ensure_nicknet_attrs();    // the same for the conv + GRU model's kernels; defined in nicknet.hip
+int ensure_linear_attention_attrs();   // linear_attention.hip
+int ensure_window_attention_attrs();   // window_attention.hip
 
 // Looks up, once per device, the address of the built-in histogram of vad_threshold_sweep_noalloc_f32; sweep.hip.
 int ensure_sweep_scratch();

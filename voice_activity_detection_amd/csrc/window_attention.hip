@@ -1,0 +1,985 @@
+// Attention with a sliding window and sinks: row i of a sequence sees key j when j <= i and (i - j < window or j < sinks).
+//
+//   P = softmax over the visible keys of scale q k^T,  O = P V
+//   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Every kernel keeps rows of one side in registers (queries for O and dQ, keys for dK and dV) and streams tiles of 64
+// rows of the other side through LDS, visiting only tiles that some row of the block sees.  Scores are formed
+// transposed -- own rows along the lanes, streamed rows down the result tile -- so that the softmax of a row stays
+// within four lanes and the weights are, without moving, the operand of the second product.  The forward pass goes over
+// the keys once with a running maximum and sum, and keeps (maximum, 1 / sum) per row for the backward pass, both in
+// float32 and in units of log2.
+//
+// Key heads shared by several query heads: the forward pass and dQ run per query head, dK and dV add their query heads
+// in registers.  The few sink keys are seen by every later row; their share of dK and dV is a second kernel over
+// segments of the rows, joined in a fixed order.
+//
+// A row outside a key's window must not feel what that key holds: scores are replaced, not multiplied, where the mask
+// says so, and where a partly visible tile holds an infinity or a NaN, 0 * NaN in the matrix product is avoided by adding
+// its rows one at a time.
+
+#include <mutex>
+#include <type_traits>
+
+#include "sequence_device.h"
+
+namespace vad {
+namespace {
+using namespace sq;
+
+constexpr int kTile = 64;           // streamed rows
+constexpr int kThreads = 256;
+
+template <typename T>
+struct WindowArgs {
+    Heads<const T> q, k, v, go;
+    const T* o;                     // outputs of the forward pass (backward)
+    T* out;                         // o, or dq
+    T* dk;
+    T* dv;
+    float* stats;                   // (row, head): maximum, 1 / sum
+    float* delta;                   // (row, head): rowsum(dO O)
+    float* parts;                   // (seq, kv head, 1 + segments, dk | dv, sinks, dim)
+    Sequences seq;
+    int n_seq, heads, kv_heads, dim, window, sinks, segments;
+    float scale;
+    bool wide, wide_out;
+};
+
+template <typename T, int DP>
+struct TileShape {
+    static constexpr int kLd = DP + Elem<T>::kPer16B;
+    static constexpr int kPieces = kTile * DP / Elem<T>::kPer16B / kThreads;
+    static constexpr int kPPR = DP / Elem<T>::kPer16B;
+    static constexpr size_t kLds = (size_t)2 * kTile * kLd * sizeof(T) + (3 * kTile + 4) * sizeof(float);
+};
+
+// 64 rows from t0 on of one head, rows from len on as zero
+template <typename T, int DP>
+struct Staged {
+    u32x4 r[TileShape<T, DP>::kPieces];
+    __device__ __forceinline__ void fetch(const T* p, int64_t st, int t0, int len, int dim, bool wide) {
+        using C = TileShape<T, DP>;
+#pragma unroll
+        for (int n = 0; n < C::kPieces; ++n) {
+            const int i = threadIdx.x + n * kThreads, row = i / C::kPPR;
+            r[n] = u32x4{0, 0, 0, 0};
+            if (t0 + row < len) r[n] = load_piece(p + (int64_t)(t0 + row) * st, i % C::kPPR * Elem<T>::kPer16B, dim, wide);
+        }
+    }
+    __device__ __forceinline__ void put(T* tile) const {
+        using C = TileShape<T, DP>;
+#pragma unroll
+        for (int n = 0; n < C::kPieces; ++n) {
+            const int i = threadIdx.x + n * kThreads;
+            *reinterpret_cast<u32x4*>(tile + i / C::kPPR * C::kLd + i % C::kPPR * Elem<T>::kPer16B) = r[n];
+        }
+    }
+    __device__ __forceinline__ bool not_finite() const {
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < TileShape<T, DP>::kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
+        return bad;
+    }
+};
+
+// acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
+// own row.  `careful`: only rows that `sees` admits are touched.
+template <typename T, int DP, int NB, typename Sees>
+__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB], f32x4 (&acc)[DP / 16][NB], bool careful, Sees sees) {
+    constexpr int kLd = TileShape<T, DP>::kLd;
+    if (!careful) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            Frag<T> f[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) {
+                const Frag<T> x = frag_columns(tile, kLd, 32 * t, 16 * b);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) acc[b][nb] = mma(x, f[nb], acc[b][nb]);
+            }
+        }
+        return;
+    }
+    const int l = lane_id(), g = l >> 4;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+                for (int gg = 0; gg < 4; ++gg) {
+                    const float w = __shfl(p[kb][nb][i], (l & 15) + 16 * gg);
+                    const int row = 16 * kb + 4 * gg + i;
+                    if (sees(row, nb)) {
+#pragma unroll
+                        for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[b][nb][e] = fmaf(w, (float)tile[row * kLd + 16 * b + 4 * g + e], acc[b][nb][e]);
+                    }
+                }
+}
+
+// s = tile own^T for the 64 streamed rows
+template <typename T, int DP, int NB>
+__device__ __forceinline__ void scores(const T* tile, const Frag<T> (&own)[NB][DP / 32], f32x4 (&s)[4][NB]) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[kb][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+            const Frag<T> x = frag_natural(tile, TileShape<T, DP>::kLd, 16 * kb, 32 * d);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) s[kb][nb] = mma(x, own[nb][d], s[kb][nb]);
+        }
+    }
+}
+
+__device__ __forceinline__ float across_groups_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float across_groups_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// The key tiles that rows r0 .. r1 see: the first sink tile if it lies before the band, then the band's.
+struct KeyTiles {
+    int band, end;                  // first rows of the band's first tile, and past its last
+    bool sink;
+    __device__ __forceinline__ KeyTiles(int r0, int r1, int window, int sinks) {
+        const int lo = r0 - window + 1;
+        band = lo > 0 ? lo / kTile * kTile : 0;
+        end = r1 / kTile * kTile + kTile;
+        sink = sinks > 0 && band > 0;
+    }
+    __device__ __forceinline__ int first() const { return sink ? 0 : band; }
+    __device__ __forceinline__ int next(int t) const { return sink && t == 0 ? band : t + kTile; }
+};
+
+// BACK == false: O and stats.  BACK == true: dQ and delta.
+template <typename T, int DP, int NB, bool BACK>
+__global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) {
+    using C = TileShape<T, DP>;
+    extern __shared__ char lds_raw[];
+    T* sk = reinterpret_cast<T*>(lds_raw);
+    T* sv = sk + kTile * C::kLd;
+    int* flags = reinterpret_cast<int*>(sv + kTile * C::kLd);
+    const int h = blockIdx.y, s = blockIdx.z, hk = h / (a.heads / a.kv_heads);
+    int64_t first, len64;
+    sequence_rows(a.seq, s, first, len64);
+    const int len = (int)len64, dim = a.dim;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const T* qp = head_ptr(a.q, a.seq, s, first, h);
+    const T* kp = head_ptr(a.k, a.seq, s, first, hk);
+    const T* vp = head_ptr(a.v, a.seq, s, first, hk);
+    const T* gp = BACK ? head_ptr(a.go, a.seq, s, first, h) : nullptr;
+    const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
+    const float l2scale = a.scale * kLog2e;
+    constexpr int kRows = 64 * NB;
+    zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
+    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+    int turn = 0;
+    for (int64_t r0_64 = (int64_t)blockIdx.x * kRows; r0_64 < len; r0_64 += (int64_t)gridDim.x * kRows) {
+        const int r0 = (int)r0_64, r1 = (len - r0 < kRows ? len - r0 : kRows) + r0 - 1;
+        const int w0 = r0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
+        Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
+        f32x4 acc[DP / 16][NB];
+        float m[NB], sum[NB], delta[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int row = w0 + 16 * nb + c;
+            const bool live = row < len;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) qf[nb][d] = load_row_frag<T>(qp + (int64_t)row * a.q.st, live, 32 * d + 8 * g, dim, a.wide);
+            m[nb] = -INFINITY;
+            sum[nb] = 0.0f;
+            if (BACK) {
+                const int64_t at = (row_base + row) * a.heads + h;
+                float x = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    gf[nb][d] = load_row_frag<T>(gp + (int64_t)row * a.go.st, live, 32 * d + 8 * g, dim, a.wide);
+                    const Frag<T> of = load_row_frag<T>(a.o + at * dim, live, 32 * d + 8 * g, dim, a.wide_out);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x = fmaf((float)gf[nb][d][j], (float)of[j], x);
+                }
+                delta[nb] = across_groups_sum(x);
+                m[nb] = live ? a.stats[2 * at] : 0.0f;
+                sum[nb] = live ? a.stats[2 * at + 1] : 0.0f;
+                if (live && g == 0) a.delta[at] = delta[nb];
+            }
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const KeyTiles tiles(r0, r1, a.window, a.sinks);
+        Staged<T, DP> rk, rv;
+        rk.fetch(kp, a.k.st, tiles.first(), len, dim, a.wide);
+        rv.fetch(vp, a.v.st, tiles.first(), len, dim, a.wide);
+        for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), turn ^= 1) {
+            __syncthreads();                                   // the tile before is read
+            rk.put(sk);
+            rv.put(sv);
+            const bool edge = !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window);
+            if (edge && (BACK ? rk : rv).not_finite()) flags[turn] = 1;
+            __syncthreads();
+            const bool careful = edge && flags[turn];
+            if (threadIdx.x == 0) flags[turn ^ 1] = 0;
+            const int nt = tiles.next(t);
+            if (nt < tiles.end) {
+                rk.fetch(kp, a.k.st, nt, len, dim, a.wide);
+                rv.fetch(vp, a.v.st, nt, len, dim, a.wide);
+            }
+            if (t > w1 || (w0 - (t + kTile - 1) >= a.window && t >= a.sinks)) continue;      // nothing for this wave
+            f32x4 p[4][NB];
+            scores<T, DP, NB>(sk, qf, p);
+            const bool masked = !(t + kTile - 1 <= w0 && w1 - t < a.window);
+            const auto sees = [&](int row, int nb) {
+                const int j = t + row, gap = w0 + 16 * nb + c - j;
+                return ((unsigned)gap < (unsigned)a.window) | ((gap >= 0) & (j < a.sinks));
+            };
+            if (masked) {
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[kb][nb][i] = sees(16 * kb + 4 * g + i, nb) ? p[kb][nb][i] : -INFINITY;
+            }
+            if (!BACK) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float top = p[0][nb][0];
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top = fmaxf(top, p[kb][nb][i]);
+                    const float now = fmaxf(m[nb], across_groups_max(top) * l2scale);
+                    const float base = now == -INFINITY ? 0.0f : now;
+                    const float shrink = __builtin_amdgcn_exp2f(m[nb] - base);
+                    m[nb] = now;
+                    float part = 0.0f;
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[kb][nb][i] = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -base));
+                            part += p[kb][nb][i];
+                        }
+                    sum[nb] = fmaf(sum[nb], shrink, part);
+#pragma unroll
+                    for (int b = 0; b < DP / 16; ++b) acc[b][nb] *= shrink;
+                }
+                accumulate<T, DP, NB>(sv, p, acc, careful, sees);
+            } else {
+                f32x4 dp[4][NB];
+                scores<T, DP, NB>(sv, gf, dp);
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -m[nb])) * sum[nb];
+                            dp[kb][nb][i] = (p[kb][nb][i] == -INFINITY) & masked ? 0.0f : x * (dp[kb][nb][i] - delta[nb]) * a.scale;
+                        }
+                accumulate<T, DP, NB>(sk, dp, acc, careful, sees);
+            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int row = w0 + 16 * nb + c;
+            const int64_t at = (row_base + row) * a.heads + h;
+            float f = 1.0f;
+            if (!BACK) {
+                f = 1.0f / across_groups_sum(sum[nb]);
+                if (a.stats && row < len && g == 0) {
+                    a.stats[2 * at] = m[nb];
+                    a.stats[2 * at + 1] = f;
+                }
+            }
+            if (row < len) {
+#pragma unroll
+                for (int b = 0; b < DP / 16; ++b) store_quad(a.out + at * dim, 16 * b + 4 * g, dim, acc[b][nb] * f, a.wide_out);
+            }
+        }
+    }
+}
+
+// dK and dV.  SINKS == false: the block's keys against the rows of their window.  SINKS == true: the sink keys against the
+// rows beyond their window, one segment of the rows.
+template <typename T, int DP, int NB, bool SINKS>
+__global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) {
+    using C = TileShape<T, DP>;
+    extern __shared__ char lds_raw[];
+    T* sqr = reinterpret_cast<T*>(lds_raw);
+    T* sgo = sqr + kTile * C::kLd;
+    float* sm = reinterpret_cast<float*>(sgo + kTile * C::kLd);
+    float* sinv = sm + kTile;
+    float* sdelta = sinv + kTile;
+    int* flags = reinterpret_cast<int*>(sdelta + kTile);
+    const int hk = blockIdx.y, s = blockIdx.z, group = a.heads / a.kv_heads;
+    int64_t first, len64;
+    sequence_rows(a.seq, s, first, len64);
+    const int len = (int)len64, dim = a.dim;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const T* kp = head_ptr(a.k, a.seq, s, first, hk);
+    const T* vp = head_ptr(a.v, a.seq, s, first, hk);
+    const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
+    const float l2scale = a.scale * kLog2e;
+    constexpr int kKeys = 64 * NB;
+    if (!SINKS) {
+        zero_outside(a.dk, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
+        zero_outside(a.dv, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
+    }
+    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+    int turn = 0;
+    for (int64_t j0_64 = SINKS ? 0 : (int64_t)blockIdx.x * kKeys; j0_64 < (SINKS ? (len < 1 ? len : 1) : len);
+         j0_64 += SINKS ? 1 : (int64_t)gridDim.x * kKeys) {
+        const int j0 = (int)j0_64;
+        const int w0 = j0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
+        // the rows [i0, i1) that see the keys
+        int i0 = j0, i1;
+        if (SINKS) {
+            const int beyond = len > a.window ? len - a.window : 0;
+            const int per = ((beyond + a.segments - 1) / a.segments + kTile - 1) / kTile * kTile;
+            const int64_t lo = a.window + (int64_t)blockIdx.x * per;
+            i0 = (int)(lo < len ? lo : len);
+            i1 = (int)(lo + per < len ? lo + per : len);
+        } else {
+            const int64_t hi = (int64_t)j0 + kKeys - 1 + a.window;
+            i1 = (int)(hi < len ? hi : len);
+        }
+        const int keys = SINKS ? (a.sinks < len ? a.sinks : len) : len;
+        Frag<T> kf[NB][DP / 32], vf[NB][DP / 32];
+        f32x4 dk[DP / 16][NB], dv[DP / 16][NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int key = w0 + 16 * nb + c;
+            const bool live = key < keys;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                kf[nb][d] = load_row_frag<T>(kp + (int64_t)key * a.k.st, live, 32 * d + 8 * g, dim, a.wide);
+                vf[nb][d] = load_row_frag<T>(vp + (int64_t)key * a.v.st, live, 32 * d + 8 * g, dim, a.wide);
+            }
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) dk[b][nb] = dv[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
+        Staged<T, DP> rq, rg;
+        float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;
+        const auto fetch = [&](int step) {
+            const int h = hk * group + step / n_tiles, t = i0 + step % n_tiles * kTile;
+            rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1, dim, a.wide);
+            rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1, dim, a.wide);
+            const int row = t + threadIdx.x;
+            if (threadIdx.x < kTile) {
+                const int64_t at = (row_base + row) * a.heads + h;
+                rm = row < i1 ? a.stats[2 * at] : 0.0f;
+                rinv = row < i1 ? a.stats[2 * at + 1] : 0.0f;
+                rdelta = row < i1 ? a.delta[at] : 0.0f;
+            }
+        };
+        const int steps = n_tiles * group;
+        if (steps) fetch(0);
+        for (int step = 0; step < steps; ++step, turn ^= 1) {
+            const int t = i0 + step % n_tiles * kTile;
+            __syncthreads();
+            rq.put(sqr);
+            rg.put(sgo);
+            if (threadIdx.x < kTile) {
+                sm[threadIdx.x] = rm;
+                sinv[threadIdx.x] = rinv;
+                sdelta[threadIdx.x] = rdelta;
+            }
+            const bool edge = SINKS || !(t >= j0 + kKeys - 1 && t + kTile - 1 - j0 < a.window);
+            if (edge && (rq.not_finite() || rg.not_finite())) flags[turn] = 1;
+            __syncthreads();
+            const bool careful = edge && flags[turn];
+            if (threadIdx.x == 0) flags[turn ^ 1] = 0;
+            if (step + 1 < steps) fetch(step + 1);
+            if (w0 >= keys || (!SINKS && (t + kTile - 1 < w0 || t - w1 >= a.window))) continue;
+            const auto sees = [&](int row, int nb) {
+                const int i = t + row, j = w0 + 16 * nb + c;
+                return (i < i1) & (SINKS ? (j < keys) & (i - j >= a.window) : (unsigned)(i - j) < (unsigned)a.window);
+            };
+            const bool masked = SINKS || !(t >= w1 && t + kTile - 1 - w0 < a.window && t + kTile <= i1);
+            f32x4 p[4][NB], dp[4][NB];
+            scores<T, DP, NB>(sqr, kf, p);
+            scores<T, DP, NB>(sgo, vf, dp);
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                const f32x4 mm = *reinterpret_cast<const f32x4*>(sm + 16 * kb + 4 * g);
+                const f32x4 inv = *reinterpret_cast<const f32x4*>(sinv + 16 * kb + 4 * g);
+                const f32x4 dl = *reinterpret_cast<const f32x4*>(sdelta + 16 * kb + 4 * g);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool see = !masked | sees(16 * kb + 4 * g + i, nb);
+                        const float x = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -mm[i])) * inv[i];
+                        p[kb][nb][i] = see ? x : 0.0f;
+                        dp[kb][nb][i] = see ? x * (dp[kb][nb][i] - dl[i]) * a.scale : 0.0f;
+                    }
+            }
+            accumulate<T, DP, NB>(sgo, p, dv, careful, sees);
+            accumulate<T, DP, NB>(sqr, dp, dk, careful, sees);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int key = w0 + 16 * nb + c;
+            if (key < a.sinks && key < len) {
+                // a sink key's sums go to the joining kernel in float32: [0] of its window, [1 + n] of segment n
+                float* out = a.parts + (((((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + blockIdx.x : 0)) * 2) * a.sinks + key) * dim;
+#pragma unroll
+                for (int b = 0; b < DP / 16; ++b) {
+                    store_quad(out, 16 * b + 4 * g, dim, dk[b][nb], false);
+                    store_quad(out + (int64_t)a.sinks * dim, 16 * b + 4 * g, dim, dv[b][nb], false);
+                }
+            } else if (!SINKS && key < len) {
+                const int64_t at = ((row_base + key) * a.kv_heads + hk) * dim;
+#pragma unroll
+                for (int b = 0; b < DP / 16; ++b) {
+                    store_quad(a.dk + at, 16 * b + 4 * g, dim, dk[b][nb], a.wide_out);
+                    store_quad(a.dv + at, 16 * b + 4 * g, dim, dv[b][nb], a.wide_out);
+                }
+            }
+        }
+        if (SINKS) break;
+    }
+}
+
+// dK and dV of the sink keys: their window's sums and those of all segments, in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_join_kernel(WindowArgs<T> a) {
+    const int hk = blockIdx.y, s = blockIdx.z;
+    int64_t first, len;
+    sequence_rows(a.seq, s, first, len);
+    const int64_t n = (int64_t)a.sinks * a.dim, e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (e >= 2 * n) return;
+    const int which = e >= n, key = (int)((e % n) / a.dim), d = (int)(e % a.dim);
+    if (key >= len) return;
+    const float* p = a.parts + ((int64_t)s * a.kv_heads + hk) * (1 + a.segments) * 2 * n + e;
+    float x = 0.0f;
+    for (int i = 0; i <= a.segments; ++i) x += p[(int64_t)i * 2 * n];
+    const int64_t row = (a.seq.starts ? first : (int64_t)s * a.seq.max_len) + key;
+    (which ? a.dv : a.dk)[(row * a.kv_heads + hk) * a.dim + d] = (T)x;
+}
+
+// ---- one row against a rolling cache ----
+//
+// Slot j < sinks holds row j, slot sinks + r the latest row i >= sinks with (i - sinks) % window == r: exactly the rows
+// that row pos[b] sees.  The step stores its own key and value and reads min(pos + 1, sinks + window) slots.
+
+template <typename T>
+struct StepArgs {
+    Heads<const T> q, k, v;         // (batch, head) rows; st unused
+    Heads<T> ck, cv;                // (batch, slot, head)
+    const int64_t* pos;
+    T* o;
+    float* parts;                   // (batch, head, split): maximum, sum, dim values
+    int heads, kv_heads, dim, window, sinks, splits, chunks;
+    float scale;
+    bool wide;
+};
+
+// A wave takes 64 / (lanes of a row) slots at a time; a lane keeps 16 bytes of the row for each of GB query heads.
+template <typename T, int DP, int GB>
+__global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
+    constexpr int VE = Elem<T>::kPer16B, kLanes = DP / VE, kRows = 64 / kLanes, kUnroll = 4;
+    __shared__ float s_ml[kThreads / 64][GB][2];
+    __shared__ float s_acc[kThreads / 64][GB][DP];
+    const int split = blockIdx.x, hk = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, b = blockIdx.z;
+    const int group = a.heads / a.kv_heads;
+    const int lane = lane_id(), wave = threadIdx.x >> 6, d = lane % kLanes * VE, r = lane / kLanes;
+    const int64_t pos = a.pos[b];
+    const int slots = a.sinks + a.window;
+    const int n = pos < 0 ? 0 : (int)(pos + 1 < slots ? pos + 1 : slots);
+    const int own = pos < 0 ? -1 : (int)(pos < a.sinks ? pos : a.sinks + (pos - a.sinks) % a.window);
+    const int per = (n + a.splits - 1) / a.splits;
+    const int lo = split * per, hi = lo + per < n ? lo + per : n;
+    const T* kn = a.k.p + b * a.k.sb + hk * a.k.sh;
+    const T* vn = a.v.p + b * a.v.sb + hk * a.v.sh;
+    T* ck = a.ck.p + b * a.ck.sb + hk * a.ck.sh;
+    T* cv = a.cv.p + b * a.cv.sb + hk * a.cv.sh;
+    const float l2scale = a.scale * kLog2e;
+    float q[GB][VE], acc[GB][VE], m[GB], sum[GB];
+#pragma unroll
+    for (int x = 0; x < GB; ++x) {
+        const int h = hk * group + chunk * GB + x;
+        const bool live = chunk * GB + x < group;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            q[x][e] = live && d + e < a.dim ? (float)a.q.p[b * a.q.sb + h * a.q.sh + d + e] * l2scale : 0.0f;
+            acc[x][e] = 0.0f;
+        }
+        m[x] = -INFINITY;
+        sum[x] = 0.0f;
+    }
+    for (int base = lo + wave * kRows; base < hi; base += kThreads / 64 * kRows * kUnroll) {
+        u32x4 kr[kUnroll], vr[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int slot = base + u * (kThreads / 64) * kRows + r;
+            kr[u] = vr[u] = u32x4{0, 0, 0, 0};
+            if (slot < hi) {
+                const bool mine = slot == own;
+                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.wide);
+                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.wide);
+                if (mine && chunk == 0) {
+                    if (a.wide) {
+                        if (d < a.dim) {
+                            *reinterpret_cast<u32x4*>(ck + slot * a.ck.st + d) = kr[u];
+                            *reinterpret_cast<u32x4*>(cv + slot * a.cv.st + d) = vr[u];
+                        }
+                    } else {
+                        for (int e = 0; e < VE && d + e < a.dim; ++e) {
+                            ck[slot * a.ck.st + d + e] = kn[d + e];
+                            cv[slot * a.cv.st + d + e] = vn[d + e];
+                        }
+                    }
+                }
+            }
+        }
+        float sc[kUnroll][GB];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            T kk[VE];
+            __builtin_memcpy(kk, &kr[u], 16);
+            const bool live = base + u * (kThreads / 64) * kRows + r < hi;
+#pragma unroll
+            for (int x = 0; x < GB; ++x) {
+                float t = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) t = fmaf(q[x][e], (float)kk[e], t);
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) t += __shfl_xor(t, o);
+                sc[u][x] = live ? t : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < GB; ++x) {
+            float now = m[x];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) now = fmaxf(now, sc[u][x]);
+            const float ref = now == -INFINITY ? 0.0f : now;
+            const float shrink = __builtin_amdgcn_exp2f(m[x] - ref);
+            m[x] = now;
+            sum[x] *= shrink;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[x][e] *= shrink;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                T vv[VE];
+                __builtin_memcpy(vv, &vr[u], 16);
+                const float p = __builtin_amdgcn_exp2f(sc[u][x] - ref);
+                sum[x] += p;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) acc[x][e] = fmaf(p, (float)vv[e], acc[x][e]);
+            }
+        }
+    }
+    // join the rows of a wave, then the waves
+#pragma unroll
+    for (int x = 0; x < GB; ++x) {
+#pragma unroll
+        for (int o = kLanes; o < 64; o <<= 1) {
+            const float om = __shfl_xor(m[x], o), now = fmaxf(m[x], om), ref = now == -INFINITY ? 0.0f : now;
+            const float f = __builtin_amdgcn_exp2f(m[x] - ref), fo = __builtin_amdgcn_exp2f(om - ref);
+            sum[x] = sum[x] * f + __shfl_xor(sum[x], o) * fo;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[x][e] = acc[x][e] * f + __shfl_xor(acc[x][e], o) * fo;
+            m[x] = now;
+        }
+        if (r == 0) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) s_acc[wave][x][d + e] = acc[x][e];
+            if (d == 0) {
+                s_ml[wave][x][0] = m[x];
+                s_ml[wave][x][1] = sum[x];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < GB * DP; i += kThreads) {
+        const int x = i / DP, dd = i % DP;
+        if (chunk * GB + x >= group || dd >= a.dim) continue;
+        float now = -INFINITY, total = 0.0f, value = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) now = fmaxf(now, s_ml[w][x][0]);
+        const float ref = now == -INFINITY ? 0.0f : now;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[w][x][0] - ref);
+            total = fmaf(s_ml[w][x][1], f, total);
+            value = fmaf(s_acc[w][x][dd], f, value);
+        }
+        const int64_t head = (int64_t)b * a.heads + hk * group + chunk * GB + x;
+        if (a.splits == 1) {
+            a.o[head * a.dim + dd] = (T)(n ? value / total : 0.0f);
+        } else {
+            float* out = a.parts + (head * a.splits + split) * (a.dim + 2);
+            out[2 + dd] = value;
+            if (dd == 0) {
+                out[0] = now;
+                out[1] = total;
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(128) void window_step_join_kernel(StepArgs<T> a) {
+    const int64_t head = blockIdx.x;
+    const int d = threadIdx.x;
+    if (d >= a.dim) return;
+    const float* p = a.parts + head * a.splits * (a.dim + 2);
+    const int stride = a.dim + 2;
+    float now = -INFINITY, total = 0.0f, value = 0.0f;
+    for (int i = 0; i < a.splits; ++i) now = fmaxf(now, p[i * stride]);
+    const float ref = now == -INFINITY ? 0.0f : now;
+    for (int i = 0; i < a.splits; ++i) {
+        const float f = __builtin_amdgcn_exp2f(p[i * stride] - ref);
+        total = fmaf(p[i * stride + 1], f, total);
+        value = fmaf(p[i * stride + 2 + d], f, value);
+    }
+    a.o[head * a.dim + d] = (T)(a.pos[head / a.heads] < 0 ? 0.0f : value / total);
+}
+
+// Rows of whole sequences into their slots: slot by slot, the row that it holds behind the sequence's last.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_fill_kernel(StepArgs<T> a, Sequences seq, int64_t* __restrict__ pos) {
+    const int hk = blockIdx.y, b = blockIdx.z;
+    int64_t first, len;
+    sequence_rows(seq, b, first, len);
+    if (pos && blockIdx.x == 0 && hk == 0 && threadIdx.x == 0) pos[b] = len;
+    const T* kp = head_ptr(a.k, seq, b, first, hk);
+    const T* vp = head_ptr(a.v, seq, b, first, hk);
+    T* ck = a.ck.p + b * a.ck.sb + hk * a.ck.sh;
+    T* cv = a.cv.p + b * a.cv.sb + hk * a.cv.sh;
+    const int pieces = (a.dim + Elem<T>::kPer16B - 1) / Elem<T>::kPer16B;
+    const int64_t total = (int64_t)(a.sinks + a.window) * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t slot = i / pieces;
+        const int d = (int)(i % pieces) * Elem<T>::kPer16B;
+        int64_t row = slot;
+        if (slot >= a.sinks) {
+            const int64_t rolled = len - a.sinks, at = slot - a.sinks;
+            row = at < rolled ? a.sinks + at + (rolled - 1 - at) / a.window * a.window : len;
+        }
+        if (row >= len) continue;
+        if (a.wide) {
+            *reinterpret_cast<u32x4*>(ck + slot * a.ck.st + d) = load_piece(kp + row * a.k.st, d, a.dim, true);
+            *reinterpret_cast<u32x4*>(cv + slot * a.cv.st + d) = load_piece(vp + row * a.v.st, d, a.dim, true);
+        } else {
+            for (int e = d; e < d + Elem<T>::kPer16B && e < a.dim; ++e) {
+                ck[slot * a.ck.st + e] = kp[row * a.k.st + e];
+                cv[slot * a.cv.st + e] = vp[row * a.v.st + e];
+            }
+        }
+    }
+}
+
+template <typename T>
+Heads<const T> heads_of(const void* p, const int64_t* s) {
+    return {static_cast<const T*>(p), s[0], s[1], s[2]};
+}
+template <typename T>
+bool wide_rows(const Heads<T>& x, int dim) {
+    constexpr int VE = 16 / sizeof(T);
+    return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.sb % VE == 0 && x.st % VE == 0 && x.sh % VE == 0 && dim % VE == 0;
+}
+
+template <typename T>
+constexpr int own_blocks() { return sizeof(T) == 2 ? 2 : 1; }     // 16-row blocks of own rows per wave
+
+template <typename F>
+void for_dim(int dim, F f) {
+    if (dim <= 32)
+        f(std::integral_constant<int, 32>{});
+    else if (dim <= 64)
+        f(std::integral_constant<int, 64>{});
+    else
+        f(std::integral_constant<int, 128>{});
+}
+
+unsigned row_tiles(int64_t max_len, int rows) {
+    const int64_t n = (max_len + rows - 1) / rows;
+    return (unsigned)(n < 1 ? 1 : n);
+}
+
+template <typename T>
+int run_forward(WindowArgs<T> a, hipStream_t st) {
+    for_dim(a.dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value, NB = own_blocks<T>();
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), dim3(kThreads),
+                           (TileShape<T, DP>::kLds), st, a);
+    });
+    VAD_HIP_CHECK(hipGetLastError());
+    return VAD_OK;
+}
+
+template <typename T>
+int run_backward(WindowArgs<T> a, hipStream_t st) {
+    for_dim(a.dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value, NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
+        const dim3 block(kThreads);
+        const size_t lds = TileShape<T, DP>::kLds;
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, true>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), block, lds, st, a);
+        hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, lds, st, a);
+        if (a.sinks > 0) {
+            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true>), dim3(a.segments, a.kv_heads, a.n_seq), block, lds, st, a);
+            hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
+        }
+    });
+    VAD_HIP_CHECK(hipGetLastError());
+    return VAD_OK;
+}
+
+template <typename T, int DP>
+int allow_tiles() {
+    constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
+    const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, true>),
+                       reinterpret_cast<const void*>(&window_keys_kernel<T, DP, NK, false>), reinterpret_cast<const void*>(&window_keys_kernel<T, DP, 1, true>)};
+    for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)TileShape<T, DP>::kLds));
+    return VAD_OK;
+}
+
+// Segments of the rows beyond the window for the sink keys' gradients: at least 512 rows each, enough blocks to fill the chip.
+int sink_segments(int64_t n_seq, int64_t max_len, int kv_heads, int window) {
+    const int64_t beyond = max_len > window ? max_len - window : 0, blocks = n_seq * kv_heads;
+    int64_t n = (512 + blocks - 1) / blocks;
+    if (n > beyond / 512) n = beyond / 512;
+    return (int)(n < 1 ? 1 : n);
+}
+
+int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype, int64_t window, int sinks) {
+    VAD_REQUIRE(dtype == VAD_DTYPE_F32 || dtype == VAD_DTYPE_BF16, "dtype must be VAD_DTYPE_F32 or VAD_DTYPE_BF16, got %d", dtype);
+    VAD_REQUIRE(dim >= 1 && dim <= VAD_MAX_HEAD_DIM, "head dimension %d out of range 1..%d", dim, VAD_MAX_HEAD_DIM);
+    VAD_REQUIRE(kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 && heads <= 65535, "%d heads cannot share %d key heads", heads, kv_heads);
+    VAD_REQUIRE(window >= 1 && window <= (1 << 30), "window %lld out of range", (long long)window);
+    VAD_REQUIRE(sinks >= 0 && sinks <= VAD_MAX_SINKS, "sinks %d out of range 0..%d", sinks, VAD_MAX_SINKS);
+    VAD_REQUIRE(n_seq >= 0 && n_seq <= 65535, "sequence count %lld out of range 0..65535", (long long)n_seq);
+    VAD_REQUIRE(n_tokens >= 0 && max_len >= 0 && n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
+    return VAD_OK;
+}
+
+}  // namespace
+
+// The float32 tiles of 65 and more columns use more than 64 KB of LDS: opt in once per device.
+int ensure_window_attention_attrs() {
+    static std::mutex mu;
+    static bool done[64] = {false};
+    int dev = 0;
+    VAD_HIP_CHECK(hipGetDevice(&dev));
+    VAD_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev]) return VAD_OK;
+    int rc = VAD_OK;
+    if ((rc = allow_tiles<float, 32>()) != VAD_OK || (rc = allow_tiles<float, 64>()) != VAD_OK || (rc = allow_tiles<float, 128>()) != VAD_OK ||
+        (rc = allow_tiles<__bf16, 32>()) != VAD_OK || (rc = allow_tiles<__bf16, 64>()) != VAD_OK || (rc = allow_tiles<__bf16, 128>()) != VAD_OK)
+        return rc;
+    done[dev] = true;
+    return VAD_OK;
+}
+}  // namespace vad
+
+extern "C" int vad_window_attention_forward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                            const void* v_dev, const int64_t* v_strides, const int64_t* starts_dev, int64_t n_seq,
+                                            int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype, int64_t window,
+                                            int sinks, float scale, void* o_dev, float* stats_dev, void* stream) {
+    using namespace vad;
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, kv_heads, dim, dtype, window, sinks);
+    if (rc != VAD_OK) return rc;
+    VAD_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    VAD_REQUIRE(q_strides && k_strides && v_strides, "null pointer argument");
+    if (n_seq == 0 || (starts_dev ? n_tokens : max_len) == 0) return VAD_OK;
+    VAD_REQUIRE(q_dev && k_dev && v_dev && o_dev, "null pointer argument");
+    rc = ensure_window_attention_attrs();
+    if (rc != VAD_OK) return rc;
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) T;
+        WindowArgs<T> a = {};
+        a.q = heads_of<T>(q_dev, q_strides);
+        a.k = heads_of<T>(k_dev, k_strides);
+        a.v = heads_of<T>(v_dev, v_strides);
+        a.out = static_cast<T*>(o_dev);
+        a.stats = stats_dev;
+        a.seq = {starts_dev, n_tokens, max_len};
+        a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
+        a.window = (int)window, a.sinks = sinks, a.scale = scale;
+        a.wide = wide_rows(a.q, dim) && wide_rows(a.k, dim) && wide_rows(a.v, dim);
+        a.wide_out = reinterpret_cast<uintptr_t>(o_dev) % 16 == 0 && dim % (16 / sizeof(T)) == 0;
+        return run_forward<T>(a, static_cast<hipStream_t>(stream));
+    };
+    return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
+}
+
+extern "C" size_t vad_window_attention_workspace_bytes(int64_t n_seq, int64_t n_rows, int64_t max_len, int heads, int kv_heads, int dim,
+                                                       int64_t window, int sinks) {
+    using namespace vad;
+    if (n_seq <= 0 || n_rows <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || window <= 0 || sinks < 0) return 0;
+    size_t floats = (size_t)n_rows * heads;
+    if (sinks > 0) floats += (size_t)n_seq * kv_heads * (1 + sink_segments(n_seq, max_len, kv_heads, (int)window)) * 2 * sinks * dim;
+    return floats * sizeof(float);
+}
+
+extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                             const void* v_dev, const int64_t* v_strides, const void* o_dev, const void* do_dev,
+                                             const int64_t* do_strides, const float* stats_dev, const int64_t* starts_dev, int64_t n_seq,
+                                             int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype,
+                                             int64_t window, int sinks, float scale, void* dq_dev, void* dk_dev, void* dv_dev,
+                                             void* workspace_dev, size_t workspace_bytes, void* stream) {
+    using namespace vad;
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, kv_heads, dim, dtype, window, sinks);
+    if (rc != VAD_OK) return rc;
+    VAD_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    VAD_REQUIRE(q_strides && k_strides && v_strides && do_strides, "null pointer argument");
+    if (n_seq == 0 || (starts_dev ? n_tokens : max_len) == 0) return VAD_OK;
+    VAD_REQUIRE(q_dev && k_dev && v_dev && o_dev && do_dev && stats_dev && dq_dev && dk_dev && dv_dev && workspace_dev, "null pointer argument");
+    const int64_t n_rows = starts_dev ? n_tokens : n_seq * max_len;
+    const size_t need = vad_window_attention_workspace_bytes(n_seq, n_rows, max_len, heads, kv_heads, dim, window, sinks);
+    VAD_REQUIRE(workspace_bytes >= need, "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
+    rc = ensure_window_attention_attrs();
+    if (rc != VAD_OK) return rc;
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) T;
+        WindowArgs<T> a = {};
+        a.q = heads_of<T>(q_dev, q_strides);
+        a.k = heads_of<T>(k_dev, k_strides);
+        a.v = heads_of<T>(v_dev, v_strides);
+        a.go = heads_of<T>(do_dev, do_strides);
+        a.o = static_cast<const T*>(o_dev);
+        a.out = static_cast<T*>(dq_dev);
+        a.dk = static_cast<T*>(dk_dev);
+        a.dv = static_cast<T*>(dv_dev);
+        a.stats = const_cast<float*>(stats_dev);
+        a.delta = static_cast<float*>(workspace_dev);
+        a.parts = a.delta + n_rows * heads;
+        a.seq = {starts_dev, n_tokens, max_len};
+        a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
+        a.window = (int)window, a.sinks = sinks, a.scale = scale;
+        a.segments = sink_segments(n_seq, max_len, kv_heads, (int)window);
+        a.wide = wide_rows(a.q, dim) && wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.go, dim);
+        a.wide_out = (reinterpret_cast<uintptr_t>(o_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
+                      reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0 && dim % (16 / sizeof(T)) == 0;
+        return run_backward<T>(a, static_cast<hipStream_t>(stream));
+    };
+    return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
+}
+
+namespace vad {
+namespace {
+
+// Splits of a row's slots: enough blocks to fill the chip, at least 64 slots each.
+int step_splits(int64_t batch, int kv_heads, int chunks, int64_t slots) {
+    const int64_t blocks = batch * kv_heads * chunks;
+    int64_t n = (1024 + blocks - 1) / blocks;
+    if (n > slots / 64) n = slots / 64;
+    if (n > 64) n = 64;
+    return (int)(n < 1 ? 1 : n);
+}
+int step_heads(int group) { return group >= 4 ? 4 : (group >= 2 ? 2 : 1); }      // query heads of a block
+
+template <typename T>
+int run_step(StepArgs<T> a, int64_t batch, hipStream_t st) {
+    const int group = a.heads / a.kv_heads, gb = step_heads(group);
+    const dim3 grid(a.splits, a.kv_heads * a.chunks, (unsigned)batch), block(kThreads);
+    for_dim(a.dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (gb == 4)
+            hipLaunchKernelGGL((window_step_kernel<T, DP, 4>), grid, block, 0, st, a);
+        else if (gb == 2)
+            hipLaunchKernelGGL((window_step_kernel<T, DP, 2>), grid, block, 0, st, a);
+        else
+            hipLaunchKernelGGL((window_step_kernel<T, DP, 1>), grid, block, 0, st, a);
+    });
+    VAD_HIP_CHECK(hipGetLastError());
+    if (a.splits > 1) {
+        hipLaunchKernelGGL((window_step_join_kernel<T>), dim3((unsigned)(batch * a.heads)), dim3(128), 0, st, a);
+        VAD_HIP_CHECK(hipGetLastError());
+    }
+    return VAD_OK;
+}
+
+}  // namespace
+}  // namespace vad
+
+extern "C" size_t vad_window_step_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int64_t window, int sinks) {
+    using namespace vad;
+    if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || window <= 0 || sinks < 0) return 0;
+    const int group = heads / kv_heads, gb = step_heads(group), splits = step_splits(batch, kv_heads, (group + gb - 1) / gb, sinks + window);
+    return splits > 1 ? (size_t)batch * heads * splits * (dim + 2) * sizeof(float) : 0;
+}
+
+extern "C" int vad_window_attention_step(const void* q_dev, const int64_t* q_strides, const void* k_dev, const int64_t* k_strides,
+                                         const void* v_dev, const int64_t* v_strides, void* cache_k_dev, const int64_t* cache_k_strides,
+                                         void* cache_v_dev, const int64_t* cache_v_strides, const int64_t* pos_dev, int64_t batch,
+                                         int heads, int kv_heads, int dim, int dtype, int64_t window, int sinks, float scale, void* o_dev,
+                                         void* workspace_dev, size_t workspace_bytes, void* stream) {
+    using namespace vad;
+    int rc = check_heads(batch, 0, 0, heads, kv_heads, dim, dtype, window, sinks);
+    if (rc != VAD_OK) return rc;
+    VAD_REQUIRE(scale > 0.0f && scale < INFINITY, "scale must be positive and finite");
+    if (batch == 0) return VAD_OK;
+    VAD_REQUIRE(q_dev && k_dev && v_dev && cache_k_dev && cache_v_dev && pos_dev && o_dev && q_strides && k_strides && v_strides &&
+                    cache_k_strides && cache_v_strides,
+                "null pointer argument");
+    const size_t need = vad_window_step_workspace_bytes(batch, heads, kv_heads, dim, window, sinks);
+    VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) T;
+        StepArgs<T> a = {};
+        a.q = {static_cast<const T*>(q_dev), q_strides[0], 0, q_strides[1]};
+        a.k = {static_cast<const T*>(k_dev), k_strides[0], 0, k_strides[1]};
+        a.v = {static_cast<const T*>(v_dev), v_strides[0], 0, v_strides[1]};
+        a.ck = {static_cast<T*>(cache_k_dev), cache_k_strides[0], cache_k_strides[1], cache_k_strides[2]};
+        a.cv = {static_cast<T*>(cache_v_dev), cache_v_strides[0], cache_v_strides[1], cache_v_strides[2]};
+        a.pos = pos_dev;
+        a.o = static_cast<T*>(o_dev);
+        a.parts = static_cast<float*>(workspace_dev);
+        a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.window = (int)window, a.sinks = sinks, a.scale = scale;
+        const int group = heads / kv_heads, gb = step_heads(group);
+        a.chunks = (group + gb - 1) / gb;
+        a.splits = step_splits(batch, kv_heads, a.chunks, sinks + window);
+        a.wide = wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.ck, dim) && wide_rows(a.cv, dim);
+        return run_step<T>(a, batch, static_cast<hipStream_t>(stream));
+    };
+    return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
+}
+
+extern "C" int vad_window_cache_fill(const void* k_dev, const int64_t* k_strides, const void* v_dev, const int64_t* v_strides,
+                                     const int64_t* starts_dev, int64_t n_seq, int64_t n_tokens, int64_t max_len, int kv_heads, int dim,
+                                     int dtype, int64_t window, int sinks, void* cache_k_dev, const int64_t* cache_k_strides,
+                                     void* cache_v_dev, const int64_t* cache_v_strides, int64_t* pos_dev, void* stream) {
+    using namespace vad;
+    int rc = check_heads(n_seq, n_tokens, max_len, kv_heads, kv_heads, dim, dtype, window, sinks);
+    if (rc != VAD_OK) return rc;
+    if (n_seq == 0) return VAD_OK;
+    const bool empty = (starts_dev ? n_tokens : max_len) == 0;
+    VAD_REQUIRE(k_strides && v_strides && cache_k_strides && cache_v_strides && cache_k_dev && cache_v_dev && (empty || (k_dev && v_dev)),
+                "null pointer argument");
+    const auto run = [&](auto zero) {
+        typedef decltype(zero) T;
+        StepArgs<T> a = {};
+        a.k = heads_of<T>(k_dev, k_strides);
+        a.v = heads_of<T>(v_dev, v_strides);
+        a.ck = {static_cast<T*>(cache_k_dev), cache_k_strides[0], cache_k_strides[1], cache_k_strides[2]};
+        a.cv = {static_cast<T*>(cache_v_dev), cache_v_strides[0], cache_v_strides[1], cache_v_strides[2]};
+        a.kv_heads = kv_heads, a.dim = dim, a.window = (int)window, a.sinks = sinks;
+        a.wide = wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.ck, dim) && wide_rows(a.cv, dim);
+        const Sequences seq = {starts_dev, n_tokens, max_len};
+        const int64_t blocks = (((int64_t)sinks + window) * dim * sizeof(T) / 16 + kThreads) / kThreads;
+        hipLaunchKernelGGL((window_fill_kernel<T>), dim3((unsigned)(blocks < 256 ? blocks : 256), kv_heads, (unsigned)n_seq), dim3(kThreads), 0,
+                           static_cast<hipStream_t>(stream), a, seq, pos_dev);
+        VAD_HIP_CHECK(hipGetLastError());
+        return (int)VAD_OK;
+    };
+    return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
+}
