@@ -415,8 +415,8 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *                are float32.
  *   rows         q, k, v and the gradients of outputs are read through strides in ELEMENTS given on the host: {sequence,
  *                row, head} (steps: {batch, head}, caches: {batch, slot, head}); the head dimension is dense.  Any alignment
- *                works; rows that start 16-byte aligned with a head dimension of whole 16-byte pieces take the wide path.
- *                Outputs are dense (rows, heads, dim).
+ *                works; rows at 4-byte boundaries with a head dimension of whole 8- or 16-byte pieces take wide loads.
+ *                Row strides and dense rows (heads * dim) are below VAD_MAX_ROW_STRIDE.  Outputs are dense (rows, heads, dim).
  *   sequences    starts_dev == NULL: n_seq sequences of max_len rows each.  Otherwise the rows of all sequences are packed
  *                behind one another in n_tokens rows and starts_dev holds n_seq + 1 ascending int64 on the device, sequence s
  *                being rows starts[s] .. starts[s+1] - 1 (empty ones allowed).  The table is NOT validated: entries are clamped
@@ -430,6 +430,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
 #define VAD_DTYPE_BF16 1
 #define VAD_MAX_HEAD_DIM 128
 #define VAD_MAX_SINKS 64
+#define VAD_MAX_ROW_STRIDE (1 << 24)
 
 /*
  * Layer norm: y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (var: mean squared deviation).

@@ -57,13 +57,9 @@ struct Params {
 };
 
 __device__ __forceinline__ float group_sum(float v, int lanes, float* scratch) {
-    if (lanes <= 64) {
-        for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor(v, o);
-        return v;
-    }
+    if (lanes <= 64) return lanes_sum(v, lanes);
     // a whole block: the same order for every thread
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    v = lanes_sum(v, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();

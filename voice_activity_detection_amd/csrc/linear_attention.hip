@@ -13,8 +13,8 @@
 // walk of every span starts from its joined state.
 //
 // Wave w of a block owns columns 16 w .. 16 w + 15 of the state and of the outputs.  The state stays in float32; for
-// bfloat16 inputs its update multiplies v by the decay in float32 and splits the product exactly into three bfloat16
-// terms, so the state has float32's accuracy; the weights a^(i-j) (q . k) and the copy of the state that q is
+// bfloat16 inputs its update multiplies v by the decay in float32 and splits the product into bfloat16 terms -- three, which
+// is exact, where the state is handed out or crosses spans, two (2^-17) where it only feeds outputs of 8 bits; the weights a^(i-j) (q . k) and the copy of the state that q is
 // multiplied with are rounded to bfloat16 once.
 
 #include <mutex>
@@ -44,7 +44,8 @@ struct WalkArgs {
     const float* log_decay;
     float* spans;                      // [walk][seq][head][span][dim][dim]
     int n_seq, heads, dim, n_spans;
-    bool wide, wide_out;
+    int mode;                          // how rows are read
+    bool wide_out;
 };
 
 __device__ __forceinline__ float log2_decay(float ld) {
@@ -71,8 +72,13 @@ struct WalkShape {
 };
 
 // The (row block, key block) pairs of a piece's weights: the lower triangle, and the two blocks above it that share a
-// contraction of 32 keys with a diagonal block and must read as zero.
-__device__ const signed char kPairs[12][2] = {{0, 0}, {1, 0}, {1, 1}, {2, 0}, {2, 1}, {2, 2}, {3, 0}, {3, 1}, {3, 2}, {3, 3}, {0, 1}, {2, 3}};
+// contraction of 32 keys with a diagonal block and must read as zero.  Two bits a pair.
+constexpr unsigned pack_pairs(int which) {
+    const int p[12][2] = {{0, 0}, {1, 0}, {1, 1}, {2, 0}, {2, 1}, {2, 2}, {3, 0}, {3, 1}, {3, 2}, {3, 3}, {0, 1}, {2, 3}};
+    unsigned r = 0;
+    for (int t = 0; t < 12; ++t) r |= (unsigned)p[t][which] << (2 * t);
+    return r;
+}
 
 // float32 values as the sum of three bfloat16 (24 bits); not-finite values in the first term alone
 __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&f)[3]) {
@@ -87,9 +93,16 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&f)[3]) {
     }
 }
 
-template <typename T, int DP, bool STATE>
-__global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
+// Waves per SIMD that the registers are shared out for.
+template <typename T, int DP>
+constexpr int walk_waves() { return sizeof(T) == 2 && DP < 128 ? 3 : 2; }
+
+// WIDE: every row is read and written by whole 16-byte pieces (a.mode, a.wide_out), which saves the other forms' registers.
+template <typename T, int DP, bool STATE, bool WIDE>
+__global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kernel(WalkArgs<T> a) {
     using C = WalkShape<T, DP>;
+    const int mode = WIDE ? kWide : a.mode;
+    const bool wide_out = WIDE || a.wide_out;
     extern __shared__ char lds_raw[];
     T* sk = reinterpret_cast<T*>(lds_raw);
     T* sv = sk + kPiece * C::kLd;
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
     if (!STATE) zero_outside(w.o, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, span, a.n_spans);
     const int64_t per = span_rows(len, a.n_spans);
     const int64_t t0 = span * per, t1 = t0 + per < len ? t0 + per : len;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int64_t head = (int64_t)s * a.heads + h, elems = (int64_t)dim * dim;
     float* spans = a.spans ? a.spans + (((int64_t)blockIdx.y * a.n_seq * a.heads + head) * a.n_spans + span) * elems : nullptr;
     if (STATE) {
@@ -144,20 +157,36 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
     const T* qp = STATE ? nullptr : head_ptr(w.q, a.seq, s, first, h);
     T* op = w.o + ((a.seq.starts ? first : (int64_t)s * a.seq.max_len) * a.heads + h) * dim;
     constexpr int PPR = DP / Elem<T>::kPer16B;
+    const int sign = w.reverse ? -1 : 1;
     u32x4 rk[C::kPieces], rv[C::kPieces], rq[C::kPieces];
     auto fetch = [&](int64_t tc) {
+        const int64_t at = w.reverse ? len - 1 - tc : tc;
+        const T* kc = kp + at * w.k.st;
+        const T* vc = vp + at * w.v.st;
+        const T* qc = STATE ? nullptr : qp + at * w.q.st;
+        const int left = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);
 #pragma unroll
         for (int n = 0; n < C::kPieces; ++n) {
-            const int p = threadIdx.x + n * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B;
+            const int p = threadIdx.x + n * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B, sr = sign * row;
             rk[n] = rv[n] = rq[n] = u32x4{0, 0, 0, 0};
-            if (tc + row < t1) {
-                const int64_t at = w.reverse ? len - 1 - (tc + row) : tc + row;
-                rk[n] = load_piece(kp + at * w.k.st, pc, dim, a.wide);
-                rv[n] = load_piece(vp + at * w.v.st, pc, dim, a.wide);
-                if (!STATE) rq[n] = load_piece(qp + at * w.q.st, pc, dim, a.wide);
+            if (row < left) {
+                rk[n] = load_piece(kc + sr * (int)w.k.st, pc, dim, mode);
+                rv[n] = load_piece(vc + sr * (int)w.v.st, pc, dim, mode);
+                if (!STATE) rq[n] = load_piece(qc + sr * (int)w.q.st, pc, dim, mode);
             }
         }
     };
+    // Powers of the decay.  A row and key block m apart need a^(16 m + c - 4 g - i) = a^(16 m - 15) a^c a^(15 - 4 g - i), a
+    // diagonal block its own; the state's update a^(64 - row) = a^(16 m') a a^(15 - 4 g - i).
+    const float a1 = power(l2, 1.0f), a16 = power(l2, 16.0f), a32 = a16 * a16, ac = power(l2, (float)c);
+    const float within = w.within * ac * a1, across = w.across * ac;
+    float tail[4], diagonal[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        tail[i] = power(l2, (float)(15 - 4 * g - i));
+        diagonal[i] = c >= 4 * g + i ? w.within * power(l2, (float)(c - 4 * g - i)) : 0.0f;
+    }
+    const bool third = w.s1 || STATE;        // a state that is handed out or crosses spans keeps float32's accuracy
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     fetch(t0);
     __syncthreads();
@@ -184,16 +213,24 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
         f32x4 o[4];
         if (!STATE) {
             // weights of the piece: rows in columns of the tile, keys 16 kb + 4 g + i down its lanes
-            for (int t = wave; t < 12; t += C::kWaves) {
-                const int rb = kPairs[t][0], kb = kPairs[t][1];
+#pragma unroll
+            for (int u = 0; u < (12 + C::kWaves - 1) / C::kWaves; ++u) {
+                const int t = wave + u * C::kWaves;
+                if (t >= 12) break;
+                const int rb = (pack_pairs(0) >> (2 * t)) & 3, kb = (pack_pairs(1) >> (2 * t)) & 3;
                 f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (kb <= rb) {
 #pragma unroll
                     for (int d = 0; d < DP; d += 32)
                         acc = mma(frag_natural(sk, C::kLd, 16 * kb, d), frag_natural(sq_, C::kLd, 16 * rb, d), acc);
-                    const int gap = 16 * (rb - kb) + c - 4 * g;
+                    if (kb == rb) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i] = gap >= i ? acc[i] * (w.within * power(l2, (float)(gap - i))) : 0.0f;
+                        for (int i = 0; i < 4; ++i) acc[i] = c >= 4 * g + i ? acc[i] * diagonal[i] : 0.0f;
+                    } else {
+                        const float f = within * (rb - kb == 1 ? 1.0f : (rb - kb == 2 ? a16 : a32));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * tail[i] * f;
+                    }
                 }
                 Quad<T> p;
 #pragma unroll
@@ -209,7 +246,9 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
                 o[rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) o[rb] = mma(hf[d], frag_split(sq_, C::kLd, 16 * rb, 32 * d), o[rb]);
-                o[rb] *= w.across * power(l2, (float)(16 * rb + c));
+                o[rb] *= across;
+                if (rb & 1) o[rb] *= a16;
+                if (rb & 2) o[rb] *= a32;
             }
         }
         Frag<T> vf[2];
@@ -220,17 +259,24 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
         const bool last = tc + kPiece >= t1;
         const bool finish = !STATE && last && t1 == len && w.s1;
         if (!last || STATE || finish) {
-            const float less = finish && !w.reverse ? 1.0f : 0.0f;       // the forward walk hands out S, not a S
-            const float keep = power(l2, (float)n - less);
+            const bool less = finish && !w.reverse;                        // the forward walk hands out S, not a S
+            const float keep = n == kPiece && !less ? a32 * a32 : power(l2, (float)(n - (less ? 1 : 0)));
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) H[b] *= keep;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 float x[8];
+                if (n == kPiece) {
+                    // the varying factor first: a product of constants would be kept in registers across the pieces
+                    const float f = w.update * (less ? 1.0f : a1) * (t ? 1.0f : a32);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int row = 32 * t + 4 * g + (j < 4 ? j : 12 + j);
-                    x[j] = row < n ? (float)vf[t][j] * (w.update * power(l2, (float)(n - row) - less)) : 0.0f;
+                    for (int j = 0; j < 8; ++j) x[j] = (float)vf[t][j] * tail[j & 3] * (j < 4 ? f * a16 : f);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int row = 32 * t + 4 * g + (j < 4 ? j : 12 + j);
+                        x[j] = row < n ? (float)vf[t][j] * (w.update * power(l2, (float)(n - row - (less ? 1 : 0)))) : 0.0f;
+                    }
                 }
                 if constexpr (sizeof(T) == 2) {
                     bf16x8 f[3];
@@ -239,7 +285,8 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
                     for (int b = 0; b < DP / 16; ++b) {
                         const bf16x8 kf = frag_columns(sk, C::kLd, 32 * t, 16 * b);
 #pragma unroll
-                        for (int m = 2; m >= 0; --m) H[b] = mma(kf, f[m], H[b]);
+                        for (int m = 2; m >= 0; --m)
+                            if (m < 2 || third) H[b] = mma(kf, f[m], H[b]);
                     }
                 } else {
                     f32x8 f;
@@ -252,27 +299,34 @@ __global__ __launch_bounds__(DP * 4) void decay_walk_kernel(WalkArgs<T> a) {
         }
         if (!STATE) {
             __syncthreads();
-            if (!careful) {
+            // Infinities and NaN among the piece's v: only rows behind them may feel them, and 0 * inf is NaN.  They stay out
+            // of the matrix product and are added key by key.
+            if (careful) {
 #pragma unroll
-                for (int rb = 0; rb < 4; ++rb)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int t = 0; t <= rb / 2; ++t) o[rb] = mma(vf[t], frag_split(sp, C::kLdP, 16 * rb, 32 * t), o[rb]);
-            } else {
-                // an infinity or NaN among the piece's v: a matrix product would carry it (0 * inf) to the rows before it
-#pragma unroll
-                for (int rb = 0; rb < 4; ++rb)
-                    for (int key = 0; key <= 16 * rb + c && key < n; ++key)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            o[rb][i] = fmaf((float)sp[(16 * rb + c) * C::kLdP + key], (float)sv[key * C::kLd + 16 * wave + 4 * g + i], o[rb][i]);
+                    for (int j = 0; j < 8; ++j) vf[t][j] = fabsf((float)vf[t][j]) < INFINITY ? vf[t][j] : (T)0.0f;
             }
+#pragma unroll
+            for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+                for (int t = 0; t <= rb / 2; ++t) o[rb] = mma(vf[t], frag_split(sp, C::kLdP, 16 * rb, 32 * t), o[rb]);
+            if (careful) {
+#pragma unroll
+                for (int rb = 0; rb < 4; ++rb)
+#pragma unroll 1
+                    for (int key = 0; key <= 16 * rb + c; ++key)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = (float)sv[key * C::kLd + 16 * wave + 4 * g + i];
+                            if (!(fabsf(x) < INFINITY)) o[rb][i] = fmaf((float)sp[(16 * rb + c) * C::kLdP + key], x, o[rb][i]);
+                        }
+            }
+            T* oc = op + (w.reverse ? len - 1 - tc : tc) * a.heads * dim;
 #pragma unroll
             for (int rb = 0; rb < 4; ++rb) {
                 const int row = 16 * rb + c;
-                if (row < n) {
-                    const int64_t at = w.reverse ? len - 1 - (tc + row) : tc + row;
-                    store_quad(op + at * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], a.wide_out);
-                }
+                if (row < n) store_quad(oc + sign * row * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], wide_out);
             }
         }
         __syncthreads();
@@ -304,10 +358,17 @@ __global__ __launch_bounds__(256) void decay_join_kernel(WalkArgs<T> a) {
     float x = 0.0f;
     if (w.s0) x = w.s0[head * elems + (w.s0_transposed ? e % a.dim * a.dim + e / a.dim : e)] * (w.reverse ? 1.0f : power(l2, 1.0f));
     float* p = a.spans + (((int64_t)blockIdx.y * a.n_seq * a.heads + head) * a.n_spans) * elems + e;
-    for (int64_t u = 0; u < used; ++u, p += elems) {
-        const float own = u + 1 < used ? *p : 0.0f;
-        *p = x;
-        x = fmaf(x, keep, own);
+    constexpr int kAhead = 8;                                // loads in flight; the sums are a chain
+    for (int64_t u = 0; u < used; u += kAhead) {
+        float own[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) own[i] = u + i + 1 < used ? p[(u + i) * elems] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (u + i < used) {
+                p[(u + i) * elems] = x;
+                x = fmaf(x, keep, own[i]);
+            }
     }
 }
 
@@ -379,20 +440,22 @@ int span_count(int64_t n_seq, int64_t max_len, int64_t heads, int walks) {
     return (int)(n < 1 ? 1 : n);
 }
 
-template <typename T>
+template <typename T, int DP>
 int allow_walks() {
-    const void* f[] = {reinterpret_cast<const void*>(&decay_walk_kernel<T, 32, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 32, true>),
-                       reinterpret_cast<const void*>(&decay_walk_kernel<T, 64, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 64, true>),
-                       reinterpret_cast<const void*>(&decay_walk_kernel<T, 128, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, 128, true>)};
-    const size_t lds[] = {WalkShape<T, 32>::kLds, WalkShape<T, 64>::kLds, WalkShape<T, 128>::kLds};
-    for (int i = 0; i < 6; ++i) VAD_HIP_CHECK(hipFuncSetAttribute(f[i], hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds[i / 2]));
+    const void* f[] = {reinterpret_cast<const void*>(&decay_walk_kernel<T, DP, false, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, DP, false, true>),
+                       reinterpret_cast<const void*>(&decay_walk_kernel<T, DP, true, false>), reinterpret_cast<const void*>(&decay_walk_kernel<T, DP, true, true>)};
+    for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)WalkShape<T, DP>::kLds));
     return VAD_OK;
 }
 
 template <typename T, int DP, bool STATE>
 void launch_walk(const WalkArgs<T>& a, int walks, hipStream_t st) {
-    hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE>), dim3((unsigned)(a.n_seq * a.heads * a.n_spans), (unsigned)walks),
-                       dim3((WalkShape<T, DP>::kThreads)), (WalkShape<T, DP>::kLds), st, a);
+    const dim3 grid((unsigned)(a.n_seq * a.heads * a.n_spans), (unsigned)walks), block((WalkShape<T, DP>::kThreads));
+    constexpr size_t lds = WalkShape<T, DP>::kLds;
+    if (a.mode == kWide && a.wide_out)
+        hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE, true>), grid, block, lds, st, a);
+    else
+        hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE, false>), grid, block, lds, st, a);
 }
 template <typename T, bool STATE>
 void launch_walk(const WalkArgs<T>& a, int walks, hipStream_t st) {
@@ -423,16 +486,6 @@ Heads<const T> heads_of(const void* p, const int64_t* strides) {
     return {static_cast<const T*>(p), strides[0], strides[1], strides[2]};
 }
 template <typename T>
-bool wide_rows(const Heads<const T>& x, int dim) {
-    constexpr int VE = Elem<T>::kPer16B;
-    return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.sb % VE == 0 && x.st % VE == 0 && x.sh % VE == 0 && dim % VE == 0;
-}
-template <typename T>
-bool wide_quads(const T* p, int dim) {
-    return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && dim % 4 == 0;
-}
-
-template <typename T>
 int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, Sequences seq,
                 int n_seq, int heads, int dim, const float* log_decay, float scale, const float* s0, void* o, float* s1, int n_spans,
                 float* ws, hipStream_t st) {
@@ -445,8 +498,8 @@ int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* 
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
-    a.wide = wide_rows(a.walk[0].q, dim) && wide_rows(a.walk[0].k, dim) && wide_rows(a.walk[0].v, dim);
-    a.wide_out = wide_quads(static_cast<const T*>(o), dim);
+    a.mode = std::min({load_mode(a.walk[0].q, dim), load_mode(a.walk[0].k, dim), load_mode(a.walk[0].v, dim)});
+    a.wide_out = wide_rows(static_cast<const T*>(o), dim);
     return run_walks(a, 1, st);
 }
 
@@ -466,8 +519,8 @@ int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t*
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
-    a.wide = wide_rows(Q, dim) && wide_rows(K, dim) && wide_rows(V, dim) && wide_rows(G, dim);
-    a.wide_out = wide_quads(static_cast<const T*>(dq), dim) && wide_quads(static_cast<const T*>(dk), dim) && wide_quads(static_cast<const T*>(dv), dim);
+    a.mode = std::min({load_mode(Q, dim), load_mode(K, dim), load_mode(V, dim), load_mode(G, dim)});
+    a.wide_out = wide_rows(static_cast<const T*>(dq), dim) && wide_rows(static_cast<const T*>(dk), dim) && wide_rows(static_cast<const T*>(dv), dim);
     return run_walks(a, 3, st);
 }
 
@@ -477,6 +530,12 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(heads >= 1, "heads must be positive, got %d", heads);
     VAD_REQUIRE(n_seq >= 0 && n_tokens >= 0 && max_len >= 0, "negative sequence count or length");
     VAD_REQUIRE(n_seq <= 0x7FFFFFFF / heads / 64, "too many sequences for one launch");
+    VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
+    return VAD_OK;
+}
+
+int check_rows(const int64_t* strides) {
+    VAD_REQUIRE(strides[1] >= 0 && strides[1] < VAD_MAX_ROW_STRIDE, "row stride %lld out of range", (long long)strides[1]);
     return VAD_OK;
 }
 
@@ -491,10 +550,10 @@ int ensure_linear_attention_attrs() {
     VAD_REQUIRE(dev >= 0 && dev < 64, "device index %d out of range", dev);
     std::lock_guard<std::mutex> lock(mu);
     if (done[dev]) return VAD_OK;
-    int rc = allow_walks<float>();
-    if (rc != VAD_OK) return rc;
-    rc = allow_walks<__bf16>();
-    if (rc != VAD_OK) return rc;
+    int rc = VAD_OK;
+    if ((rc = allow_walks<float, 32>()) != VAD_OK || (rc = allow_walks<float, 64>()) != VAD_OK || (rc = allow_walks<float, 128>()) != VAD_OK ||
+        (rc = allow_walks<__bf16, 32>()) != VAD_OK || (rc = allow_walks<__bf16, 64>()) != VAD_OK || (rc = allow_walks<__bf16, 128>()) != VAD_OK)
+        return rc;
     done[dev] = true;
     return VAD_OK;
 }
@@ -520,6 +579,8 @@ extern "C" int vad_linear_attention_forward(const void* q_dev, const int64_t* q_
     const bool empty = starts_dev ? n_tokens == 0 : max_len == 0;
     VAD_REQUIRE(empty || (q_dev && k_dev && v_dev && o_dev), "null pointer argument");
     VAD_REQUIRE(!state_in_dev || state_in_dev != state_out_dev, "state_out must not be state_in");
+    for (const int64_t* strides : {q_strides, k_strides, v_strides})
+        if ((rc = check_rows(strides)) != VAD_OK) return rc;
     const size_t need = vad_linear_attention_workspace_bytes(n_seq, max_len, heads, dim, 0);
     VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
     rc = ensure_linear_attention_attrs();
@@ -549,6 +610,8 @@ extern "C" int vad_linear_attention_backward(const void* q_dev, const int64_t* q
     const bool empty = starts_dev ? n_tokens == 0 : max_len == 0;
     VAD_REQUIRE(empty || (q_dev && k_dev && v_dev && do_dev && dq_dev && dk_dev && dv_dev), "null pointer argument");
     VAD_REQUIRE(!dstate_out_dev || dstate_out_dev != dstate_in_dev, "dstate_in must not be dstate_out");
+    for (const int64_t* strides : {q_strides, k_strides, v_strides, do_strides})
+        if ((rc = check_rows(strides)) != VAD_OK) return rc;
     const size_t need = vad_linear_attention_workspace_bytes(n_seq, max_len, heads, dim, 1);
     VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
     rc = ensure_linear_attention_attrs();

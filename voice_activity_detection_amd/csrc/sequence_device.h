@@ -13,6 +13,8 @@
 #pragma once
 #include <math.h>
 
+#include <algorithm>
+
 #include "vad_internal.h"
 
 namespace vad {
@@ -24,6 +26,10 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+// global memory takes 16-byte accesses at any 4-byte boundary
+typedef u32x4 u32x4_any __attribute__((aligned(4)));
+typedef u32x2 u32x2_any __attribute__((aligned(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -56,6 +62,61 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
 }
 
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & 63); }
+
+// ---- across lanes, without the LDS unit ----
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
+}
+// The values that lanes i and i ^ 16 (i ^ 32) hold, the same pair in both: the swap exchanges the odd half of its first
+// operand's lanes with the even half of its second's.  (The results are copied out before the cast: a bit cast of a
+// vector's element reads element 0.)
+template <int DISTANCE>
+__device__ __forceinline__ void lane_pair(float x, float& a, float& b) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    unsigned first, second;
+    if (DISTANCE == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        first = r[0], second = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        first = r[0], second = r[1];
+    }
+    a = __builtin_bit_cast(float, first);
+    b = __builtin_bit_cast(float, second);
+}
+// Sum over aligned groups of `lanes` lanes (a power of two, uniform), the same value in each.
+__device__ __forceinline__ float lanes_sum(float x, int lanes) {
+    if (lanes > 1) x += dpp<0xB1>(x);           // lane ^ 1
+    if (lanes > 2) x += dpp<0x4E>(x);           // lane ^ 2
+    if (lanes > 4) x += dpp<0x141>(x);          // the other quad of the half row
+    if (lanes > 8) x += dpp<0x140>(x);          // the other half of the row
+    if (lanes > 16) {
+        float a, b;
+        lane_pair<16>(x, a, b);
+        x = a + b;
+    }
+    if (lanes > 32) {
+        float a, b;
+        lane_pair<32>(x, a, b);
+        x = a + b;
+    }
+    return x;
+}
+// Over the four lanes that hold the same column of a result tile.
+__device__ __forceinline__ float groups_sum(float x) {
+    float a, b;
+    lane_pair<16>(x, a, b);
+    lane_pair<32>(a + b, a, b);
+    return a + b;
+}
+__device__ __forceinline__ float groups_max(float x) {
+    float a, b;
+    lane_pair<16>(x, a, b);
+    lane_pair<32>(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
 
 // ---- rows in global memory ----
 
@@ -105,14 +166,21 @@ __device__ __forceinline__ T* head_ptr(const Heads<T>& x, const Sequences& q, in
     return x.p + (q.starts ? first * x.st : (int64_t)s * x.sb) + (int64_t)h * x.sh;
 }
 
-// 16 bytes of a row from column c; columns from `cols` on read as zero.  `wide`: rows start 16-byte aligned and cols is
-// a multiple of a 16-byte piece (uniform over the launch).
+// 16 bytes of a row from column c; columns from `cols` on read as zero.  The mode is uniform over the launch: kWide where
+// rows start 4-byte aligned and cols is a multiple of a 16-byte piece, kHalf where it is one of 8 bytes, else kScalar,
+// element by element.
+enum { kScalar = 0, kHalf = 1, kWide = 2 };
 template <typename T>
-__device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, bool wide) {
+__device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, int mode) {
     constexpr int VE = Elem<T>::kPer16B;
     u32x4 r = {0, 0, 0, 0};
-    if (wide) {
-        if (c < cols) r = *reinterpret_cast<const u32x4*>(row + c);
+    if (mode != kScalar) {
+        if (c + VE <= cols) {
+            r = *reinterpret_cast<const u32x4_any*>(row + c);
+        } else if (mode == kHalf && c < cols) {
+            const u32x2 a = *reinterpret_cast<const u32x2_any*>(row + c);
+            r = u32x4{a[0], a[1], 0, 0};
+        }
     } else {
         T v[VE];
 #pragma unroll
@@ -120,6 +188,27 @@ __device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, bool 
         __builtin_memcpy(&r, v, 16);
     }
     return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_piece(T* row, int c, int cols, u32x4 v, int mode) {
+    constexpr int VE = Elem<T>::kPer16B;
+    if (mode != kScalar && c + VE <= cols) {
+        *reinterpret_cast<u32x4_any*>(row + c) = v;
+    } else {
+        T e[VE];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+            if (c + i < cols) row[c + i] = e[i];
+    }
+}
+
+template <typename T>
+int load_mode(const Heads<T>& x, int dim) {
+    constexpr int VE = 16 / sizeof(T);
+    const uint64_t at = reinterpret_cast<uintptr_t>(x.p) | (uint64_t)(x.sb * sizeof(T)) | (uint64_t)(x.st * sizeof(T)) | (uint64_t)(x.sh * sizeof(T));
+    return at % 4 ? kScalar : (dim % VE == 0 ? kWide : (dim % (VE / 2) == 0 ? kHalf : kScalar));
 }
 
 // Whether any of the values in a 16-byte piece is an infinity or a NaN.
@@ -138,13 +227,13 @@ __device__ __forceinline__ bool piece_not_finite(u32x4 v) {
 
 // A natural-order fragment straight from global memory: this lane's row, columns c .. c + 7.
 template <typename T>
-__device__ __forceinline__ Frag<T> load_row_frag(const T* row, bool live, int c, int cols, bool wide) {
+__device__ __forceinline__ Frag<T> load_row_frag(const T* row, bool live, int c, int cols, int mode) {
     Frag<T> f;
     u32x4 v[sizeof(Frag<T>) / 16];
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(Frag<T>) / 16); ++i) {
         v[i] = u32x4{0, 0, 0, 0};
-        if (live) v[i] = load_piece(row, c + i * Elem<T>::kPer16B, cols, wide);
+        if (live) v[i] = load_piece(row, c + i * Elem<T>::kPer16B, cols, mode);
     }
     __builtin_memcpy(&f, v, sizeof(f));
     return f;
@@ -212,6 +301,25 @@ __device__ __forceinline__ f32x8 frag_columns(const float* tile, int ld, int r0,
     return f;
 }
 
+// An operand's infinities and NaN taken out: they become zero, and `code` holds 1 for each +inf, 2^7 for each -inf, 2^14
+// for each NaN.  A product of `code` with zeros and ones adds them up exactly (64 terms); code_value turns the sum back
+// into what the values themselves would have contributed.
+template <typename T>
+__device__ __forceinline__ void take_out(Frag<T>& x, Frag<T>& code) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = (float)x[j];
+        const bool fine = fabsf(v) < INFINITY;
+        code[j] = (T)(fine ? 0.0f : (v == INFINITY ? 1.0f : (v == -INFINITY ? 128.0f : 16384.0f)));
+        x[j] = fine ? x[j] : (T)0.0f;
+    }
+}
+__device__ __forceinline__ float code_value(float n) {
+    const int c = (int)n;
+    const float plus = (c & 127) ? INFINITY : 0.0f, minus = (c & (127 << 7)) ? -INFINITY : 0.0f;
+    return c >= 1 << 14 ? NAN : plus + minus;
+}
+
 // Two stacked result tiles as an operand in split order.
 __device__ __forceinline__ void to_frag(f32x4 a, f32x4 b, bf16x8& f) {
 #pragma unroll
@@ -228,21 +336,31 @@ __device__ __forceinline__ void to_frag(f32x4 a, f32x4 b, f32x8& f) {
     }
 }
 
-// Four consecutive values of an output row; `wide`: the row and its columns allow one store.
+// Four consecutive values of an output row; `wide`: rows start 4-byte aligned (wide_rows).
 template <typename T>
 __device__ __forceinline__ void store_quad(T* row, int c, int cols, f32x4 v, bool wide) {
-    if (wide) {
-        if (c < cols) {
-            Quad<T> q;
+    if (wide && c + 4 <= cols) {
+        T q[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
-            *reinterpret_cast<Quad<T>*>(row + c) = q;
+        for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+        if (sizeof(T) == 4) {
+            u32x4 r;
+            __builtin_memcpy(&r, q, 16);
+            *reinterpret_cast<u32x4_any*>(row + c) = r;
+        } else {
+            u32x2 r;
+            __builtin_memcpy(&r, q, 8);
+            *reinterpret_cast<u32x2_any*>(row + c) = r;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (c + i < cols) row[c + i] = (T)v[i];
     }
+}
+template <typename T>
+bool wide_rows(const T* p, int dim) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim * sizeof(T) % 4 == 0;
 }
 
 }  // namespace sq

@@ -43,85 +43,84 @@ struct WindowArgs {
     Sequences seq;
     int n_seq, heads, kv_heads, dim, window, sinks, segments;
     float scale;
-    bool wide, wide_out;
+    int mode;                       // how rows of q, k, v, dO are read
+    bool wide_out;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int NT = kThreads>
 struct TileShape {
     static constexpr int kLd = DP + Elem<T>::kPer16B;
-    static constexpr int kPieces = kTile * DP / Elem<T>::kPer16B / kThreads;
+    static constexpr int kPieces = kTile * DP / Elem<T>::kPer16B / NT;
     static constexpr int kPPR = DP / Elem<T>::kPer16B;
     static constexpr size_t kLds = (size_t)2 * kTile * kLd * sizeof(T) + (3 * kTile + 4) * sizeof(float);
 };
 
 // 64 rows from t0 on of one head, rows from len on as zero
-template <typename T, int DP>
+template <typename T, int DP, int NT>
 struct Staged {
-    u32x4 r[TileShape<T, DP>::kPieces];
-    __device__ __forceinline__ void fetch(const T* p, int64_t st, int t0, int len, int dim, bool wide) {
-        using C = TileShape<T, DP>;
+    using C = TileShape<T, DP, NT>;
+    u32x4 r[C::kPieces];
+    __device__ __forceinline__ void fetch(const T* p, int64_t st, int t0, int len, int dim, int mode) {
 #pragma unroll
         for (int n = 0; n < C::kPieces; ++n) {
-            const int i = threadIdx.x + n * kThreads, row = i / C::kPPR;
+            const int i = threadIdx.x + n * NT, row = i / C::kPPR;
             r[n] = u32x4{0, 0, 0, 0};
-            if (t0 + row < len) r[n] = load_piece(p + (int64_t)(t0 + row) * st, i % C::kPPR * Elem<T>::kPer16B, dim, wide);
+            if (t0 + row < len) r[n] = load_piece(p + (int64_t)(t0 + row) * st, i % C::kPPR * Elem<T>::kPer16B, dim, mode);
         }
     }
     __device__ __forceinline__ void put(T* tile) const {
-        using C = TileShape<T, DP>;
 #pragma unroll
         for (int n = 0; n < C::kPieces; ++n) {
-            const int i = threadIdx.x + n * kThreads;
+            const int i = threadIdx.x + n * NT;
             *reinterpret_cast<u32x4*>(tile + i / C::kPPR * C::kLd + i % C::kPPR * Elem<T>::kPer16B) = r[n];
         }
     }
     __device__ __forceinline__ bool not_finite() const {
         bool bad = false;
 #pragma unroll
-        for (int n = 0; n < TileShape<T, DP>::kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
+        for (int n = 0; n < C::kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
         return bad;
     }
 };
 
 // acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
-// own row.  `careful`: only rows that `sees` admits are touched.
+// own row.  `careful`: the tile holds infinities or NaN, which only rows that `sees` admits may feel (0 * inf is NaN).
 template <typename T, int DP, int NB, typename Sees>
 __device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB], f32x4 (&acc)[DP / 16][NB], bool careful, Sees sees) {
     constexpr int kLd = TileShape<T, DP>::kLd;
-    if (!careful) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            Frag<T> f[NB];
+    for (int t = 0; t < 2; ++t) {
+        Frag<T> f[NB];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
+        for (int nb = 0; nb < NB; ++nb) to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
+        if (!careful) {
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) {
                 const Frag<T> x = frag_columns(tile, kLd, 32 * t, 16 * b);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) acc[b][nb] = mma(x, f[nb], acc[b][nb]);
             }
-        }
-        return;
-    }
-    const int l = lane_id(), g = l >> 4;
+        } else {
+            const int g = lane_id() >> 4;
+            Frag<T> seen[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
+                for (int j = 0; j < 8; ++j) seen[nb][j] = (T)(sees(32 * t + 4 * g + (j < 4 ? j : 12 + j), nb) ? 1.0f : 0.0f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll 1
-                for (int gg = 0; gg < 4; ++gg) {
-                    const float w = __shfl(p[kb][nb][i], (l & 15) + 16 * gg);
-                    const int row = 16 * kb + 4 * gg + i;
-                    if (sees(row, nb)) {
+            for (int b = 0; b < DP / 16; ++b) {
+                Frag<T> x = frag_columns(tile, kLd, 32 * t, 16 * b), code;
+                take_out<T>(x, code);
 #pragma unroll
-                        for (int b = 0; b < DP / 16; ++b)
+                for (int nb = 0; nb < NB; ++nb) {
+                    const f32x4 n = mma(code, seen[nb], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    acc[b][nb] = mma(x, f[nb], acc[b][nb]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[b][nb][e] = fmaf(w, (float)tile[row * kLd + 16 * b + 4 * g + e], acc[b][nb][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[b][nb][e] += code_value(n[e]);
                 }
+            }
+        }
+    }
 }
 
 // s = tile own^T for the 64 streamed rows
@@ -140,15 +139,6 @@ __device__ __forceinline__ void scores(const T* tile, const Frag<T> (&own)[NB][D
     }
 }
 
-__device__ __forceinline__ float across_groups_max(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float across_groups_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
 // The key tiles that rows r0 .. r1 see: the first sink tile if it lies before the band, then the band's.
 struct KeyTiles {
     int band, end;                  // first rows of the band's first tile, and past its last
@@ -165,7 +155,7 @@ struct KeyTiles {
 
 // BACK == false: O and stats.  BACK == true: dQ and delta.
 template <typename T, int DP, int NB, bool BACK>
-__global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) {
+__global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> a) {
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
     T* sk = reinterpret_cast<T*>(lds_raw);
@@ -197,7 +187,7 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
             const int row = w0 + 16 * nb + c;
             const bool live = row < len;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) qf[nb][d] = load_row_frag<T>(qp + (int64_t)row * a.q.st, live, 32 * d + 8 * g, dim, a.wide);
+            for (int d = 0; d < DP / 32; ++d) qf[nb][d] = load_row_frag<T>(qp + (int64_t)row * a.q.st, live, 32 * d + 8 * g, dim, a.mode);
             m[nb] = -INFINITY;
             sum[nb] = 0.0f;
             if (BACK) {
@@ -205,12 +195,12 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
                 float x = 0.0f;
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
-                    gf[nb][d] = load_row_frag<T>(gp + (int64_t)row * a.go.st, live, 32 * d + 8 * g, dim, a.wide);
-                    const Frag<T> of = load_row_frag<T>(a.o + at * dim, live, 32 * d + 8 * g, dim, a.wide_out);
+                    gf[nb][d] = load_row_frag<T>(gp + (int64_t)row * a.go.st, live, 32 * d + 8 * g, dim, a.mode);
+                    const Frag<T> of = load_row_frag<T>(a.o + at * dim, live, 32 * d + 8 * g, dim, a.mode);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x = fmaf((float)gf[nb][d][j], (float)of[j], x);
                 }
-                delta[nb] = across_groups_sum(x);
+                delta[nb] = groups_sum(x);
                 m[nb] = live ? a.stats[2 * at] : 0.0f;
                 sum[nb] = live ? a.stats[2 * at + 1] : 0.0f;
                 if (live && g == 0) a.delta[at] = delta[nb];
@@ -219,9 +209,9 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
             for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const KeyTiles tiles(r0, r1, a.window, a.sinks);
-        Staged<T, DP> rk, rv;
-        rk.fetch(kp, a.k.st, tiles.first(), len, dim, a.wide);
-        rv.fetch(vp, a.v.st, tiles.first(), len, dim, a.wide);
+        Staged<T, DP, kThreads> rk, rv;
+        rk.fetch(kp, a.k.st, tiles.first(), len, dim, a.mode);
+        rv.fetch(vp, a.v.st, tiles.first(), len, dim, a.mode);
         for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), turn ^= 1) {
             __syncthreads();                                   // the tile before is read
             rk.put(sk);
@@ -233,8 +223,8 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
             if (threadIdx.x == 0) flags[turn ^ 1] = 0;
             const int nt = tiles.next(t);
             if (nt < tiles.end) {
-                rk.fetch(kp, a.k.st, nt, len, dim, a.wide);
-                rv.fetch(vp, a.v.st, nt, len, dim, a.wide);
+                rk.fetch(kp, a.k.st, nt, len, dim, a.mode);
+                rv.fetch(vp, a.v.st, nt, len, dim, a.mode);
             }
             if (t > w1 || (w0 - (t + kTile - 1) >= a.window && t >= a.sinks)) continue;      // nothing for this wave
             f32x4 p[4][NB];
@@ -260,7 +250,7 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
                     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, p[kb][nb][i]);
-                    const float now = fmaxf(m[nb], across_groups_max(top) * l2scale);
+                    const float now = fmaxf(m[nb], groups_max(top) * l2scale);
                     const float base = now == -INFINITY ? 0.0f : now;
                     const float shrink = __builtin_amdgcn_exp2f(m[nb] - base);
                     m[nb] = now;
@@ -298,7 +288,7 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
             const int64_t at = (row_base + row) * a.heads + h;
             float f = 1.0f;
             if (!BACK) {
-                f = 1.0f / across_groups_sum(sum[nb]);
+                f = 1.0f / groups_sum(sum[nb]);
                 if (a.stats && row < len && g == 0) {
                     a.stats[2 * at] = m[nb];
                     a.stats[2 * at + 1] = f;
@@ -314,9 +304,12 @@ __global__ __launch_bounds__(kThreads) void window_rows_kernel(WindowArgs<T> a) 
 
 // dK and dV.  SINKS == false: the block's keys against the rows of their window.  SINKS == true: the sink keys against the
 // rows beyond their window, one segment of the rows.
+//
+// The sink keys are few: there a block is one wave with 16 of them, blocks take turns at the segments.
 template <typename T, int DP, int NB, bool SINKS>
-__global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) {
-    using C = TileShape<T, DP>;
+__global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(WindowArgs<T> a) {
+    constexpr int NT = SINKS ? 64 : kThreads;
+    using C = TileShape<T, DP, NT>;
     extern __shared__ char lds_raw[];
     T* sqr = reinterpret_cast<T*>(lds_raw);
     T* sgo = sqr + kTile * C::kLd;
@@ -325,6 +318,7 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
     float* sdelta = sinv + kTile;
     int* flags = reinterpret_cast<int*>(sdelta + kTile);
     const int hk = blockIdx.y, s = blockIdx.z, group = a.heads / a.kv_heads;
+    const int segment = SINKS ? blockIdx.x % a.segments : 0;
     int64_t first, len64;
     sequence_rows(a.seq, s, first, len64);
     const int len = (int)len64, dim = a.dim;
@@ -333,15 +327,15 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
     const T* vp = head_ptr(a.v, a.seq, s, first, hk);
     const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
     const float l2scale = a.scale * kLog2e;
-    constexpr int kKeys = 64 * NB;
+    constexpr int kKeys = NT / 4 * NB;
     if (!SINKS) {
         zero_outside(a.dk, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
         zero_outside(a.dv, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
     }
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     int turn = 0;
-    for (int64_t j0_64 = SINKS ? 0 : (int64_t)blockIdx.x * kKeys; j0_64 < (SINKS ? (len < 1 ? len : 1) : len);
-         j0_64 += SINKS ? 1 : (int64_t)gridDim.x * kKeys) {
+    // (the sink keys' blocks take one turn)
+    for (int64_t j0_64 = (SINKS ? blockIdx.x / a.segments : (int64_t)blockIdx.x) * kKeys; j0_64 < len; j0_64 += SINKS ? len : (int64_t)gridDim.x * kKeys) {
         const int j0 = (int)j0_64;
         const int w0 = j0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
         // the rows [i0, i1) that see the keys
@@ -349,7 +343,7 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
         if (SINKS) {
             const int beyond = len > a.window ? len - a.window : 0;
             const int per = ((beyond + a.segments - 1) / a.segments + kTile - 1) / kTile * kTile;
-            const int64_t lo = a.window + (int64_t)blockIdx.x * per;
+            const int64_t lo = a.window + (int64_t)segment * per;
             i0 = (int)(lo < len ? lo : len);
             i1 = (int)(lo + per < len ? lo + per : len);
         } else {
@@ -365,19 +359,19 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
             const bool live = key < keys;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) {
-                kf[nb][d] = load_row_frag<T>(kp + (int64_t)key * a.k.st, live, 32 * d + 8 * g, dim, a.wide);
-                vf[nb][d] = load_row_frag<T>(vp + (int64_t)key * a.v.st, live, 32 * d + 8 * g, dim, a.wide);
+                kf[nb][d] = load_row_frag<T>(kp + (int64_t)key * a.k.st, live, 32 * d + 8 * g, dim, a.mode);
+                vf[nb][d] = load_row_frag<T>(vp + (int64_t)key * a.v.st, live, 32 * d + 8 * g, dim, a.mode);
             }
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) dk[b][nb] = dv[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
-        Staged<T, DP> rq, rg;
-        float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;
+        Staged<T, DP, NT> rq, rg;
+        float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;          // of row threadIdx.x of the tile
         const auto fetch = [&](int step) {
             const int h = hk * group + step / n_tiles, t = i0 + step % n_tiles * kTile;
-            rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1, dim, a.wide);
-            rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1, dim, a.wide);
+            rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1, dim, a.mode);
+            rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1, dim, a.mode);
             const int row = t + threadIdx.x;
             if (threadIdx.x < kTile) {
                 const int64_t at = (row_base + row) * a.heads + h;
@@ -387,9 +381,10 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
             }
         };
         const int steps = n_tiles * group;
-        if (steps) fetch(0);
+        if (steps && !SINKS) fetch(0);
         for (int step = 0; step < steps; ++step, turn ^= 1) {
             const int t = i0 + step % n_tiles * kTile;
+            if (SINKS) fetch(step);                // one wave: its registers hold no tile ahead, other blocks hide the wait
             __syncthreads();
             rq.put(sqr);
             rg.put(sgo);
@@ -403,7 +398,7 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
             __syncthreads();
             const bool careful = edge && flags[turn];
             if (threadIdx.x == 0) flags[turn ^ 1] = 0;
-            if (step + 1 < steps) fetch(step + 1);
+            if (!SINKS && step + 1 < steps) fetch(step + 1);
             if (w0 >= keys || (!SINKS && (t + kTile - 1 < w0 || t - w1 >= a.window))) continue;
             const auto sees = [&](int row, int nb) {
                 const int i = t + row, j = w0 + 16 * nb + c;
@@ -436,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
             const int key = w0 + 16 * nb + c;
             if (key < a.sinks && key < len) {
                 // a sink key's sums go to the joining kernel in float32: [0] of its window, [1 + n] of segment n
-                float* out = a.parts + (((((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + blockIdx.x : 0)) * 2) * a.sinks + key) * dim;
+                float* out = a.parts + (((((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + segment : 0)) * 2) * a.sinks + key) * dim;
 #pragma unroll
                 for (int b = 0; b < DP / 16; ++b) {
                     store_quad(out, 16 * b + 4 * g, dim, dk[b][nb], false);
@@ -451,7 +446,6 @@ __global__ __launch_bounds__(kThreads) void window_keys_kernel(WindowArgs<T> a) 
                 }
             }
         }
-        if (SINKS) break;
     }
 }
 
@@ -486,7 +480,7 @@ struct StepArgs {
     float* parts;                   // (batch, head, split): maximum, sum, dim values
     int heads, kv_heads, dim, window, sinks, splits, chunks;
     float scale;
-    bool wide;
+    int mode;                       // how rows of k, v and the caches are read
 };
 
 // A wave takes 64 / (lanes of a row) slots at a time; a lane keeps 16 bytes of the row for each of GB query heads.
@@ -530,20 +524,11 @@ __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
             kr[u] = vr[u] = u32x4{0, 0, 0, 0};
             if (slot < hi) {
                 const bool mine = slot == own;
-                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.wide);
-                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.wide);
-                if (mine && chunk == 0) {
-                    if (a.wide) {
-                        if (d < a.dim) {
-                            *reinterpret_cast<u32x4*>(ck + slot * a.ck.st + d) = kr[u];
-                            *reinterpret_cast<u32x4*>(cv + slot * a.cv.st + d) = vr[u];
-                        }
-                    } else {
-                        for (int e = 0; e < VE && d + e < a.dim; ++e) {
-                            ck[slot * a.ck.st + d + e] = kn[d + e];
-                            cv[slot * a.cv.st + d + e] = vn[d + e];
-                        }
-                    }
+                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.mode);
+                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.mode);
+                if (mine && chunk == 0) {       // the slot is read from the new row above, by every chunk
+                    store_piece(ck + slot * a.ck.st, d, a.dim, kr[u], a.mode);
+                    store_piece(cv + slot * a.cv.st, d, a.dim, vr[u], a.mode);
                 }
             }
         }
@@ -674,26 +659,14 @@ __global__ __launch_bounds__(kThreads) void window_fill_kernel(StepArgs<T> a, Se
             row = at < rolled ? a.sinks + at + (rolled - 1 - at) / a.window * a.window : len;
         }
         if (row >= len) continue;
-        if (a.wide) {
-            *reinterpret_cast<u32x4*>(ck + slot * a.ck.st + d) = load_piece(kp + row * a.k.st, d, a.dim, true);
-            *reinterpret_cast<u32x4*>(cv + slot * a.cv.st + d) = load_piece(vp + row * a.v.st, d, a.dim, true);
-        } else {
-            for (int e = d; e < d + Elem<T>::kPer16B && e < a.dim; ++e) {
-                ck[slot * a.ck.st + e] = kp[row * a.k.st + e];
-                cv[slot * a.cv.st + e] = vp[row * a.v.st + e];
-            }
-        }
+        store_piece(ck + slot * a.ck.st, d, a.dim, load_piece(kp + row * a.k.st, d, a.dim, a.mode), a.mode);
+        store_piece(cv + slot * a.cv.st, d, a.dim, load_piece(vp + row * a.v.st, d, a.dim, a.mode), a.mode);
     }
 }
 
 template <typename T>
 Heads<const T> heads_of(const void* p, const int64_t* s) {
     return {static_cast<const T*>(p), s[0], s[1], s[2]};
-}
-template <typename T>
-bool wide_rows(const Heads<T>& x, int dim) {
-    constexpr int VE = 16 / sizeof(T);
-    return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && x.sb % VE == 0 && x.st % VE == 0 && x.sh % VE == 0 && dim % VE == 0;
 }
 
 template <typename T>
@@ -734,7 +707,7 @@ int run_backward(WindowArgs<T> a, hipStream_t st) {
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, true>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), block, lds, st, a);
         hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, lds, st, a);
         if (a.sinks > 0) {
-            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true>), dim3(a.segments, a.kv_heads, a.n_seq), block, lds, st, a);
+            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true>), dim3(a.segments * ((a.sinks + 15) / 16), a.kv_heads, a.n_seq), dim3(64), lds, st, a);
             hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
         }
     });
@@ -751,11 +724,12 @@ int allow_tiles() {
     return VAD_OK;
 }
 
-// Segments of the rows beyond the window for the sink keys' gradients: at least 512 rows each, enough blocks to fill the chip.
+// Segments of the rows beyond the window for the sink keys' gradients: at least 128 rows each, enough one-wave blocks to fill
+// the chip.
 int sink_segments(int64_t n_seq, int64_t max_len, int kv_heads, int window) {
     const int64_t beyond = max_len > window ? max_len - window : 0, blocks = n_seq * kv_heads;
-    int64_t n = (512 + blocks - 1) / blocks;
-    if (n > beyond / 512) n = beyond / 512;
+    int64_t n = (2048 + blocks - 1) / blocks;
+    if (n > beyond / 128) n = beyond / 128;
     return (int)(n < 1 ? 1 : n);
 }
 
@@ -767,6 +741,7 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(sinks >= 0 && sinks <= VAD_MAX_SINKS, "sinks %d out of range 0..%d", sinks, VAD_MAX_SINKS);
     VAD_REQUIRE(n_seq >= 0 && n_seq <= 65535, "sequence count %lld out of range 0..65535", (long long)n_seq);
     VAD_REQUIRE(n_tokens >= 0 && max_len >= 0 && n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
+    VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
     return VAD_OK;
 }
 
@@ -814,8 +789,8 @@ extern "C" int vad_window_attention_forward(const void* q_dev, const int64_t* q_
         a.seq = {starts_dev, n_tokens, max_len};
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
-        a.wide = wide_rows(a.q, dim) && wide_rows(a.k, dim) && wide_rows(a.v, dim);
-        a.wide_out = reinterpret_cast<uintptr_t>(o_dev) % 16 == 0 && dim % (16 / sizeof(T)) == 0;
+        a.mode = std::min({load_mode(a.q, dim), load_mode(a.k, dim), load_mode(a.v, dim)});
+        a.wide_out = wide_rows(a.out, dim);
         return run_forward<T>(a, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -866,9 +841,9 @@ extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
         a.segments = sink_segments(n_seq, max_len, kv_heads, (int)window);
-        a.wide = wide_rows(a.q, dim) && wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.go, dim);
-        a.wide_out = (reinterpret_cast<uintptr_t>(o_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
-                      reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0 && dim % (16 / sizeof(T)) == 0;
+        const Heads<const T> o = {a.o, 0, (int64_t)heads * dim, dim};
+        a.mode = std::min({load_mode(a.q, dim), load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.go, dim), load_mode(o, dim)});
+        a.wide_out = wide_rows(a.out, dim) && wide_rows(a.dk, dim) && wide_rows(a.dv, dim);
         return run_backward<T>(a, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -948,7 +923,7 @@ extern "C" int vad_window_attention_step(const void* q_dev, const int64_t* q_str
         const int group = heads / kv_heads, gb = step_heads(group);
         a.chunks = (group + gb - 1) / gb;
         a.splits = step_splits(batch, kv_heads, a.chunks, sinks + window);
-        a.wide = wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.ck, dim) && wide_rows(a.cv, dim);
+        a.mode = std::min({load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.ck, dim), load_mode(a.cv, dim)});
         return run_step<T>(a, batch, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -973,7 +948,7 @@ extern "C" int vad_window_cache_fill(const void* k_dev, const int64_t* k_strides
         a.ck = {static_cast<T*>(cache_k_dev), cache_k_strides[0], cache_k_strides[1], cache_k_strides[2]};
         a.cv = {static_cast<T*>(cache_v_dev), cache_v_strides[0], cache_v_strides[1], cache_v_strides[2]};
         a.kv_heads = kv_heads, a.dim = dim, a.window = (int)window, a.sinks = sinks;
-        a.wide = wide_rows(a.k, dim) && wide_rows(a.v, dim) && wide_rows(a.ck, dim) && wide_rows(a.cv, dim);
+        a.mode = std::min({load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.ck, dim), load_mode(a.cv, dim)});
         const Sequences seq = {starts_dev, n_tokens, max_len};
         const int64_t blocks = (((int64_t)sinks + window) * dim * sizeof(T) / 16 + kThreads) / kThreads;
         hipLaunchKernelGGL((window_fill_kernel<T>), dim3((unsigned)(blocks < 256 ? blocks : 256), kv_heads, (unsigned)n_seq), dim3(kThreads), 0,

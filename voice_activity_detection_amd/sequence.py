@@ -13,16 +13,24 @@ runs on the current stream of the tensors' device, allocates only through torch,
 captured into a HIP graph after ``init()``.
 """
 import ctypes
+import functools
 import math
+import operator
 
 import torch
+from torch._C import _cuda_getCurrentRawStream
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 MAX_HEAD_DIM = 128
 MAX_SINKS = 64
+MAX_ROW_STRIDE = 1 << 24
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+# A call's host time is a good part of a live frame's: what follows from shapes and strides alone (checks, stride tables,
+# workspace sizes) is worked out once per shape and remembered by it; checks that touch the tensors are spelled out inline
+# and explained only after they have failed.
 
 
 def _ptr(t):
@@ -33,26 +41,19 @@ def _strides(*s):
     return (ctypes.c_int64 * len(s))(*s)
 
 
-class _on:
-    """The device of a tensor as the current one, where it is not; yields its current stream."""
-
-    def __init__(self, t):
-        self.device = t.device
-        self.guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.device.index:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _call(fn, device, *args):
+    """fn on the current stream of ``device`` (an index), with that device as the current one."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc)
 
 
-def _scratch(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def _scratch(n, like):
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
 
 
 def _check_tensor(name, t, dtype=None, device=None):
@@ -67,8 +68,28 @@ def _check_tensor(name, t, dtype=None, device=None):
         raise ValueError('%s is on %s, expected %s' % (name, t.device, device))
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _check_like(q, k, v):
+    """q, k and v: CUDA tensors of one device and type."""
+    if type(q) is type(k) is type(v) is torch.Tensor and q.is_cuda and q.dtype in _DTYPES and q.dtype is k.dtype is v.dtype \
+            and q.get_device() == k.get_device() == v.get_device():
+        return
+    _check_tensor('q', q)
+    _check_tensor('k', k, q.dtype, q.device)
+    _check_tensor('v', v, q.dtype, q.device)
+
+
+def _dense(t):
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _once(backward):
+    """A backward pass that raises where its results are differentiated again, without once_differentiable's cost where the
+    graph is not kept for that."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 # ---- layer norm ----
@@ -86,35 +107,43 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     for name, p in (('weight', weight), ('bias', bias)):
         if p is None:
             continue
-        _check_tensor(name, p, device=x.device)
-        if tuple(p.shape) != (x.size(-1),):
+        _check_tensor(name, p, p.dtype if isinstance(p, torch.Tensor) else None)
+        if p.get_device() != x.get_device():
+            raise ValueError('%s is on %s, expected %s' % (name, p.device, x.device))
+        if p.dim() != 1 or p.size(0) != x.size(-1):
             raise ValueError('%s must have shape (%d,), got %s' % (name, x.size(-1), tuple(p.shape)))
-        if p.dtype not in (torch.float32, x.dtype):
+        if p.dtype is not torch.float32 and p.dtype is not x.dtype:
             raise ValueError('%s must be float32 or %s, got %s' % (name, x.dtype, p.dtype))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise ValueError('weight and bias must have the same type')
-    if _wants_grad(x, weight, bias):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _norm_forward(x, weight, bias, eps, False)[0]
 
 
 def _as_rows(x):
     """(rows, cols) with dense columns: a view of x where its strides allow, else a copy."""
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x
     rows = x.reshape(-1, x.size(-1)) if x.numel() else x.new_empty((x.numel() // x.size(-1), x.size(-1)))
     return rows if rows.stride(1) == 1 or rows.size(1) == 1 else rows.contiguous()
 
 
 def _norm_forward(x, weight, bias, eps, keep):
     rows = _as_rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows.size(0), 2), dtype=torch.float32, device=x.device) if keep else None
-    weight = weight if weight is None else weight.contiguous()
-    bias = bias if bias is None else bias.contiguous()
-    wt = weight if weight is not None else bias
-    with _on(x) as stream:
-        _lib.check(_lib.lib().vad_layer_norm_forward(
-            rows.data_ptr(), rows.size(0), rows.size(1), rows.stride(0), _ptr(weight), _ptr(bias), _DTYPES[x.dtype],
-            0 if wt is None else _DTYPES[wt.dtype], eps, y.data_ptr(), _ptr(stats), stream))
+    n, cols = rows.shape
+    y = x.new_empty(x.shape)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+    wt = 0
+    if weight is not None:
+        weight = weight.contiguous()
+        wt = _DTYPES[weight.dtype]
+    if bias is not None:
+        bias = bias.contiguous()
+        wt = _DTYPES[bias.dtype]
+    _call(_lib.lib().vad_layer_norm_forward, x.get_device(), rows.data_ptr(), n, cols, rows.stride(0), _ptr(weight), _ptr(bias),
+          _DTYPES[x.dtype], wt, eps, y.data_ptr(), _ptr(stats))
     return y, stats
 
 
@@ -127,74 +156,92 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         rows, dyr = _as_rows(x), _as_rows(dy)
         n, cols = rows.shape
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dx = x.new_empty(x.shape) if need_x else None
         dw = torch.empty(cols, dtype=ctx.param, device=x.device) if need_w else None
         db = torch.empty(cols, dtype=ctx.param, device=x.device) if need_b else None
         L = _lib.lib()
-        ws = _scratch(L.vad_layer_norm_workspace_bytes(n, cols) if need_w or need_b else 0, x.device)
+        size = L.vad_layer_norm_workspace_bytes(n, cols) if need_w or need_b else 0
+        ws = _scratch(size, x)
         weight = weight if weight is None else weight.contiguous()
-        with _on(x) as stream:
-            _lib.check(L.vad_layer_norm_backward(
-                rows.data_ptr(), dyr.data_ptr(), n, cols, rows.stride(0), dyr.stride(0), _ptr(weight), _DTYPES[x.dtype],
-                0 if ctx.param is None else _DTYPES[ctx.param], stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                _ptr(ws), 0 if ws is None else ws.numel(), stream))
+        _call(L.vad_layer_norm_backward, x.get_device(), rows.data_ptr(), dyr.data_ptr(), n, cols, rows.stride(0), dyr.stride(0),
+              _ptr(weight), _DTYPES[x.dtype], 0 if ctx.param is None else _DTYPES[ctx.param], stats.data_ptr(), _ptr(dx), _ptr(dw),
+              _ptr(db), _ptr(ws), size)
         return dx, dw, db, None
 
 
 # ---- heads over sequences ----
 
 class _Layout:
-    """Shape of a call over whole sequences: checked once, kept for the backward pass."""
+    """What the shapes of a call over whole sequences say; one object per combination, see ``_layout``."""
 
-    def __init__(self, q, k, v, starts, max_len, shared):
-        for name, t in (('q', q), ('k', k), ('v', v)):
-            _check_tensor(name, t, None if name == 'q' else q.dtype, q.device)
-            if t.dim() != (4 if starts is None else 3):
-                raise ValueError('%s must be (batch, length, heads, dim), or (rows, heads, dim) with starts; got %s'
-                                 % (name, tuple(t.shape)))
-        if k.shape != v.shape or q.shape[:-2] != k.shape[:-2] or q.size(-1) != k.size(-1):
-            raise ValueError('shapes of q %s, k %s and v %s do not go together' % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-        self.heads, self.dim = q.shape[-2:]
-        self.kv_heads = k.size(-2)
+    def __init__(self, qs, ks, vs, n_starts, max_len, shared):
+        for name, s in (('q', qs), ('k', ks), ('v', vs)):
+            if len(s) != (4 if n_starts is None else 3):
+                raise ValueError('%s must be (batch, length, heads, dim), or (rows, heads, dim) with starts; got %s' % (name, tuple(s)))
+        if ks != vs or qs[:-2] != ks[:-2] or qs[-1] != ks[-1]:
+            raise ValueError('shapes of q %s, k %s and v %s do not go together' % (tuple(qs), tuple(ks), tuple(vs)))
+        self.heads, self.dim = qs[-2:]
+        self.kv_heads = ks[-2]
         if self.heads < 1 or self.kv_heads < 1 or not 1 <= self.dim <= MAX_HEAD_DIM:
-            raise ValueError('heads must be positive and dim 1 .. %d, got %s' % (MAX_HEAD_DIM, tuple(q.shape)))
+            raise ValueError('heads must be positive and dim 1 .. %d, got %s' % (MAX_HEAD_DIM, tuple(qs)))
         if self.heads % self.kv_heads or (not shared and self.heads != self.kv_heads):
             raise ValueError('%d query heads cannot use %d key heads' % (self.heads, self.kv_heads))
-        self.rows_shape = q.shape[:-2]
-        if starts is None:
-            self.n_seq, self.max_len = q.shape[:2]
-            self.n_rows = self.n_seq * self.max_len
-        else:
-            _check_tensor('starts', starts, torch.int64, q.device)
-            if starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
-                raise ValueError('starts must be a contiguous 1-D tensor of at least one entry')
-            self.n_seq, self.n_rows = starts.numel() - 1, q.size(0)
+        self.packed = n_starts is not None
+        if self.packed:
+            self.n_seq, self.n_rows = n_starts - 1, qs[0]
             if max_len is not None and max_len < 0:
                 raise ValueError('max_len must not be negative, got %r' % (max_len,))
-            self.max_len = self.n_rows if max_len is None else min(int(max_len), self.n_rows)
-        self.n_tokens = self.n_rows if starts is not None else 0
-        self.dtype = _DTYPES[q.dtype]
-        self.packed = starts is not None
+            self.max_len = self.n_rows if max_len is None else min(max_len, self.n_rows)
+            self.sequences = self.n_seq, self.n_rows, self.max_len
+        else:
+            self.n_seq, self.max_len = qs[:2]
+            self.n_rows = self.n_seq * self.max_len
+            self.sequences = self.n_seq, 0, self.max_len
+        self.state_shape = (self.n_seq, self.heads, self.dim, self.dim)
+        self.table = functools.lru_cache(maxsize=64)(self._table)
+
+    def _table(self, s):
+        return _strides(*((0,) + s[:2] if self.packed else s[:3]))
 
     def operand(self, t):
         """t with a dense head dimension, and its {sequence, row, head} strides."""
-        if t.size(-1) > 1 and t.stride(-1) != 1:
+        t = _dense(t)
+        if t.stride(-3) >= MAX_ROW_STRIDE:
             t = t.contiguous()
-        return t, _strides(*((0,) + t.stride()[:2] if self.packed else t.stride()[:3]))
+        return t, self.table(t.stride())
 
-    def output(self, like, heads):
+    def output(self, like):
         # no sequence: nothing is launched that could set the rows to zero
-        make = torch.zeros if self.n_seq == 0 else torch.empty
-        return make(self.rows_shape + (heads, self.dim), dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape) if self.n_seq else like.new_zeros(like.shape)
 
-    def sequences(self, starts):
-        return _ptr(starts), self.n_seq, self.n_tokens, self.max_len
+    @functools.cached_property
+    def decay_workspace(self):
+        size = _lib.lib().vad_linear_attention_workspace_bytes
+        return [size(self.n_seq, self.max_len, self.heads, self.dim, back) for back in (0, 1)]
+
+    @functools.lru_cache(maxsize=64)
+    def window_workspace(self, window, sinks):
+        return _lib.lib().vad_window_attention_workspace_bytes(self.n_seq, self.n_rows, self.max_len, self.heads, self.kv_heads,
+                                                               self.dim, window, sinks)
+
+
+_layout_of = functools.lru_cache(maxsize=256)(_Layout)
+
+
+def _layout(q, k, v, starts, max_len, shared):
+    _check_like(q, k, v)
+    if starts is None:
+        return _layout_of(q.shape, k.shape, v.shape, None, None, shared)
+    _check_tensor('starts', starts, torch.int64, q.device)
+    if starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
+        raise ValueError('starts must be a contiguous 1-D tensor of at least one entry')
+    return _layout_of(q.shape, k.shape, v.shape, starts.numel(), None if max_len is None else operator.index(max_len), shared)
 
 
 def _scale(scale, dim):
@@ -207,11 +254,12 @@ def _scale(scale, dim):
 
 # ---- linear attention with a decay per head ----
 
-def _check_decay(log_decay, heads, device):
-    _check_tensor('log_decay', log_decay, torch.float32, device)
-    if tuple(log_decay.shape) != (heads,) or not log_decay.is_contiguous():
+def _check_decay(log_decay, heads, like):
+    if type(log_decay) is not torch.Tensor or log_decay.dtype is not torch.float32 or log_decay.get_device() != like.get_device():
+        _check_tensor('log_decay', log_decay, torch.float32, like.device)
+    if log_decay.dim() != 1 or log_decay.size(0) != heads or not log_decay.is_contiguous():
         raise ValueError('log_decay must be a contiguous tensor of shape (%d,), got %s' % (heads, tuple(log_decay.shape)))
-    if _wants_grad(log_decay):
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError('log_decay is a constant of the operator and gets no gradient: pass log_decay.detach()')
 
 
@@ -224,30 +272,28 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, starts=None, ma
                    every sequence's last row, the one ``linear_attention_step`` goes on from.
     ``max_len``    longest sequence of a packed call, a hint that sizes the launch.
     Gradients reach q, k, v and state."""
-    lay = _Layout(q, k, v, starts, max_len, False)
-    _check_decay(log_decay, lay.heads, q.device)
+    lay = _layout(q, k, v, starts, max_len, False)
+    _check_decay(log_decay, lay.heads, q)
     scale = _scale(scale, lay.dim)
     if state is not None:
         _check_tensor('state', state, torch.float32, q.device)
-        if tuple(state.shape) != (lay.n_seq, lay.heads, lay.dim, lay.dim):
-            raise ValueError('state must have shape %s, got %s' % ((lay.n_seq, lay.heads, lay.dim, lay.dim), tuple(state.shape)))
-    if _wants_grad(q, k, v, state):
+        if state.shape != lay.state_shape:
+            raise ValueError('state must have shape %s, got %s' % (lay.state_shape, tuple(state.shape)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         return _LinearAttention.apply(q, k, v, state, log_decay, starts, scale, lay)
     return _decay_forward(q, k, v, state, log_decay, starts, scale, lay)
 
 
 def _decay_forward(q, k, v, state, log_decay, starts, scale, lay):
-    o = lay.output(q, lay.heads)
-    out = torch.empty((lay.n_seq, lay.heads, lay.dim, lay.dim), dtype=torch.float32, device=q.device)
+    o = lay.output(q)
+    out = torch.empty(lay.state_shape, dtype=torch.float32, device=q.device)
     (q, qs), (k, ks), (v, vs) = lay.operand(q), lay.operand(k), lay.operand(v)
     state = state if state is None else state.contiguous()
-    L = _lib.lib()
-    ws = _scratch(L.vad_linear_attention_workspace_bytes(lay.n_seq, lay.max_len, lay.heads, lay.dim, 0), q.device)
-    with _on(q) as stream:
-        _lib.check(L.vad_linear_attention_forward(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, *lay.sequences(starts), lay.heads, lay.dim, lay.dtype,
-            log_decay.data_ptr(), scale, _ptr(state), o.data_ptr(), out.data_ptr(), _ptr(ws),
-            0 if ws is None else ws.numel(), stream))
+    size = lay.decay_workspace[0]
+    ws = _scratch(size, q)
+    _call(_lib.lib().vad_linear_attention_forward, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(starts),
+          *lay.sequences, lay.heads, lay.dim, _DTYPES[q.dtype], log_decay.data_ptr(), scale, _ptr(state), o.data_ptr(), out.data_ptr(),
+          _ptr(ws), size)
     return o, out
 
 
@@ -260,7 +306,7 @@ class _LinearAttention(torch.autograd.Function):
         return _decay_forward(q, k, v, state, log_decay, starts, scale, lay)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do, dstate):
         q, k, v, state, log_decay, starts = ctx.saved_tensors
         lay = ctx.lay
@@ -268,63 +314,69 @@ class _LinearAttention(torch.autograd.Function):
             return (None,) * 8
         do = torch.zeros_like(q) if do is None else do
         dstate = dstate if dstate is None else dstate.contiguous()
-        dq, dk, dv = (lay.output(q, lay.heads) for _ in range(3))
+        dq, dk, dv = lay.output(q), lay.output(k), lay.output(v)
         need_state = state is not None and ctx.needs_input_grad[3]
-        dstate_in = torch.empty(state.shape, dtype=torch.float32, device=q.device) if need_state else None
+        dstate_in = torch.empty(lay.state_shape, dtype=torch.float32, device=q.device) if need_state else None
         state = state if state is None else state.contiguous()
-        (q, qs), (k, ks), (v, vs), (do, gs) = (lay.operand(t) for t in (q, k, v, do))
-        L = _lib.lib()
-        ws = _scratch(L.vad_linear_attention_workspace_bytes(lay.n_seq, lay.max_len, lay.heads, lay.dim, 1), q.device)
-        with _on(q) as stream:
-            _lib.check(L.vad_linear_attention_backward(
-                q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, do.data_ptr(), gs, *lay.sequences(starts), lay.heads, lay.dim,
-                lay.dtype, log_decay.data_ptr(), ctx.scale, _ptr(state), _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                _ptr(dstate_in), _ptr(ws), 0 if ws is None else ws.numel(), stream))
+        (q, qs), (k, ks), (v, vs), (do, gs) = lay.operand(q), lay.operand(k), lay.operand(v), lay.operand(do)
+        size = lay.decay_workspace[1]
+        ws = _scratch(size, q)
+        _call(_lib.lib().vad_linear_attention_backward, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, do.data_ptr(),
+              gs, _ptr(starts), *lay.sequences, lay.heads, lay.dim, _DTYPES[q.dtype], log_decay.data_ptr(), ctx.scale, _ptr(state),
+              _ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dstate_in), _ptr(ws), size)
         return dq, dk, dv, dstate_in, None, None, None, None
 
 
-def _step_operands(q, k, v, shared):
-    for name, t in (('q', q), ('k', k), ('v', v)):
-        _check_tensor(name, t, None if name == 'q' else q.dtype, q.device)
-        if t.dim() != 3:
-            raise ValueError('%s must be (batch, heads, dim), got %s' % (name, tuple(t.shape)))
-    if k.shape != v.shape or q.size(0) != k.size(0) or q.size(2) != k.size(2):
-        raise ValueError('shapes of q %s, k %s and v %s do not go together' % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    heads, dim, kv_heads = q.size(1), q.size(2), k.size(1)
+@functools.lru_cache(maxsize=256)
+def _step_shapes(qs, ks, vs, shared):
+    for name, s in (('q', qs), ('k', ks), ('v', vs)):
+        if len(s) != 3:
+            raise ValueError('%s must be (batch, heads, dim), got %s' % (name, tuple(s)))
+    if ks != vs or qs[0] != ks[0] or qs[2] != ks[2]:
+        raise ValueError('shapes of q %s, k %s and v %s do not go together' % (tuple(qs), tuple(ks), tuple(vs)))
+    batch, heads, dim = qs
+    kv_heads = ks[1]
     if heads < 1 or kv_heads < 1 or not 1 <= dim <= MAX_HEAD_DIM:
-        raise ValueError('heads must be positive and dim 1 .. %d, got %s' % (MAX_HEAD_DIM, tuple(q.shape)))
+        raise ValueError('heads must be positive and dim 1 .. %d, got %s' % (MAX_HEAD_DIM, tuple(qs)))
     if heads % kv_heads or (not shared and heads != kv_heads):
         raise ValueError('%d query heads cannot use %d key heads' % (heads, kv_heads))
-    out = []
-    for t in (q, k, v):
-        t = t if dim == 1 or t.stride(2) == 1 else t.contiguous()
-        out.append((t, _strides(t.stride(0), t.stride(1))))
-    return out
+    return batch, heads, kv_heads, dim, (batch, heads, dim, dim)
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_table(s):
+    return _strides(*s[:-1])
+
+
+def _step_operands(q, k, v):
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    return q, _step_table(q.stride()), k, _step_table(k.stride()), v, _step_table(v.stride())
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One row of ``linear_attention`` per sequence: q, k, v (batch, heads, dim); ``state`` (batch, heads, dim, dim) float32,
     contiguous, is updated in place.  Returns o (batch, heads, dim).  Inference only."""
-    (q, qs), (k, ks), (v, vs) = _step_operands(q, k, v, False)
-    batch, heads, dim = q.shape
-    _check_decay(log_decay, heads, q.device)
+    _check_like(q, k, v)
+    batch, heads, _, dim, state_shape = _step_shapes(q.shape, k.shape, v.shape, False)
+    _check_decay(log_decay, heads, q)
     scale = _scale(scale, dim)
-    _check_tensor('state', state, torch.float32, q.device)
-    if tuple(state.shape) != (batch, heads, dim, dim) or not state.is_contiguous():
-        raise ValueError('state must be a contiguous tensor of shape %s, got %s' % ((batch, heads, dim, dim), tuple(state.shape)))
-    if _wants_grad(q, k, v, state):
+    if type(state) is not torch.Tensor or state.dtype is not torch.float32 or state.get_device() != q.get_device():
+        _check_tensor('state', state, torch.float32, q.device)
+    if state.shape != state_shape or not state.is_contiguous():
+        raise ValueError('state must be a contiguous tensor of shape %s, got %s' % (state_shape, tuple(state.shape)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError('linear_attention_step has no gradient: call it under torch.no_grad(), or use linear_attention')
-    o = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-    with _on(q) as stream:
-        _lib.check(_lib.lib().vad_linear_attention_step(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, heads, dim, _DTYPES[q.dtype], log_decay.data_ptr(), scale,
-            state.data_ptr(), o.data_ptr(), stream))
+    o = q.new_empty(q.shape)
+    q, qs, k, ks, v, vs = _step_operands(q, k, v)
+    _call(_lib.lib().vad_linear_attention_step, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, heads, dim,
+          _DTYPES[q.dtype], log_decay.data_ptr(), scale, state.data_ptr(), o.data_ptr())
     return o
 
 
 # ---- attention with a sliding window and sinks ----
 
 def _check_window(window, sinks, scale, dim):
+    window, sinks = operator.index(window), operator.index(sinks)
     if not 1 <= window <= 1 << 30:
         raise ValueError('window must be 1 .. 2^30, got %r' % (window,))
     if not 0 <= sinks <= MAX_SINKS:
@@ -332,7 +384,7 @@ def _check_window(window, sinks, scale, dim):
     scale = _scale(scale, dim)
     if scale <= 0.0:
         raise ValueError('scale must be positive, got %r' % (scale,))
-    return int(window), int(sinks), scale
+    return window, sinks, scale
 
 
 def window_attention(q, k, v, window, sinks=0, scale=None, starts=None, max_len=None):
@@ -342,21 +394,19 @@ def window_attention(q, k, v, window, sinks=0, scale=None, starts=None, max_len=
     ``k``, ``v``  may have fewer heads than q: query head h reads key head ``h // (heads // kv_heads)``.
     ``scale``   positive, dim ** -0.5 unless given.  ``max_len`` as in ``linear_attention``.
     Returns a tensor of q's shape; gradients reach q, k and v."""
-    lay = _Layout(q, k, v, starts, max_len, True)
+    lay = _layout(q, k, v, starts, max_len, True)
     window, sinks, scale = _check_window(window, sinks, scale, lay.dim)
-    if _wants_grad(q, k, v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowAttention.apply(q, k, v, starts, window, sinks, scale, lay)
     return _window_forward(q, k, v, starts, window, sinks, scale, lay, False)[0]
 
 
 def _window_forward(q, k, v, starts, window, sinks, scale, lay, keep):
-    o = lay.output(q, lay.heads)
+    o = lay.output(q)
     stats = torch.empty((lay.n_rows, lay.heads, 2), dtype=torch.float32, device=q.device) if keep else None
     (q, qs), (k, ks), (v, vs) = lay.operand(q), lay.operand(k), lay.operand(v)
-    with _on(q) as stream:
-        _lib.check(_lib.lib().vad_window_attention_forward(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, *lay.sequences(starts), lay.heads, lay.kv_heads, lay.dim, lay.dtype,
-            window, sinks, scale, o.data_ptr(), _ptr(stats), stream))
+    _call(_lib.lib().vad_window_attention_forward, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(starts),
+          *lay.sequences, lay.heads, lay.kv_heads, lay.dim, _DTYPES[q.dtype], window, sinks, scale, o.data_ptr(), _ptr(stats))
     return o, stats
 
 
@@ -370,31 +420,40 @@ class _WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, do):
         q, k, v, o, stats, starts = ctx.saved_tensors
         lay = ctx.lay
         window, sinks, scale = ctx.call
-        dq, dk, dv = lay.output(q, lay.heads), lay.output(q, lay.kv_heads), lay.output(q, lay.kv_heads)
-        (q, qs), (k, ks), (v, vs), (do, gs) = (lay.operand(t) for t in (q, k, v, do))
-        L = _lib.lib()
-        ws = _scratch(L.vad_window_attention_workspace_bytes(lay.n_seq, lay.n_rows, lay.max_len, lay.heads, lay.kv_heads, lay.dim,
-                                                             window, sinks), q.device)
-        with _on(q) as stream:
-            _lib.check(L.vad_window_attention_backward(
-                q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, o.data_ptr(), do.data_ptr(), gs, stats.data_ptr(),
-                *lay.sequences(starts), lay.heads, lay.kv_heads, lay.dim, lay.dtype, window, sinks, scale, dq.data_ptr(),
-                dk.data_ptr(), dv.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream))
+        dq, dk, dv = lay.output(q), lay.output(k), lay.output(v)
+        (q, qs), (k, ks), (v, vs), (do, gs) = lay.operand(q), lay.operand(k), lay.operand(v), lay.operand(do)
+        size = lay.window_workspace(window, sinks)
+        ws = _scratch(size, q)
+        _call(_lib.lib().vad_window_attention_backward, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, o.data_ptr(),
+              do.data_ptr(), gs, stats.data_ptr(), _ptr(starts), *lay.sequences, lay.heads, lay.kv_heads, lay.dim, _DTYPES[q.dtype], window,
+              sinks, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), size)
         return dq, dk, dv, None, None, None, None, None
 
 
-def _check_cache(name, c, batch, window, sinks, kv_heads, dim, dtype, device):
-    _check_tensor(name, c, dtype, device)
-    if tuple(c.shape) != (batch, sinks + window, kv_heads, dim):
-        raise ValueError('%s must have shape %s, got %s' % (name, (batch, sinks + window, kv_heads, dim), tuple(c.shape)))
-    if dim > 1 and c.stride(3) != 1 or any(n > 1 and s == 0 for n, s in zip(c.shape, c.stride())):
+@functools.lru_cache(maxsize=1024)
+def _cache_table(name, shape, stride, batch, slots, kv_heads, dim):
+    want = (batch, slots, kv_heads, dim)
+    if shape != want:
+        raise ValueError('%s must have shape %s, got %s' % (name, want, tuple(shape)))
+    if dim > 1 and stride[3] != 1 or any(n > 1 and s == 0 for n, s in zip(shape, stride)):
         raise ValueError('%s must have a dense last dimension and no broadcast one' % name)
-    return _strides(*c.stride()[:3])
+    return _strides(*stride[:3])
+
+
+def _check_cache(name, c, like, batch, slots, kv_heads, dim):
+    if type(c) is not torch.Tensor or c.dtype is not like.dtype or c.get_device() != like.get_device():
+        _check_tensor(name, c, like.dtype, like.device)
+    return _cache_table(name, c.shape, c.stride(), batch, slots, kv_heads, dim)
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_workspace(batch, heads, kv_heads, dim, window, sinks):
+    return _lib.lib().vad_window_step_workspace_bytes(batch, heads, kv_heads, dim, window, sinks)
 
 
 def window_attention_step(q, k, v, cache_k, cache_v, pos, window, sinks=0, scale=None):
@@ -406,24 +465,23 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, window, sinks=0, scale
     ``pos``    (batch,) int64 CUDA tensor: rows the sequence has had before this one; not changed.  Where it is negative
                the output is zero and the cache stays as it is.
     Returns o (batch, heads, dim).  Inference only."""
-    (q, qs), (k, ks), (v, vs) = _step_operands(q, k, v, True)
-    batch, heads, dim = q.shape
-    kv_heads = k.size(1)
+    _check_like(q, k, v)
+    batch, heads, kv_heads, dim, _ = _step_shapes(q.shape, k.shape, v.shape, True)
     window, sinks, scale = _check_window(window, sinks, scale, dim)
-    cks = _check_cache('cache_k', cache_k, batch, window, sinks, kv_heads, dim, q.dtype, q.device)
-    cvs = _check_cache('cache_v', cache_v, batch, window, sinks, kv_heads, dim, q.dtype, q.device)
+    cks = _check_cache('cache_k', cache_k, q, batch, sinks + window, kv_heads, dim)
+    cvs = _check_cache('cache_v', cache_v, q, batch, sinks + window, kv_heads, dim)
     _check_tensor('pos', pos, torch.int64, q.device)
-    if tuple(pos.shape) != (batch,) or not pos.is_contiguous():
+    if pos.dim() != 1 or pos.size(0) != batch or not pos.is_contiguous():
         raise ValueError('pos must be a contiguous tensor of shape (%d,), got %s' % (batch, tuple(pos.shape)))
-    if _wants_grad(q, k, v, cache_k, cache_v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or cache_k.requires_grad or cache_v.requires_grad):
         raise ValueError('window_attention_step has no gradient: call it under torch.no_grad(), or use window_attention')
-    o = torch.empty((batch, heads, dim), dtype=q.dtype, device=q.device)
-    L = _lib.lib()
-    ws = _scratch(L.vad_window_step_workspace_bytes(batch, heads, kv_heads, dim, window, sinks), q.device)
-    with _on(q) as stream:
-        _lib.check(L.vad_window_attention_step(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, cache_k.data_ptr(), cks, cache_v.data_ptr(), cvs, pos.data_ptr(), batch,
-            heads, kv_heads, dim, _DTYPES[q.dtype], window, sinks, scale, o.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel(), stream))
+    o = q.new_empty(q.shape)
+    q, qs, k, ks, v, vs = _step_operands(q, k, v)
+    size = _step_workspace(batch, heads, kv_heads, dim, window, sinks)
+    ws = _scratch(size, q)
+    _call(_lib.lib().vad_window_attention_step, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, cache_k.data_ptr(),
+          cks, cache_v.data_ptr(), cvs, pos.data_ptr(), batch, heads, kv_heads, dim, _DTYPES[q.dtype], window, sinks, scale, o.data_ptr(),
+          _ptr(ws), size)
     return o
 
 
@@ -431,14 +489,12 @@ def window_cache_fill(k, v, cache_k, cache_v, window, sinks=0, starts=None):
     """Keys and values of whole sequences into rolling caches, as the steps after them expect it: (batch, length, kv_heads,
     dim), or packed with ``starts``.  Slots that no row belongs to stay as they are.  Returns ``pos`` (batch,) int64: the
     lengths."""
-    lay = _Layout(k, k, v, starts, None, True)
+    lay = _layout(k, k, v, starts, None, True)
     window, sinks, _ = _check_window(window, sinks, None, lay.dim)
-    cks = _check_cache('cache_k', cache_k, lay.n_seq, window, sinks, lay.heads, lay.dim, k.dtype, k.device)
-    cvs = _check_cache('cache_v', cache_v, lay.n_seq, window, sinks, lay.heads, lay.dim, k.dtype, k.device)
+    cks = _check_cache('cache_k', cache_k, k, lay.n_seq, sinks + window, lay.heads, lay.dim)
+    cvs = _check_cache('cache_v', cache_v, k, lay.n_seq, sinks + window, lay.heads, lay.dim)
     pos = torch.empty(lay.n_seq, dtype=torch.int64, device=k.device)
     (k, ks), (v, vs) = lay.operand(k), lay.operand(v)
-    with _on(k) as stream:
-        _lib.check(_lib.lib().vad_window_cache_fill(
-            k.data_ptr(), ks, v.data_ptr(), vs, *lay.sequences(starts), lay.heads, lay.dim, lay.dtype, window, sinks,
-            cache_k.data_ptr(), cks, cache_v.data_ptr(), cvs, pos.data_ptr(), stream))
+    _call(_lib.lib().vad_window_cache_fill, k.get_device(), k.data_ptr(), ks, v.data_ptr(), vs, _ptr(starts), *lay.sequences, lay.heads,
+          lay.dim, _DTYPES[k.dtype], window, sinks, cache_k.data_ptr(), cks, cache_v.data_ptr(), cvs, pos.data_ptr())
     return pos
