@@ -415,7 +415,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *                are float32.
  *   rows         q, k, v and the gradients of outputs are read through strides in ELEMENTS given on the host: {sequence,
  *                row, head} (steps: {batch, head}, caches: {batch, slot, head}); the head dimension is dense.  Any alignment
- *                works; rows at 4-byte boundaries with a head dimension of whole 8- or 16-byte pieces take wide loads.
+ *                works; rows of whole 4-byte words at 4-byte boundaries take wide loads.
  *                Row strides and dense rows (heads * dim) are below VAD_MAX_ROW_STRIDE.  Outputs are dense (rows, heads, dim).
  *   sequences    starts_dev == NULL: n_seq sequences of max_len rows each.  Otherwise the rows of all sequences are packed
  *                behind one another in n_tokens rows and starts_dev holds n_seq + 1 ascending int64 on the device, sequence s
@@ -430,7 +430,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
 #define VAD_DTYPE_BF16 1
 #define VAD_MAX_HEAD_DIM 128
 #define VAD_MAX_SINKS 64
-#define VAD_MAX_ROW_STRIDE (1 << 24)
+#define VAD_MAX_ROW_STRIDE (1 << 22)
 
 /*
  * Layer norm: y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (var: mean squared deviation).

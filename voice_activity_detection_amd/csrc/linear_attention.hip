@@ -44,8 +44,7 @@ struct WalkArgs {
     const float* log_decay;
     float* spans;                      // [walk][seq][head][span][dim][dim]
     int n_seq, heads, dim, n_spans;
-    int mode;                          // how rows are read
-    bool wide_out;
+    bool whole;                        // all rows are whole words at 4-byte boundaries
 };
 
 __device__ __forceinline__ float log2_decay(float ld) {
@@ -67,7 +66,6 @@ struct WalkShape {
     static constexpr int kThreads = kWaves * 64;
     static constexpr int kLd = DP + Elem<T>::kPer16B;
     static constexpr int kLdP = kPiece + Elem<T>::kPer16B;
-    static constexpr int kPieces = kPiece * DP / Elem<T>::kPer16B / kThreads;       // 16-byte pieces a thread stages
     static constexpr size_t kLds = (size_t)(3 * kPiece * kLd + kPiece * kLdP) * sizeof(T) + 16;
 };
 
@@ -97,12 +95,10 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&f)[3]) {
 template <typename T, int DP>
 constexpr int walk_waves() { return sizeof(T) == 2 && DP < 128 ? 3 : 2; }
 
-// WIDE: every row is read and written by whole 16-byte pieces (a.mode, a.wide_out), which saves the other forms' registers.
-template <typename T, int DP, bool STATE, bool WIDE>
+// BUF: rows are whole words at 4-byte boundaries (a.whole).
+template <typename T, int DP, bool STATE, bool BUF>
 __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kernel(WalkArgs<T> a) {
     using C = WalkShape<T, DP>;
-    const int mode = WIDE ? kWide : a.mode;
-    const bool wide_out = WIDE || a.wide_out;
     extern __shared__ char lds_raw[];
     T* sk = reinterpret_cast<T*>(lds_raw);
     T* sv = sk + kPiece * C::kLd;
@@ -156,25 +152,14 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
     const T* vp = head_ptr(w.v, a.seq, s, first, h);
     const T* qp = STATE ? nullptr : head_ptr(w.q, a.seq, s, first, h);
     T* op = w.o + ((a.seq.starts ? first : (int64_t)s * a.seq.max_len) * a.heads + h) * dim;
-    constexpr int PPR = DP / Elem<T>::kPer16B;
     const int sign = w.reverse ? -1 : 1;
-    u32x4 rk[C::kPieces], rv[C::kPieces], rq[C::kPieces];
-    auto fetch = [&](int64_t tc) {
+    Staged<T, DP, C::kThreads, BUF> rk, rv, rq;
+    const auto fetch = [&](int64_t tc) {
         const int64_t at = w.reverse ? len - 1 - tc : tc;
-        const T* kc = kp + at * w.k.st;
-        const T* vc = vp + at * w.v.st;
-        const T* qc = STATE ? nullptr : qp + at * w.q.st;
-        const int left = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);
-#pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) {
-            const int p = threadIdx.x + n * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B, sr = sign * row;
-            rk[n] = rv[n] = rq[n] = u32x4{0, 0, 0, 0};
-            if (row < left) {
-                rk[n] = load_piece(kc + sr * (int)w.k.st, pc, dim, mode);
-                rv[n] = load_piece(vc + sr * (int)w.v.st, pc, dim, mode);
-                if (!STATE) rq[n] = load_piece(qc + sr * (int)w.q.st, pc, dim, mode);
-            }
-        }
+        const int rows = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);
+        rk.fetch(kp, w.k.st, at, rows, dim, w.reverse);
+        rv.fetch(vp, w.v.st, at, rows, dim, w.reverse);
+        if (!STATE) rq.fetch(qp, w.q.st, at, rows, dim, w.reverse);
     };
     // Powers of the decay.  A row and key block m apart need a^(16 m + c - 4 g - i) = a^(16 m - 15) a^c a^(15 - 4 g - i), a
     // diagonal block its own; the state's update a^(64 - row) = a^(16 m') a a^(15 - 4 g - i).
@@ -193,18 +178,12 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
     int turn = 0;
     for (int64_t tc = t0; tc < t1; tc += kPiece, turn ^= 1) {
         const int n = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < C::kPieces; ++i) {
-            const int p = threadIdx.x + i * C::kThreads, row = p / PPR, pc = p % PPR * Elem<T>::kPer16B;
-            *reinterpret_cast<u32x4*>(sk + row * C::kLd + pc) = rk[i];
-            *reinterpret_cast<u32x4*>(sv + row * C::kLd + pc) = rv[i];
-            if (!STATE) {
-                *reinterpret_cast<u32x4*>(sq_ + row * C::kLd + pc) = rq[i];
-                bad |= piece_not_finite<T>(rv[i]);
-            }
+        rk.put(sk, dim);
+        rv.put(sv, dim);
+        if (!STATE) {
+            rq.put(sq_, dim);
+            if (rv.not_finite()) flags[turn] = 1;
         }
-        if (bad) flags[turn] = 1;
         __syncthreads();
         const bool careful = !STATE && flags[turn];
         if (threadIdx.x == 0) flags[turn ^ 1] = 0;
@@ -326,7 +305,7 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
 #pragma unroll
             for (int rb = 0; rb < 4; ++rb) {
                 const int row = 16 * rb + c;
-                if (row < n) store_quad(oc + sign * row * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], wide_out);
+                if (row < n) store_quad(oc + sign * row * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], BUF);
             }
         }
         __syncthreads();
@@ -452,7 +431,7 @@ template <typename T, int DP, bool STATE>
 void launch_walk(const WalkArgs<T>& a, int walks, hipStream_t st) {
     const dim3 grid((unsigned)(a.n_seq * a.heads * a.n_spans), (unsigned)walks), block((WalkShape<T, DP>::kThreads));
     constexpr size_t lds = WalkShape<T, DP>::kLds;
-    if (a.mode == kWide && a.wide_out)
+    if (a.whole)
         hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE, true>), grid, block, lds, st, a);
     else
         hipLaunchKernelGGL((decay_walk_kernel<T, DP, STATE, false>), grid, block, lds, st, a);
@@ -498,8 +477,7 @@ int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* 
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
-    a.mode = std::min({load_mode(a.walk[0].q, dim), load_mode(a.walk[0].k, dim), load_mode(a.walk[0].v, dim)});
-    a.wide_out = wide_rows(static_cast<const T*>(o), dim);
+    a.whole = whole_words(a.walk[0].q, dim) && whole_words(a.walk[0].k, dim) && whole_words(a.walk[0].v, dim) && whole_words(a.walk[0].o, dim);
     return run_walks(a, 1, st);
 }
 
@@ -519,8 +497,8 @@ int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t*
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
-    a.mode = std::min({load_mode(Q, dim), load_mode(K, dim), load_mode(V, dim), load_mode(G, dim)});
-    a.wide_out = wide_rows(static_cast<const T*>(dq), dim) && wide_rows(static_cast<const T*>(dk), dim) && wide_rows(static_cast<const T*>(dv), dim);
+    a.whole = whole_words(Q, dim) && whole_words(K, dim) && whole_words(V, dim) && whole_words(G, dim);
+    for (const Walk<T>& w : a.walk) a.whole = a.whole && whole_words(w.o, dim);
     return run_walks(a, 3, st);
 }
 

@@ -166,21 +166,14 @@ __device__ __forceinline__ T* head_ptr(const Heads<T>& x, const Sequences& q, in
     return x.p + (q.starts ? first * x.st : (int64_t)s * x.sb) + (int64_t)h * x.sh;
 }
 
-// 16 bytes of a row from column c; columns from `cols` on read as zero.  The mode is uniform over the launch: kWide where
-// rows start 4-byte aligned and cols is a multiple of a 16-byte piece, kHalf where it is one of 8 bytes, else kScalar,
-// element by element.
-enum { kScalar = 0, kHalf = 1, kWide = 2 };
+// 16 bytes of a row from column c; columns from `cols` on read as zero.  `whole`: rows start at 4-byte boundaries, so that
+// pieces inside the row are one load (uniform over the launch).
 template <typename T>
-__device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, int mode) {
+__device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, bool whole) {
     constexpr int VE = Elem<T>::kPer16B;
-    u32x4 r = {0, 0, 0, 0};
-    if (mode != kScalar) {
-        if (c + VE <= cols) {
-            r = *reinterpret_cast<const u32x4_any*>(row + c);
-        } else if (mode == kHalf && c < cols) {
-            const u32x2 a = *reinterpret_cast<const u32x2_any*>(row + c);
-            r = u32x4{a[0], a[1], 0, 0};
-        }
+    u32x4 r;
+    if (whole && c + VE <= cols) {
+        r = *reinterpret_cast<const u32x4_any*>(row + c);
     } else {
         T v[VE];
 #pragma unroll
@@ -191,9 +184,9 @@ __device__ __forceinline__ u32x4 load_piece(const T* row, int c, int cols, int m
 }
 
 template <typename T>
-__device__ __forceinline__ void store_piece(T* row, int c, int cols, u32x4 v, int mode) {
+__device__ __forceinline__ void store_piece(T* row, int c, int cols, u32x4 v, bool whole) {
     constexpr int VE = Elem<T>::kPer16B;
-    if (mode != kScalar && c + VE <= cols) {
+    if (whole && c + VE <= cols) {
         *reinterpret_cast<u32x4_any*>(row + c) = v;
     } else {
         T e[VE];
@@ -204,11 +197,26 @@ __device__ __forceinline__ void store_piece(T* row, int c, int cols, u32x4 v, in
     }
 }
 
+// Rows at 4-byte boundaries and of whole 4-byte words: the form that buffer loads and wide stores take.
 template <typename T>
-int load_mode(const Heads<T>& x, int dim) {
-    constexpr int VE = 16 / sizeof(T);
+bool whole_words(const Heads<T>& x, int dim) {
     const uint64_t at = reinterpret_cast<uintptr_t>(x.p) | (uint64_t)(x.sb * sizeof(T)) | (uint64_t)(x.st * sizeof(T)) | (uint64_t)(x.sh * sizeof(T));
-    return at % 4 ? kScalar : (dim % VE == 0 ? kWide : (dim % (VE / 2) == 0 ? kHalf : kScalar));
+    return at % 4 == 0 && dim * sizeof(T) % 4 == 0;
+}
+template <typename T>
+bool whole_words(const T* p, int dim) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim * sizeof(T) % 4 == 0;
+}
+
+// A buffer over `rows` rows of `cols` columns, the last one cut at its end: loads past it give zero, without a branch.
+// At most 64 rows, 2^22 elements apart (VAD_MAX_ROW_STRIDE): offsets stay below 2^30 bytes.
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* p, int64_t st, int rows, int cols) {
+    const int bytes = rows > 0 ? ((rows - 1) * (int)st + cols) * (int)sizeof(T) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load_piece(__amdgpu_buffer_rsrc_t b, int offset) {
+    return __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0);
 }
 
 // Whether any of the values in a 16-byte piece is an infinity or a NaN.
@@ -220,24 +228,57 @@ __device__ __forceinline__ bool piece_not_finite(u32x4 v) {
         if (sizeof(T) == 4)
             bad |= (v[i] & 0x7F800000u) == 0x7F800000u;
         else
-            bad |= (v[i] & 0x7F800000u) == 0x7F800000u || (v[i] & 0x7F80u) == 0x7F80u;
+            bad |= ((v[i] & 0x7F800000u) == 0x7F800000u) | ((v[i] & 0x7F80u) == 0x7F80u);
     }
     return bad;
 }
 
-// A natural-order fragment straight from global memory: this lane's row, columns c .. c + 7.
-template <typename T>
-__device__ __forceinline__ Frag<T> load_row_frag(const T* row, bool live, int c, int cols, int mode) {
-    Frag<T> f;
-    u32x4 v[sizeof(Frag<T>) / 16];
+// 64 rows of one head on their way through a block's registers into an LDS tile.  BUF: by buffer loads (whole_words).
+template <typename T, int DP, int NT, bool BUF>
+struct Staged {
+    static constexpr int kPer = Elem<T>::kPer16B, kPPR = DP / kPer, kLd = DP + kPer, kPieces = 64 * kPPR / NT, kStep = NT / kPPR;
+    u32x4 r[kPieces];
+
+    // Tile row i is row at + i of the head (`back`: at - i) for i < rows, zero from there on; uniform arguments.
+    __device__ __forceinline__ void fetch(const T* p, int64_t st, int64_t at, int rows, int dim, bool back = false) {
+        rows = rows < 64 ? rows : 64;
+        const int row0 = threadIdx.x / kPPR, c = threadIdx.x % kPPR * kPer;
+        if constexpr (BUF) {
+            const auto b = row_buffer(p + (back ? at - (rows - 1) : at) * st, st, rows, dim);
+            const int col = c < dim ? c * (int)sizeof(T) : 1 << 30, pitch = (int)st * (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(Frag<T>) / 16); ++i) {
-        v[i] = u32x4{0, 0, 0, 0};
-        if (live) v[i] = load_piece(row, c + i * Elem<T>::kPer16B, cols, mode);
+            for (int n = 0; n < kPieces; ++n) {
+                const int row = row0 + n * kStep;
+                r[n] = load_piece(b, (back ? rows - 1 - row : row) * pitch + col);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < kPieces; ++n) {
+                const int row = row0 + n * kStep;
+                r[n] = u32x4{0, 0, 0, 0};
+                if (row < rows) r[n] = load_piece(p + (back ? at - row : at + row) * st, c, dim, false);
+            }
+        }
     }
-    __builtin_memcpy(&f, v, sizeof(f));
-    return f;
-}
+    __device__ __forceinline__ void put(T* tile, int dim) {
+        const int row0 = threadIdx.x / kPPR, c = threadIdx.x % kPPR * kPer;
+        if (BUF && dim < DP) {          // a piece that crosses the row's end has read on into what follows
+            const int words = (dim - c) * (int)sizeof(T) / 4;
+#pragma unroll
+            for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[n][i] = i < words ? r[n][i] : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) *reinterpret_cast<u32x4*>(tile + (row0 + n * kStep) * kLd + c) = r[n];
+    }
+    __device__ __forceinline__ bool not_finite() const {
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
+        return bad;
+    }
+};
 
 // ---- fragments from LDS ----
 
@@ -336,13 +377,13 @@ __device__ __forceinline__ void to_frag(f32x4 a, f32x4 b, f32x8& f) {
     }
 }
 
-// Four consecutive values of an output row; `wide`: rows start 4-byte aligned (wide_rows).
+// Four consecutive values of an output row; `whole`: rows start at 4-byte boundaries.
 template <typename T>
-__device__ __forceinline__ void store_quad(T* row, int c, int cols, f32x4 v, bool wide) {
-    if (wide && c + 4 <= cols) {
-        T q[4];
+__device__ __forceinline__ void store_quad(T* row, int c, int cols, f32x4 v, bool whole) {
+    T q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+    for (int i = 0; i < 4; ++i) q[i] = (T)v[i];
+    if (whole && c + 4 <= cols) {
         if (sizeof(T) == 4) {
             u32x4 r;
             __builtin_memcpy(&r, q, 16);
@@ -355,12 +396,8 @@ __device__ __forceinline__ void store_quad(T* row, int c, int cols, f32x4 v, boo
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (c + i < cols) row[c + i] = (T)v[i];
+            if (c + i < cols) row[c + i] = q[i];
     }
-}
-template <typename T>
-bool wide_rows(const T* p, int dim) {
-    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim * sizeof(T) % 4 == 0;
 }
 
 }  // namespace sq

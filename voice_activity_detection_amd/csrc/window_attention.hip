@@ -43,45 +43,33 @@ struct WindowArgs {
     Sequences seq;
     int n_seq, heads, kv_heads, dim, window, sinks, segments;
     float scale;
-    int mode;                       // how rows of q, k, v, dO are read
-    bool wide_out;
+    bool whole;                     // all rows are whole words at 4-byte boundaries
 };
 
-template <typename T, int DP, int NT = kThreads>
+template <typename T, int DP>
 struct TileShape {
     static constexpr int kLd = DP + Elem<T>::kPer16B;
-    static constexpr int kPieces = kTile * DP / Elem<T>::kPer16B / NT;
-    static constexpr int kPPR = DP / Elem<T>::kPer16B;
     static constexpr size_t kLds = (size_t)2 * kTile * kLd * sizeof(T) + (3 * kTile + 4) * sizeof(float);
 };
 
-// 64 rows from t0 on of one head, rows from len on as zero
-template <typename T, int DP, int NT>
-struct Staged {
-    using C = TileShape<T, DP, NT>;
-    u32x4 r[C::kPieces];
-    __device__ __forceinline__ void fetch(const T* p, int64_t st, int t0, int len, int dim, int mode) {
+// Own rows first .. first + 64 NB - 1 of a head (zero from row `len` on) as fragments: by way of the block's two tiles.
+template <typename T, int DP, int NB, int NT, bool BUF>
+__device__ __forceinline__ void load_own(Frag<T> (&f)[NB][DP / 32], const T* p, int64_t st, int first, int len, int dim, T* tiles) {
+    constexpr int kLd = TileShape<T, DP>::kLd;
+    const int wave = threadIdx.x >> 6;
+    Staged<T, DP, NT, BUF> r;
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) {
-            const int i = threadIdx.x + n * NT, row = i / C::kPPR;
-            r[n] = u32x4{0, 0, 0, 0};
-            if (t0 + row < len) r[n] = load_piece(p + (int64_t)(t0 + row) * st, i % C::kPPR * Elem<T>::kPer16B, dim, mode);
-        }
+    for (int n = 0; n < NB; ++n) {
+        r.fetch(p, st, first + 64 * n, len - first - 64 * n, dim);
+        r.put(tiles + n * kTile * kLd, dim);
     }
-    __device__ __forceinline__ void put(T* tile) const {
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) {
-            const int i = threadIdx.x + n * NT;
-            *reinterpret_cast<u32x4*>(tile + i / C::kPPR * C::kLd + i % C::kPPR * Elem<T>::kPer16B) = r[n];
-        }
-    }
-    __device__ __forceinline__ bool not_finite() const {
-        bool bad = false;
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int n = 0; n < C::kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
-        return bad;
-    }
-};
+        for (int d = 0; d < DP / 32; ++d) f[nb][d] = frag_natural(tiles, kLd, 16 * (NB * wave + nb), 32 * d);
+}
 
 // acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
 // own row.  `careful`: the tile holds infinities or NaN, which only rows that `sees` admits may feel (0 * inf is NaN).
@@ -154,7 +142,7 @@ struct KeyTiles {
 };
 
 // BACK == false: O and stats.  BACK == true: dQ and delta.
-template <typename T, int DP, int NB, bool BACK>
+template <typename T, int DP, int NB, bool BACK, bool BUF>
 __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> a) {
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
@@ -182,25 +170,29 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
         Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
         f32x4 acc[DP / 16][NB];
         float m[NB], sum[NB], delta[NB];
+        load_own<T, DP, NB, kThreads, BUF>(qf, qp, a.q.st, r0, len, dim, sk);
+        if (BACK) {
+            Frag<T> of[NB][DP / 32];
+            load_own<T, DP, NB, kThreads, BUF>(gf, gp, a.go.st, r0, len, dim, sk);
+            load_own<T, DP, NB, kThreads, BUF>(of, a.o + (row_base * a.heads + h) * dim, (int64_t)a.heads * dim, r0, len, dim, sk);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float x = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x = fmaf((float)gf[nb][d][j], (float)of[nb][d][j], x);
+                delta[nb] = groups_sum(x);
+            }
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int row = w0 + 16 * nb + c;
             const bool live = row < len;
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) qf[nb][d] = load_row_frag<T>(qp + (int64_t)row * a.q.st, live, 32 * d + 8 * g, dim, a.mode);
             m[nb] = -INFINITY;
             sum[nb] = 0.0f;
             if (BACK) {
                 const int64_t at = (row_base + row) * a.heads + h;
-                float x = 0.0f;
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    gf[nb][d] = load_row_frag<T>(gp + (int64_t)row * a.go.st, live, 32 * d + 8 * g, dim, a.mode);
-                    const Frag<T> of = load_row_frag<T>(a.o + at * dim, live, 32 * d + 8 * g, dim, a.mode);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x = fmaf((float)gf[nb][d][j], (float)of[j], x);
-                }
-                delta[nb] = groups_sum(x);
                 m[nb] = live ? a.stats[2 * at] : 0.0f;
                 sum[nb] = live ? a.stats[2 * at + 1] : 0.0f;
                 if (live && g == 0) a.delta[at] = delta[nb];
@@ -209,13 +201,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const KeyTiles tiles(r0, r1, a.window, a.sinks);
-        Staged<T, DP, kThreads> rk, rv;
-        rk.fetch(kp, a.k.st, tiles.first(), len, dim, a.mode);
-        rv.fetch(vp, a.v.st, tiles.first(), len, dim, a.mode);
+        Staged<T, DP, kThreads, BUF> rk, rv;
+        rk.fetch(kp, a.k.st, tiles.first(), len - tiles.first(), dim);
+        rv.fetch(vp, a.v.st, tiles.first(), len - tiles.first(), dim);
         for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), turn ^= 1) {
             __syncthreads();                                   // the tile before is read
-            rk.put(sk);
-            rv.put(sv);
+            rk.put(sk, dim);
+            rv.put(sv, dim);
             const bool edge = !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window);
             if (edge && (BACK ? rk : rv).not_finite()) flags[turn] = 1;
             __syncthreads();
@@ -223,8 +215,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             if (threadIdx.x == 0) flags[turn ^ 1] = 0;
             const int nt = tiles.next(t);
             if (nt < tiles.end) {
-                rk.fetch(kp, a.k.st, nt, len, dim, a.mode);
-                rv.fetch(vp, a.v.st, nt, len, dim, a.mode);
+                rk.fetch(kp, a.k.st, nt, len - nt, dim);
+                rv.fetch(vp, a.v.st, nt, len - nt, dim);
             }
             if (t > w1 || (w0 - (t + kTile - 1) >= a.window && t >= a.sinks)) continue;      // nothing for this wave
             f32x4 p[4][NB];
@@ -296,7 +288,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             }
             if (row < len) {
 #pragma unroll
-                for (int b = 0; b < DP / 16; ++b) store_quad(a.out + at * dim, 16 * b + 4 * g, dim, acc[b][nb] * f, a.wide_out);
+                for (int b = 0; b < DP / 16; ++b) store_quad(a.out + at * dim, 16 * b + 4 * g, dim, acc[b][nb] * f, BUF);
             }
         }
     }
@@ -306,10 +298,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 // rows beyond their window, one segment of the rows.
 //
 // The sink keys are few: there a block is one wave with 16 of them, blocks take turns at the segments.
-template <typename T, int DP, int NB, bool SINKS>
+template <typename T, int DP, int NB, bool SINKS, bool BUF>
 __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(WindowArgs<T> a) {
     constexpr int NT = SINKS ? 64 : kThreads;
-    using C = TileShape<T, DP, NT>;
+    using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
     T* sqr = reinterpret_cast<T*>(lds_raw);
     T* sgo = sqr + kTile * C::kLd;
@@ -353,25 +345,19 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
         const int keys = SINKS ? (a.sinks < len ? a.sinks : len) : len;
         Frag<T> kf[NB][DP / 32], vf[NB][DP / 32];
         f32x4 dk[DP / 16][NB], dv[DP / 16][NB];
+        load_own<T, DP, NB, NT, BUF>(kf, kp, a.k.st, j0, keys, dim, sqr);
+        load_own<T, DP, NB, NT, BUF>(vf, vp, a.v.st, j0, keys, dim, sqr);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int key = w0 + 16 * nb + c;
-            const bool live = key < keys;
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) {
-                kf[nb][d] = load_row_frag<T>(kp + (int64_t)key * a.k.st, live, 32 * d + 8 * g, dim, a.mode);
-                vf[nb][d] = load_row_frag<T>(vp + (int64_t)key * a.v.st, live, 32 * d + 8 * g, dim, a.mode);
-            }
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) dk[b][nb] = dv[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
         const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
-        Staged<T, DP, NT> rq, rg;
+        Staged<T, DP, NT, BUF> rq, rg;
         float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;          // of row threadIdx.x of the tile
         const auto fetch = [&](int step) {
             const int h = hk * group + step / n_tiles, t = i0 + step % n_tiles * kTile;
-            rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1, dim, a.mode);
-            rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1, dim, a.mode);
+            rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1 - t, dim);
+            rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1 - t, dim);
             const int row = t + threadIdx.x;
             if (threadIdx.x < kTile) {
                 const int64_t at = (row_base + row) * a.heads + h;
@@ -386,8 +372,8 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
             const int t = i0 + step % n_tiles * kTile;
             if (SINKS) fetch(step);                // one wave: its registers hold no tile ahead, other blocks hide the wait
             __syncthreads();
-            rq.put(sqr);
-            rg.put(sgo);
+            rq.put(sqr, dim);
+            rg.put(sgo, dim);
             if (threadIdx.x < kTile) {
                 sm[threadIdx.x] = rm;
                 sinv[threadIdx.x] = rinv;
@@ -434,15 +420,15 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
                 float* out = a.parts + (((((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + segment : 0)) * 2) * a.sinks + key) * dim;
 #pragma unroll
                 for (int b = 0; b < DP / 16; ++b) {
-                    store_quad(out, 16 * b + 4 * g, dim, dk[b][nb], false);
-                    store_quad(out + (int64_t)a.sinks * dim, 16 * b + 4 * g, dim, dv[b][nb], false);
+                    store_quad(out, 16 * b + 4 * g, dim, dk[b][nb], true);
+                    store_quad(out + (int64_t)a.sinks * dim, 16 * b + 4 * g, dim, dv[b][nb], true);
                 }
             } else if (!SINKS && key < len) {
                 const int64_t at = ((row_base + key) * a.kv_heads + hk) * dim;
 #pragma unroll
                 for (int b = 0; b < DP / 16; ++b) {
-                    store_quad(a.dk + at, 16 * b + 4 * g, dim, dk[b][nb], a.wide_out);
-                    store_quad(a.dv + at, 16 * b + 4 * g, dim, dv[b][nb], a.wide_out);
+                    store_quad(a.dk + at, 16 * b + 4 * g, dim, dk[b][nb], BUF);
+                    store_quad(a.dv + at, 16 * b + 4 * g, dim, dv[b][nb], BUF);
                 }
             }
         }
@@ -480,7 +466,7 @@ struct StepArgs {
     float* parts;                   // (batch, head, split): maximum, sum, dim values
     int heads, kv_heads, dim, window, sinks, splits, chunks;
     float scale;
-    int mode;                       // how rows of k, v and the caches are read
+    bool whole;                     // rows of k, v and the caches are whole words at 4-byte boundaries
 };
 
 // A wave takes 64 / (lanes of a row) slots at a time; a lane keeps 16 bytes of the row for each of GB query heads.
@@ -524,11 +510,11 @@ __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
             kr[u] = vr[u] = u32x4{0, 0, 0, 0};
             if (slot < hi) {
                 const bool mine = slot == own;
-                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.mode);
-                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.mode);
+                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.whole);
+                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.whole);
                 if (mine && chunk == 0) {       // the slot is read from the new row above, by every chunk
-                    store_piece(ck + slot * a.ck.st, d, a.dim, kr[u], a.mode);
-                    store_piece(cv + slot * a.cv.st, d, a.dim, vr[u], a.mode);
+                    store_piece(ck + slot * a.ck.st, d, a.dim, kr[u], a.whole);
+                    store_piece(cv + slot * a.cv.st, d, a.dim, vr[u], a.whole);
                 }
             }
         }
@@ -659,8 +645,8 @@ __global__ __launch_bounds__(kThreads) void window_fill_kernel(StepArgs<T> a, Se
             row = at < rolled ? a.sinks + at + (rolled - 1 - at) / a.window * a.window : len;
         }
         if (row >= len) continue;
-        store_piece(ck + slot * a.ck.st, d, a.dim, load_piece(kp + row * a.k.st, d, a.dim, a.mode), a.mode);
-        store_piece(cv + slot * a.cv.st, d, a.dim, load_piece(vp + row * a.v.st, d, a.dim, a.mode), a.mode);
+        store_piece(ck + slot * a.ck.st, d, a.dim, load_piece(kp + row * a.k.st, d, a.dim, a.whole), a.whole);
+        store_piece(cv + slot * a.cv.st, d, a.dim, load_piece(vp + row * a.v.st, d, a.dim, a.whole), a.whole);
     }
 }
 
@@ -687,29 +673,45 @@ unsigned row_tiles(int64_t max_len, int rows) {
     return (unsigned)(n < 1 ? 1 : n);
 }
 
+template <typename T, int DP, bool BUF>
+struct Kernels {
+    static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
+    static constexpr size_t kLds = TileShape<T, DP>::kLds;
+    static void forward(const WindowArgs<T>& a, hipStream_t st) {
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), dim3(kThreads), kLds, st, a);
+    }
+    static void backward(const WindowArgs<T>& a, hipStream_t st) {
+        const dim3 block(kThreads);
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, true, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), block, kLds, st, a);
+        hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, kLds, st, a);
+        if (a.sinks > 0) {
+            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.segments * ((a.sinks + 15) / 16), a.kv_heads, a.n_seq), dim3(64), kLds, st, a);
+            hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
+        }
+    }
+    static int allow() {
+        const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false, BUF>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, true, BUF>),
+                           reinterpret_cast<const void*>(&window_keys_kernel<T, DP, NK, false, BUF>), reinterpret_cast<const void*>(&window_keys_kernel<T, DP, 1, true, BUF>)};
+        for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
+        return VAD_OK;
+    }
+};
+
 template <typename T>
-int run_forward(WindowArgs<T> a, hipStream_t st) {
+int run_forward(const WindowArgs<T>& a, hipStream_t st) {
     for_dim(a.dim, [&](auto dp) {
-        constexpr int DP = decltype(dp)::value, NB = own_blocks<T>();
-        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), dim3(kThreads),
-                           (TileShape<T, DP>::kLds), st, a);
+        constexpr int DP = decltype(dp)::value;
+        a.whole ? Kernels<T, DP, true>::forward(a, st) : Kernels<T, DP, false>::forward(a, st);
     });
     VAD_HIP_CHECK(hipGetLastError());
     return VAD_OK;
 }
 
 template <typename T>
-int run_backward(WindowArgs<T> a, hipStream_t st) {
+int run_backward(const WindowArgs<T>& a, hipStream_t st) {
     for_dim(a.dim, [&](auto dp) {
-        constexpr int DP = decltype(dp)::value, NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
-        const dim3 block(kThreads);
-        const size_t lds = TileShape<T, DP>::kLds;
-        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, true>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), block, lds, st, a);
-        hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, lds, st, a);
-        if (a.sinks > 0) {
-            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true>), dim3(a.segments * ((a.sinks + 15) / 16), a.kv_heads, a.n_seq), dim3(64), lds, st, a);
-            hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
-        }
+        constexpr int DP = decltype(dp)::value;
+        a.whole ? Kernels<T, DP, true>::backward(a, st) : Kernels<T, DP, false>::backward(a, st);
     });
     VAD_HIP_CHECK(hipGetLastError());
     return VAD_OK;
@@ -717,11 +719,8 @@ int run_backward(WindowArgs<T> a, hipStream_t st) {
 
 template <typename T, int DP>
 int allow_tiles() {
-    constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
-    const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, true>),
-                       reinterpret_cast<const void*>(&window_keys_kernel<T, DP, NK, false>), reinterpret_cast<const void*>(&window_keys_kernel<T, DP, 1, true>)};
-    for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)TileShape<T, DP>::kLds));
-    return VAD_OK;
+    const int rc = Kernels<T, DP, true>::allow();
+    return rc != VAD_OK ? rc : Kernels<T, DP, false>::allow();
 }
 
 // Segments of the rows beyond the window for the sink keys' gradients: at least 128 rows each, enough one-wave blocks to fill
@@ -742,6 +741,11 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(n_seq >= 0 && n_seq <= 65535, "sequence count %lld out of range 0..65535", (long long)n_seq);
     VAD_REQUIRE(n_tokens >= 0 && max_len >= 0 && n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
     VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
+    return VAD_OK;
+}
+
+int check_rows(const int64_t* strides) {
+    VAD_REQUIRE(strides[1] >= 0 && strides[1] < VAD_MAX_ROW_STRIDE, "row stride %lld out of range", (long long)strides[1]);
     return VAD_OK;
 }
 
@@ -776,6 +780,8 @@ extern "C" int vad_window_attention_forward(const void* q_dev, const int64_t* q_
     VAD_REQUIRE(q_strides && k_strides && v_strides, "null pointer argument");
     if (n_seq == 0 || (starts_dev ? n_tokens : max_len) == 0) return VAD_OK;
     VAD_REQUIRE(q_dev && k_dev && v_dev && o_dev, "null pointer argument");
+    for (const int64_t* strides : {q_strides, k_strides, v_strides})
+        if ((rc = check_rows(strides)) != VAD_OK) return rc;
     rc = ensure_window_attention_attrs();
     if (rc != VAD_OK) return rc;
     const auto run = [&](auto zero) {
@@ -789,8 +795,7 @@ extern "C" int vad_window_attention_forward(const void* q_dev, const int64_t* q_
         a.seq = {starts_dev, n_tokens, max_len};
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
-        a.mode = std::min({load_mode(a.q, dim), load_mode(a.k, dim), load_mode(a.v, dim)});
-        a.wide_out = wide_rows(a.out, dim);
+        a.whole = whole_words(a.q, dim) && whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.out, dim);
         return run_forward<T>(a, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -818,6 +823,8 @@ extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q
     VAD_REQUIRE(q_strides && k_strides && v_strides && do_strides, "null pointer argument");
     if (n_seq == 0 || (starts_dev ? n_tokens : max_len) == 0) return VAD_OK;
     VAD_REQUIRE(q_dev && k_dev && v_dev && o_dev && do_dev && stats_dev && dq_dev && dk_dev && dv_dev && workspace_dev, "null pointer argument");
+    for (const int64_t* strides : {q_strides, k_strides, v_strides, do_strides})
+        if ((rc = check_rows(strides)) != VAD_OK) return rc;
     const int64_t n_rows = starts_dev ? n_tokens : n_seq * max_len;
     const size_t need = vad_window_attention_workspace_bytes(n_seq, n_rows, max_len, heads, kv_heads, dim, window, sinks);
     VAD_REQUIRE(workspace_bytes >= need, "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
@@ -841,9 +848,8 @@ extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
         a.segments = sink_segments(n_seq, max_len, kv_heads, (int)window);
-        const Heads<const T> o = {a.o, 0, (int64_t)heads * dim, dim};
-        a.mode = std::min({load_mode(a.q, dim), load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.go, dim), load_mode(o, dim)});
-        a.wide_out = wide_rows(a.out, dim) && wide_rows(a.dk, dim) && wide_rows(a.dv, dim);
+        a.whole = whole_words(a.q, dim) && whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.go, dim) && whole_words(a.o, dim) &&
+                  whole_words(a.out, dim) && whole_words(a.dk, dim) && whole_words(a.dv, dim);
         return run_backward<T>(a, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -923,7 +929,7 @@ extern "C" int vad_window_attention_step(const void* q_dev, const int64_t* q_str
         const int group = heads / kv_heads, gb = step_heads(group);
         a.chunks = (group + gb - 1) / gb;
         a.splits = step_splits(batch, kv_heads, a.chunks, sinks + window);
-        a.mode = std::min({load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.ck, dim), load_mode(a.cv, dim)});
+        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim);
         return run_step<T>(a, batch, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -948,7 +954,7 @@ extern "C" int vad_window_cache_fill(const void* k_dev, const int64_t* k_strides
         a.ck = {static_cast<T*>(cache_k_dev), cache_k_strides[0], cache_k_strides[1], cache_k_strides[2]};
         a.cv = {static_cast<T*>(cache_v_dev), cache_v_strides[0], cache_v_strides[1], cache_v_strides[2]};
         a.kv_heads = kv_heads, a.dim = dim, a.window = (int)window, a.sinks = sinks;
-        a.mode = std::min({load_mode(a.k, dim), load_mode(a.v, dim), load_mode(a.ck, dim), load_mode(a.cv, dim)});
+        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim);
         const Sequences seq = {starts_dev, n_tokens, max_len};
         const int64_t blocks = (((int64_t)sinks + window) * dim * sizeof(T) / 16 + kThreads) / kThreads;
         hipLaunchKernelGGL((window_fill_kernel<T>), dim3((unsigned)(blocks < 256 ? blocks : 256), kv_heads, (unsigned)n_seq), dim3(kThreads), 0,

@@ -25,7 +25,7 @@ from . import _lib
 
 MAX_HEAD_DIM = 128
 MAX_SINKS = 64
-MAX_ROW_STRIDE = 1 << 24
+MAX_ROW_STRIDE = 1 << 22
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 # A call's host time is a good part of a live frame's: what follows from shapes and strides alone (checks, stride tables,
