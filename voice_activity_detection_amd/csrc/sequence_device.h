@@ -280,6 +280,20 @@ struct Staged {
     }
 };
 
+// A tile's infinities and NaN become zero: every thread of the block cleans the pieces that it staged.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void clean_tile(T* tile) {
+    using S = Staged<T, DP, NT, true>;
+    const int row0 = threadIdx.x / S::kPPR, c = threadIdx.x % S::kPPR * S::kPer;
+#pragma unroll 1
+    for (int n = 0; n < S::kPieces; ++n) {
+        T* p = tile + (row0 + n * S::kStep) * S::kLd + c;
+#pragma unroll
+        for (int e = 0; e < S::kPer; ++e)
+            if (!(fabsf((float)p[e]) < INFINITY)) p[e] = (T)0.0f;
+    }
+}
+
 // ---- fragments from LDS ----
 
 // Lane c: row r0 + c, columns c0 + 8 g + j.
@@ -340,25 +354,6 @@ __device__ __forceinline__ f32x8 frag_columns(const float* tile, int ld, int r0,
         f[j + 4] = p[(16 + j) * ld];
     }
     return f;
-}
-
-// An operand's infinities and NaN taken out: they become zero, and `code` holds 1 for each +inf, 2^7 for each -inf, 2^14
-// for each NaN.  A product of `code` with zeros and ones adds them up exactly (64 terms); code_value turns the sum back
-// into what the values themselves would have contributed.
-template <typename T>
-__device__ __forceinline__ void take_out(Frag<T>& x, Frag<T>& code) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float v = (float)x[j];
-        const bool fine = fabsf(v) < INFINITY;
-        code[j] = (T)(fine ? 0.0f : (v == INFINITY ? 1.0f : (v == -INFINITY ? 128.0f : 16384.0f)));
-        x[j] = fine ? x[j] : (T)0.0f;
-    }
-}
-__device__ __forceinline__ float code_value(float n) {
-    const int c = (int)n;
-    const float plus = (c & 127) ? INFINITY : 0.0f, minus = (c & (127 << 7)) ? -INFINITY : 0.0f;
-    return c >= 1 << 14 ? NAN : plus + minus;
 }
 
 // Two stacked result tiles as an operand in split order.

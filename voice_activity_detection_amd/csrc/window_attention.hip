@@ -14,9 +14,11 @@
 // in registers.  The few sink keys are seen by every later row; their share of dK and dV is a second kernel over
 // segments of the rows, joined in a fixed order.
 //
-// A row outside a key's window must not feel what that key holds: scores are replaced, not multiplied, where the mask
-// says so, and where a partly visible tile holds an infinity or a NaN, 0 * NaN in the matrix product is avoided by adding
-// its rows one at a time.
+// A row outside a key's window must not feel what that key holds.  Scores are replaced, not multiplied, where the mask
+// says so.  Where a partly visible tile holds an infinity or a NaN, which the matrix product would multiply by zero, it is
+// taken out of the tile once the scores are formed.  A visible one still reaches its rows: through a weight that its own
+// score has made NaN, or, where no score depends on it (V in O, dO in dV), by a pass over the block's outputs at its end,
+// which costs a block that meets one milliseconds and the others nothing.
 
 #include <mutex>
 #include <type_traits>
@@ -72,43 +74,33 @@ __device__ __forceinline__ void load_own(Frag<T> (&f)[NB][DP / 32], const T* p, 
 }
 
 // acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
-// own row.  `careful`: the tile holds infinities or NaN, which only rows that `sees` admits may feel (0 * inf is NaN).
-template <typename T, int DP, int NB, typename Sees>
-__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB], f32x4 (&acc)[DP / 16][NB], bool careful, Sees sees) {
-    constexpr int kLd = TileShape<T, DP>::kLd;
+// own row.
+template <typename T, int DP, int NB>
+__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB], f32x4 (&acc)[DP / 16][NB]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         Frag<T> f[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
-        if (!careful) {
 #pragma unroll
-            for (int b = 0; b < DP / 16; ++b) {
-                const Frag<T> x = frag_columns(tile, kLd, 32 * t, 16 * b);
+        for (int b = 0; b < DP / 16; ++b) {
+            const Frag<T> x = frag_columns(tile, TileShape<T, DP>::kLd, 32 * t, 16 * b);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) acc[b][nb] = mma(x, f[nb], acc[b][nb]);
-            }
-        } else {
-            const int g = lane_id() >> 4;
-            Frag<T> seen[NB];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) seen[nb][j] = (T)(sees(32 * t + 4 * g + (j < 4 ? j : 12 + j), nb) ? 1.0f : 0.0f);
-#pragma unroll
-            for (int b = 0; b < DP / 16; ++b) {
-                Frag<T> x = frag_columns(tile, kLd, 32 * t, 16 * b), code;
-                take_out<T>(x, code);
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const f32x4 n = mma(code, seen[nb], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                    acc[b][nb] = mma(x, f[nb], acc[b][nb]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[b][nb][e] += code_value(n[e]);
-                }
-            }
+            for (int nb = 0; nb < NB; ++nb) acc[b][nb] = mma(x, f[nb], acc[b][nb]);
         }
     }
+}
+
+// What the infinities and NaN of rows [i0, i1) of a column add up to; zero where there are none.
+template <typename T>
+__device__ __forceinline__ float not_finite_sum(const T* p, int64_t st, int64_t i0, int64_t i1) {
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int64_t i = i0; i < i1; ++i) {
+        const float x = (float)p[i * st];
+        sum += fabsf(x) < INFINITY ? 0.0f : x;
+    }
+    return sum;
 }
 
 // s = tile own^T for the 64 streamed rows
@@ -164,6 +156,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
     zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     int turn = 0;
+    bool met = false;
     for (int64_t r0_64 = (int64_t)blockIdx.x * kRows; r0_64 < len; r0_64 += (int64_t)gridDim.x * kRows) {
         const int r0 = (int)r0_64, r1 = (len - r0 < kRows ? len - r0 : kRows) + r0 - 1;
         const int w0 = r0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
@@ -218,21 +211,31 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 rk.fetch(kp, a.k.st, nt, len - nt, dim);
                 rv.fetch(vp, a.v.st, nt, len - nt, dim);
             }
-            if (t > w1 || (w0 - (t + kTile - 1) >= a.window && t >= a.sinks)) continue;      // nothing for this wave
-            f32x4 p[4][NB];
-            scores<T, DP, NB>(sk, qf, p);
+            const bool active = t <= w1 && (w0 - (t + kTile - 1) < a.window || t < a.sinks);      // for this wave
+            f32x4 p[4][NB], dp[4][NB];
+            if (active) {
+                scores<T, DP, NB>(sk, qf, p);
+                if (BACK) scores<T, DP, NB>(sv, gf, dp);
+            }
+            if (careful) {
+                __syncthreads();
+                clean_tile<T, DP, kThreads>(BACK ? sk : sv);
+                __syncthreads();
+                met = true;
+            }
+            if (!active) continue;
             const bool masked = !(t + kTile - 1 <= w0 && w1 - t < a.window);
-            const auto sees = [&](int row, int nb) {
-                const int j = t + row, gap = w0 + 16 * nb + c - j;
-                return ((unsigned)gap < (unsigned)a.window) | ((gap >= 0) & (j < a.sinks));
-            };
             if (masked) {
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p[kb][nb][i] = sees(16 * kb + 4 * g + i, nb) ? p[kb][nb][i] : -INFINITY;
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = t + 16 * kb + 4 * g + i, gap = w0 + 16 * nb + c - j;
+                            const bool sees = ((unsigned)gap < (unsigned)a.window) | ((gap >= 0) & (j < a.sinks));
+                            p[kb][nb][i] = sees ? p[kb][nb][i] : -INFINITY;
+                        }
             }
             if (!BACK) {
 #pragma unroll
@@ -258,10 +261,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 #pragma unroll
                     for (int b = 0; b < DP / 16; ++b) acc[b][nb] *= shrink;
                 }
-                accumulate<T, DP, NB>(sv, p, acc, careful, sees);
+                accumulate<T, DP, NB>(sv, p, acc);
             } else {
-                f32x4 dp[4][NB];
-                scores<T, DP, NB>(sv, gf, dp);
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                             const float x = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -m[nb])) * sum[nb];
                             dp[kb][nb][i] = (p[kb][nb][i] == -INFINITY) & masked ? 0.0f : x * (dp[kb][nb][i] - delta[nb]) * a.scale;
                         }
-                accumulate<T, DP, NB>(sk, dp, acc, careful, sees);
+                accumulate<T, DP, NB>(sk, dp, acc);
             }
         }
 #pragma unroll
@@ -291,6 +292,16 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 for (int b = 0; b < DP / 16; ++b) store_quad(a.out + at * dim, 16 * b + 4 * g, dim, acc[b][nb] * f, BUF);
             }
         }
+        if (!BACK && met) {
+            __syncthreads();
+            for (int e = threadIdx.x; e < (r1 - r0 + 1) * dim; e += kThreads) {
+                const int row = r0 + e / dim, d = e % dim, lo = row - a.window + 1 > 0 ? row - a.window + 1 : 0;
+                const float x = not_finite_sum(vp + d, a.v.st, lo, (int64_t)row + 1) + not_finite_sum(vp + d, a.v.st, 0, lo < a.sinks ? lo : a.sinks);
+                T* o = a.out + ((row_base + row) * a.heads + h) * dim + d;
+                if (x != 0.0f) *o = (T)((float)*o + x);
+            }
+            met = false;
+        }
     }
 }
 
@@ -299,7 +310,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 //
 // The sink keys are few: there a block is one wave with 16 of them, blocks take turns at the segments.
 template <typename T, int DP, int NB, bool SINKS, bool BUF>
-__global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(WindowArgs<T> a) {
+__global__ __launch_bounds__(SINKS ? 64 : kThreads, 2) void window_keys_kernel(WindowArgs<T> a) {
     constexpr int NT = SINKS ? 64 : kThreads;
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
@@ -318,6 +329,8 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
     const T* kp = head_ptr(a.k, a.seq, s, first, hk);
     const T* vp = head_ptr(a.v, a.seq, s, first, hk);
     const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
+    // sink keys' sums go to the joining kernel in float32: [0] those of their window, [1 + n] of segment n
+    float* parts = a.parts + (((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + segment : 0)) * 2 * a.sinks * dim;
     const float l2scale = a.scale * kLog2e;
     constexpr int kKeys = NT / 4 * NB;
     if (!SINKS) {
@@ -326,6 +339,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
     }
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     int turn = 0;
+    bool met = false;
     // (the sink keys' blocks take one turn)
     for (int64_t j0_64 = (SINKS ? blockIdx.x / a.segments : (int64_t)blockIdx.x) * kKeys; j0_64 < len; j0_64 += SINKS ? len : (int64_t)gridDim.x * kKeys) {
         const int j0 = (int)j0_64;
@@ -385,15 +399,25 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
             const bool careful = edge && flags[turn];
             if (threadIdx.x == 0) flags[turn ^ 1] = 0;
             if (!SINKS && step + 1 < steps) fetch(step + 1);
-            if (w0 >= keys || (!SINKS && (t + kTile - 1 < w0 || t - w1 >= a.window))) continue;
+            const bool active = w0 < keys && (SINKS || (t + kTile - 1 >= w0 && t - w1 < a.window));
+            f32x4 p[4][NB], dp[4][NB];
+            if (active) {
+                scores<T, DP, NB>(sqr, kf, p);
+                scores<T, DP, NB>(sgo, vf, dp);
+            }
+            if (careful) {
+                __syncthreads();
+                clean_tile<T, DP, NT>(sqr);
+                clean_tile<T, DP, NT>(sgo);
+                __syncthreads();
+                met = true;
+            }
+            if (!active) continue;
             const auto sees = [&](int row, int nb) {
                 const int i = t + row, j = w0 + 16 * nb + c;
                 return (i < i1) & (SINKS ? (j < keys) & (i - j >= a.window) : (unsigned)(i - j) < (unsigned)a.window);
             };
             const bool masked = SINKS || !(t >= w1 && t + kTile - 1 - w0 < a.window && t + kTile <= i1);
-            f32x4 p[4][NB], dp[4][NB];
-            scores<T, DP, NB>(sqr, kf, p);
-            scores<T, DP, NB>(sgo, vf, dp);
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
                 const f32x4 mm = *reinterpret_cast<const f32x4*>(sm + 16 * kb + 4 * g);
@@ -409,15 +433,14 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
                         dp[kb][nb][i] = see ? x * (dp[kb][nb][i] - dl[i]) * a.scale : 0.0f;
                     }
             }
-            accumulate<T, DP, NB>(sgo, p, dv, careful, sees);
-            accumulate<T, DP, NB>(sqr, dp, dk, careful, sees);
+            accumulate<T, DP, NB>(sgo, p, dv);
+            accumulate<T, DP, NB>(sqr, dp, dk);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int key = w0 + 16 * nb + c;
             if (key < a.sinks && key < len) {
-                // a sink key's sums go to the joining kernel in float32: [0] of its window, [1 + n] of segment n
-                float* out = a.parts + (((((int64_t)s * a.kv_heads + hk) * (1 + a.segments) + (SINKS ? 1 + segment : 0)) * 2) * a.sinks + key) * dim;
+                float* out = parts + key * dim;
 #pragma unroll
                 for (int b = 0; b < DP / 16; ++b) {
                     store_quad(out, 16 * b + 4 * g, dim, dk[b][nb], true);
@@ -431,6 +454,23 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads) void window_keys_kernel(Wind
                     store_quad(a.dv + at, 16 * b + 4 * g, dim, dv[b][nb], BUF);
                 }
             }
+        }
+        if (met) {
+            __syncthreads();
+            const int n = (keys - j0 < kKeys ? keys - j0 : kKeys) * dim;
+            for (int e = threadIdx.x; e < n; e += NT) {
+                const int key = j0 + e / dim, d = e % dim;
+                const int64_t lo = SINKS ? (i0 > key + a.window ? i0 : key + a.window) : key, hi = SINKS ? i1 : (int64_t)key + a.window;
+                float x = 0.0f;
+                for (int h = hk * group; h < (hk + 1) * group; ++h)
+                    x += not_finite_sum(head_ptr(a.go, a.seq, s, first, h) + d, a.go.st, lo, hi < i1 ? hi : i1);
+                if (x == 0.0f) continue;
+                if (key < a.sinks)
+                    parts[((int64_t)a.sinks + key) * dim + d] += x;
+                else
+                    a.dv[((row_base + key) * a.kv_heads + hk) * dim + d] = (T)((float)a.dv[((row_base + key) * a.kv_heads + hk) * dim + d] + x);
+            }
+            met = false;
         }
     }
 }
@@ -675,14 +715,14 @@ unsigned row_tiles(int64_t max_len, int rows) {
 
 template <typename T, int DP, bool BUF>
 struct Kernels {
-    static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();
+    static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();       // of O; of dQ, dK and dV
     static constexpr size_t kLds = TileShape<T, DP>::kLds;
     static void forward(const WindowArgs<T>& a, hipStream_t st) {
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), dim3(kThreads), kLds, st, a);
     }
     static void backward(const WindowArgs<T>& a, hipStream_t st) {
         const dim3 block(kThreads);
-        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, true, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), block, kLds, st, a);
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NK, true, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.heads, a.n_seq), block, kLds, st, a);
         hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, kLds, st, a);
         if (a.sinks > 0) {
             hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.segments * ((a.sinks + 15) / 16), a.kv_heads, a.n_seq), dim3(64), kLds, st, a);
@@ -690,7 +730,7 @@ struct Kernels {
         }
     }
     static int allow() {
-        const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false, BUF>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, true, BUF>),
+        const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false, BUF>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NK, true, BUF>),
                            reinterpret_cast<const void*>(&window_keys_kernel<T, DP, NK, false, BUF>), reinterpret_cast<const void*>(&window_keys_kernel<T, DP, 1, true, BUF>)};
         for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
         return VAD_OK;
