@@ -44,6 +44,7 @@ struct WindowArgs {
     float* parts;                   // (seq, kv head, 1 + segments, dk | dv, sinks, dim)
     Sequences seq;
     int n_seq, heads, kv_heads, dim, window, sinks, segments;
+    unsigned tiles;                 // blocks per head and sequence
     float scale;
     bool whole;                     // all rows are whole words at 4-byte boundaries
 };
@@ -133,6 +134,13 @@ struct KeyTiles {
     __device__ __forceinline__ int next(int t) const { return sink && t == 0 ? band : t + kTile; }
 };
 
+// A launch's blocks are dealt to the eight dies in turn; this gives each die a contiguous range of the work, so that
+// neighbouring tiles and the query heads of a key head meet in one L2.
+__device__ __forceinline__ unsigned work_index() {
+    const unsigned n = gridDim.x, die = blockIdx.x % 8, rest = n % 8;
+    return die * (n / 8) + (die < rest ? die : rest) + blockIdx.x / 8;
+}
+
 // BACK == false: O and stats.  BACK == true: dQ and delta.
 template <typename T, int DP, int NB, bool BACK, bool BUF>
 __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> a) {
@@ -141,7 +149,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
     T* sk = reinterpret_cast<T*>(lds_raw);
     T* sv = sk + kTile * C::kLd;
     int* flags = reinterpret_cast<int*>(sv + kTile * C::kLd);
-    const int h = blockIdx.y, s = blockIdx.z, hk = h / (a.heads / a.kv_heads);
+    const unsigned work = work_index();
+    const int part = work % a.tiles, h = work / a.tiles % a.heads, s = work / a.tiles / a.heads, hk = h / (a.heads / a.kv_heads);
     int64_t first, len64;
     sequence_rows(a.seq, s, first, len64);
     const int len = (int)len64, dim = a.dim;
@@ -153,11 +162,11 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
     const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
     const float l2scale = a.scale * kLog2e;
     constexpr int kRows = 64 * NB;
-    zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
+    zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     int turn = 0;
     bool met = false;
-    for (int64_t r0_64 = (int64_t)blockIdx.x * kRows; r0_64 < len; r0_64 += (int64_t)gridDim.x * kRows) {
+    for (int64_t r0_64 = (int64_t)part * kRows; r0_64 < len; r0_64 += (int64_t)a.tiles * kRows) {
         const int r0 = (int)r0_64, r1 = (len - r0 < kRows ? len - r0 : kRows) + r0 - 1;
         const int w0 = r0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
         Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
@@ -238,17 +247,34 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                         }
             }
             if (!BACK) {
+                // The running maximum follows only where the weights would pass 2^8: the sums are the same, and the outputs
+                // are rescaled a few times per row instead of at every tile.
+                float top[NB];
+                bool grow = false;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    float top = p[0][nb][0];
+                    top[nb] = p[0][nb][0];
 #pragma unroll
                     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) top = fmaxf(top, p[kb][nb][i]);
-                    const float now = fmaxf(m[nb], groups_max(top) * l2scale);
-                    const float base = now == -INFINITY ? 0.0f : now;
-                    const float shrink = __builtin_amdgcn_exp2f(m[nb] - base);
-                    m[nb] = now;
+                        for (int i = 0; i < 4; ++i) top[nb] = fmaxf(top[nb], p[kb][nb][i]);
+                    top[nb] = groups_max(top[nb]) * l2scale;
+                    grow |= top[nb] > m[nb] + 8.0f;
+                }
+                if (__any(grow)) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const float now = fmaxf(m[nb], top[nb]);
+                        const float shrink = __builtin_amdgcn_exp2f(m[nb] - (now == -INFINITY ? 0.0f : now));
+                        m[nb] = now;
+                        sum[nb] *= shrink;
+#pragma unroll
+                        for (int b = 0; b < DP / 16; ++b) acc[b][nb] *= shrink;
+                    }
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float base = m[nb] == -INFINITY ? 0.0f : m[nb];
                     float part = 0.0f;
 #pragma unroll
                     for (int kb = 0; kb < 4; ++kb)
@@ -257,9 +283,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                             p[kb][nb][i] = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -base));
                             part += p[kb][nb][i];
                         }
-                    sum[nb] = fmaf(sum[nb], shrink, part);
-#pragma unroll
-                    for (int b = 0; b < DP / 16; ++b) acc[b][nb] *= shrink;
+                    sum[nb] += part;
                 }
                 accumulate<T, DP, NB>(sv, p, acc);
             } else {
@@ -310,7 +334,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 //
 // The sink keys are few: there a block is one wave with 16 of them, blocks take turns at the segments.
 template <typename T, int DP, int NB, bool SINKS, bool BUF>
-__global__ __launch_bounds__(SINKS ? 64 : kThreads, 2) void window_keys_kernel(WindowArgs<T> a) {
+__global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeof(T) == 4) ? 1 : 2) void window_keys_kernel(WindowArgs<T> a) {
     constexpr int NT = SINKS ? 64 : kThreads;
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
@@ -320,8 +344,9 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, 2) void window_keys_kernel(W
     float* sinv = sm + kTile;
     float* sdelta = sinv + kTile;
     int* flags = reinterpret_cast<int*>(sdelta + kTile);
-    const int hk = blockIdx.y, s = blockIdx.z, group = a.heads / a.kv_heads;
-    const int segment = SINKS ? blockIdx.x % a.segments : 0;
+    const unsigned work = work_index();
+    const int part = work % a.tiles, hk = work / a.tiles % a.kv_heads, s = work / a.tiles / a.kv_heads, group = a.heads / a.kv_heads;
+    const int segment = SINKS ? part % a.segments : 0;
     int64_t first, len64;
     sequence_rows(a.seq, s, first, len64);
     const int len = (int)len64, dim = a.dim;
@@ -334,14 +359,14 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, 2) void window_keys_kernel(W
     const float l2scale = a.scale * kLog2e;
     constexpr int kKeys = NT / 4 * NB;
     if (!SINKS) {
-        zero_outside(a.dk, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
-        zero_outside(a.dv, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, blockIdx.x, gridDim.x);
+        zero_outside(a.dk, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
+        zero_outside(a.dv, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
     }
     if (threadIdx.x < 2) flags[threadIdx.x] = 0;
     int turn = 0;
     bool met = false;
     // (the sink keys' blocks take one turn)
-    for (int64_t j0_64 = (SINKS ? blockIdx.x / a.segments : (int64_t)blockIdx.x) * kKeys; j0_64 < len; j0_64 += SINKS ? len : (int64_t)gridDim.x * kKeys) {
+    for (int64_t j0_64 = (SINKS ? part / a.segments : (int64_t)part) * kKeys; j0_64 < len; j0_64 += SINKS ? len : (int64_t)a.tiles * kKeys) {
         const int j0 = (int)j0_64;
         const int w0 = j0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
         // the rows [i0, i1) that see the keys
@@ -717,15 +742,18 @@ template <typename T, int DP, bool BUF>
 struct Kernels {
     static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();       // of O; of dQ, dK and dV
     static constexpr size_t kLds = TileShape<T, DP>::kLds;
-    static void forward(const WindowArgs<T>& a, hipStream_t st) {
-        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NB), a.heads, a.n_seq), dim3(kThreads), kLds, st, a);
+    static void forward(WindowArgs<T> a, hipStream_t st) {
+        a.tiles = row_tiles(a.seq.max_len, 64 * NB);
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(a.tiles * a.heads * a.n_seq), dim3(kThreads), kLds, st, a);
     }
-    static void backward(const WindowArgs<T>& a, hipStream_t st) {
+    static void backward(WindowArgs<T> a, hipStream_t st) {
         const dim3 block(kThreads);
-        hipLaunchKernelGGL((window_rows_kernel<T, DP, NK, true, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.heads, a.n_seq), block, kLds, st, a);
-        hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(row_tiles(a.seq.max_len, 64 * NK), a.kv_heads, a.n_seq), block, kLds, st, a);
+        a.tiles = row_tiles(a.seq.max_len, 64 * NK);
+        hipLaunchKernelGGL((window_rows_kernel<T, DP, NK, true, BUF>), dim3(a.tiles * a.heads * a.n_seq), block, kLds, st, a);
+        hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), block, kLds, st, a);
         if (a.sinks > 0) {
-            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.segments * ((a.sinks + 15) / 16), a.kv_heads, a.n_seq), dim3(64), kLds, st, a);
+            a.tiles = a.segments * ((a.sinks + 15) / 16);
+            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), dim3(64), kLds, st, a);
             hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
         }
     }
@@ -780,6 +808,7 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(sinks >= 0 && sinks <= VAD_MAX_SINKS, "sinks %d out of range 0..%d", sinks, VAD_MAX_SINKS);
     VAD_REQUIRE(n_seq >= 0 && n_seq <= 65535, "sequence count %lld out of range 0..65535", (long long)n_seq);
     VAD_REQUIRE(n_tokens >= 0 && max_len >= 0 && n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
+    VAD_REQUIRE((max_len / 64 + 1) * heads * n_seq <= 0x7FFFFFFF, "too many rows for one launch");
     VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
     return VAD_OK;
 }
