@@ -49,10 +49,15 @@ struct WindowArgs {
     bool whole;                     // all rows are whole words at 4-byte boundaries
 };
 
+// A block's LDS: tiles of two tensors, twice where that leaves room for two blocks on a compute unit -- the next tiles are
+// then written while the present ones are read, with one barrier between tiles instead of two.
 template <typename T, int DP>
 struct TileShape {
     static constexpr int kLd = DP + Elem<T>::kPer16B;
-    static constexpr size_t kLds = (size_t)2 * kTile * kLd * sizeof(T) + (3 * kTile + 4) * sizeof(float);
+    static constexpr int kTileElems = kTile * kLd;
+    static constexpr int kBuffers = 4 * kTileElems * sizeof(T) <= 72 * 1024 ? 2 : 1;
+    static constexpr int kExtra = 3 * kTile;          // floats per buffer beside the tiles
+    static constexpr size_t lds(int buffers) { return (size_t)buffers * (2 * kTileElems * sizeof(T) + kExtra * sizeof(float)) + 4 * sizeof(int); }
 };
 
 // Own rows first .. first + 64 NB - 1 of a head (zero from row `len` on) as fragments: by way of the block's two tiles.
@@ -146,9 +151,8 @@ template <typename T, int DP, int NB, bool BACK, bool BUF>
 __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> a) {
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
-    T* sk = reinterpret_cast<T*>(lds_raw);
-    T* sv = sk + kTile * C::kLd;
-    int* flags = reinterpret_cast<int*>(sv + kTile * C::kLd);
+    T* tiles = reinterpret_cast<T*>(lds_raw);             // K and V, once or twice
+    int* flags = reinterpret_cast<int*>(tiles + 2 * C::kBuffers * C::kTileElems);
     const unsigned work = work_index();
     const int part = work % a.tiles, h = work / a.tiles % a.heads, s = work / a.tiles / a.heads, hk = h / (a.heads / a.kv_heads);
     int64_t first, len64;
@@ -163,8 +167,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
     const float l2scale = a.scale * kLog2e;
     constexpr int kRows = 64 * NB;
     zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
-    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
-    int turn = 0;
+    // flags[turn]: the tile in hand holds infinities or NaN; the next tile's is set and the last one's cleared meanwhile
+    if (threadIdx.x < 3) flags[threadIdx.x] = 0;
+    int turn = 0, buffer = 0;
     bool met = false;
     for (int64_t r0_64 = (int64_t)part * kRows; r0_64 < len; r0_64 += (int64_t)a.tiles * kRows) {
         const int r0 = (int)r0_64, r1 = (len - r0 < kRows ? len - r0 : kRows) + r0 - 1;
@@ -172,11 +177,11 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
         Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
         f32x4 acc[DP / 16][NB];
         float m[NB], sum[NB], delta[NB];
-        load_own<T, DP, NB, kThreads, BUF>(qf, qp, a.q.st, r0, len, dim, sk);
+        load_own<T, DP, NB, kThreads, BUF>(qf, qp, a.q.st, r0, len, dim, tiles);
         if (BACK) {
             Frag<T> of[NB][DP / 32];
-            load_own<T, DP, NB, kThreads, BUF>(gf, gp, a.go.st, r0, len, dim, sk);
-            load_own<T, DP, NB, kThreads, BUF>(of, a.o + (row_base * a.heads + h) * dim, (int64_t)a.heads * dim, r0, len, dim, sk);
+            load_own<T, DP, NB, kThreads, BUF>(gf, gp, a.go.st, r0, len, dim, tiles);
+            load_own<T, DP, NB, kThreads, BUF>(of, a.o + (row_base * a.heads + h) * dim, (int64_t)a.heads * dim, r0, len, dim, tiles);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float x = 0.0f;
@@ -202,24 +207,42 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const KeyTiles tiles(r0, r1, a.window, a.sinks);
+        const KeyTiles keys(r0, r1, a.window, a.sinks);
         Staged<T, DP, kThreads, BUF> rk, rv;
-        rk.fetch(kp, a.k.st, tiles.first(), len - tiles.first(), dim);
-        rv.fetch(vp, a.v.st, tiles.first(), len - tiles.first(), dim);
-        for (int t = tiles.first(); t < tiles.end; t = tiles.next(t), turn ^= 1) {
-            __syncthreads();                                   // the tile before is read
-            rk.put(sk, dim);
-            rv.put(sv, dim);
-            const bool edge = !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window);
-            if (edge && (BACK ? rk : rv).not_finite()) flags[turn] = 1;
+        const auto fetch = [&](int t) {
+            const int left = t < keys.end ? len - t : 0;       // no branch: no rows behind the last tile
+            rk.fetch(kp, a.k.st, t, left, dim);
+            rv.fetch(vp, a.v.st, t, left, dim);
+        };
+        const auto is_edge = [&](int t) { return !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window); };
+        const auto put = [&](int t, int to, int flag) {
+            rk.put(tiles + 2 * to * C::kTileElems, dim);
+            rv.put(tiles + (2 * to + 1) * C::kTileElems, dim);
+            if (is_edge(t) && (BACK ? rk : rv).not_finite()) flags[flag] = 1;
+        };
+        fetch(keys.first());
+        __syncthreads();                                       // the own rows' fragments and the last tiles are read
+        if (C::kBuffers == 2) {
+            put(keys.first(), buffer, turn);
+            fetch(keys.next(keys.first()));
             __syncthreads();
-            const bool careful = edge && flags[turn];
-            if (threadIdx.x == 0) flags[turn ^ 1] = 0;
-            const int nt = tiles.next(t);
-            if (nt < tiles.end) {
-                rk.fetch(kp, a.k.st, nt, len - nt, dim);
-                rv.fetch(vp, a.v.st, nt, len - nt, dim);
+        }
+        for (int t = keys.first(); t < keys.end; t = keys.next(t)) {
+            const int nt = keys.next(t), after = turn == 2 ? 0 : turn + 1;
+            if (C::kBuffers == 2) {
+                put(nt, buffer ^ 1, after);
+                fetch(keys.next(nt));
+            } else {
+                if (t != keys.first()) __syncthreads();
+                put(t, 0, turn);
+                __syncthreads();
+                fetch(nt);
             }
+            T* sk = tiles + 2 * buffer * C::kTileElems;
+            T* sv = sk + C::kTileElems;
+            const bool edge = is_edge(t), careful = edge && flags[turn];
+            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
+            turn = after;
             const bool active = t <= w1 && (w0 - (t + kTile - 1) < a.window || t < a.sinks);      // for this wave
             f32x4 p[4][NB], dp[4][NB];
             if (active) {
@@ -232,7 +255,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 __syncthreads();
                 met = true;
             }
-            if (!active) continue;
+            if (active) {
             const bool masked = !(t + kTile - 1 <= w0 && w1 - t < a.window);
             if (masked) {
 #pragma unroll
@@ -298,6 +321,11 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                         }
                 accumulate<T, DP, NB>(sk, dp, acc);
             }
+            }
+            if (C::kBuffers == 2) {
+                buffer ^= 1;
+                __syncthreads();
+            }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -338,12 +366,10 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
     constexpr int NT = SINKS ? 64 : kThreads;
     using C = TileShape<T, DP>;
     extern __shared__ char lds_raw[];
-    T* sqr = reinterpret_cast<T*>(lds_raw);
-    T* sgo = sqr + kTile * C::kLd;
-    float* sm = reinterpret_cast<float*>(sgo + kTile * C::kLd);
-    float* sinv = sm + kTile;
-    float* sdelta = sinv + kTile;
-    int* flags = reinterpret_cast<int*>(sdelta + kTile);
+    constexpr int kBuffers = SINKS ? 1 : C::kBuffers;
+    T* tiles = reinterpret_cast<T*>(lds_raw);                                    // Q and dO, once or twice
+    float* extras = reinterpret_cast<float*>(tiles + 2 * kBuffers * C::kTileElems);      // maximum, 1 / sum, delta of their rows
+    int* flags = reinterpret_cast<int*>(extras + kBuffers * C::kExtra);
     const unsigned work = work_index();
     const int part = work % a.tiles, hk = work / a.tiles % a.kv_heads, s = work / a.tiles / a.kv_heads, group = a.heads / a.kv_heads;
     const int segment = SINKS ? part % a.segments : 0;
@@ -362,8 +388,8 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         zero_outside(a.dk, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
         zero_outside(a.dv, (int64_t)a.kv_heads * dim, hk * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
     }
-    if (threadIdx.x < 2) flags[threadIdx.x] = 0;
-    int turn = 0;
+    if (threadIdx.x < 3) flags[threadIdx.x] = 0;
+    int turn = 0, buffer = 0;
     bool met = false;
     // (the sink keys' blocks take one turn)
     for (int64_t j0_64 = (SINKS ? part / a.segments : (int64_t)part) * kKeys; j0_64 < len; j0_64 += SINKS ? len : (int64_t)a.tiles * kKeys) {
@@ -384,8 +410,8 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         const int keys = SINKS ? (a.sinks < len ? a.sinks : len) : len;
         Frag<T> kf[NB][DP / 32], vf[NB][DP / 32];
         f32x4 dk[DP / 16][NB], dv[DP / 16][NB];
-        load_own<T, DP, NB, NT, BUF>(kf, kp, a.k.st, j0, keys, dim, sqr);
-        load_own<T, DP, NB, NT, BUF>(vf, vp, a.v.st, j0, keys, dim, sqr);
+        load_own<T, DP, NB, NT, BUF>(kf, kp, a.k.st, j0, keys, dim, tiles);
+        load_own<T, DP, NB, NT, BUF>(vf, vp, a.v.st, j0, keys, dim, tiles);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -393,8 +419,11 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
         Staged<T, DP, NT, BUF> rq, rg;
         float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;          // of row threadIdx.x of the tile
+        const int steps = n_tiles * group;
+        const auto row_of = [&](int step) { return i0 + step % n_tiles * kTile; };
         const auto fetch = [&](int step) {
-            const int h = hk * group + step / n_tiles, t = i0 + step % n_tiles * kTile;
+            if (step >= steps) return;
+            const int h = hk * group + step / n_tiles, t = row_of(step);
             rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1 - t, dim);
             rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1 - t, dim);
             const int row = t + threadIdx.x;
@@ -405,25 +434,46 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
                 rdelta = row < i1 ? a.delta[at] : 0.0f;
             }
         };
-        const int steps = n_tiles * group;
-        if (steps && !SINKS) fetch(0);
-        for (int step = 0; step < steps; ++step, turn ^= 1) {
-            const int t = i0 + step % n_tiles * kTile;
-            if (SINKS) fetch(step);                // one wave: its registers hold no tile ahead, other blocks hide the wait
-            __syncthreads();
-            rq.put(sqr, dim);
-            rg.put(sgo, dim);
+        const auto is_edge = [&](int t) { return SINKS || !(t >= j0 + kKeys - 1 && t + kTile - 1 - j0 < a.window); };
+        const auto put = [&](int step, int to, int flag) {
+            if (step >= steps) return;
+            rq.put(tiles + 2 * to * C::kTileElems, dim);
+            rg.put(tiles + (2 * to + 1) * C::kTileElems, dim);
             if (threadIdx.x < kTile) {
-                sm[threadIdx.x] = rm;
-                sinv[threadIdx.x] = rinv;
-                sdelta[threadIdx.x] = rdelta;
+                float* e = extras + to * C::kExtra + threadIdx.x;
+                e[0] = rm;
+                e[kTile] = rinv;
+                e[2 * kTile] = rdelta;
             }
-            const bool edge = SINKS || !(t >= j0 + kKeys - 1 && t + kTile - 1 - j0 < a.window);
-            if (edge && (rq.not_finite() || rg.not_finite())) flags[turn] = 1;
+            if (is_edge(row_of(step)) && (rq.not_finite() || rg.not_finite())) flags[flag] = 1;
+        };
+        if (!SINKS) fetch(0);
+        __syncthreads();                                       // the own rows' fragments and the last tiles are read
+        if (kBuffers == 2) {
+            put(0, buffer, turn);
+            fetch(1);
             __syncthreads();
-            const bool careful = edge && flags[turn];
-            if (threadIdx.x == 0) flags[turn ^ 1] = 0;
-            if (!SINKS && step + 1 < steps) fetch(step + 1);
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int t = row_of(step), after = turn == 2 ? 0 : turn + 1;
+            if (kBuffers == 2) {
+                put(step + 1, buffer ^ 1, after);
+                fetch(step + 2);
+            } else {
+                if (SINKS) fetch(step);                        // one wave: its registers hold no tile ahead, other blocks hide the wait
+                if (step) __syncthreads();
+                put(step, 0, turn);
+                __syncthreads();
+                if (!SINKS) fetch(step + 1);
+            }
+            T* sqr = tiles + 2 * buffer * C::kTileElems;
+            T* sgo = sqr + C::kTileElems;
+            const float* sm = extras + buffer * C::kExtra;
+            const float* sinv = sm + kTile;
+            const float* sdelta = sinv + kTile;
+            const bool careful = is_edge(t) && flags[turn];
+            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
+            turn = after;
             const bool active = w0 < keys && (SINKS || (t + kTile - 1 >= w0 && t - w1 < a.window));
             f32x4 p[4][NB], dp[4][NB];
             if (active) {
@@ -437,7 +487,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
                 __syncthreads();
                 met = true;
             }
-            if (!active) continue;
+            if (active) {
             const auto sees = [&](int row, int nb) {
                 const int i = t + row, j = w0 + 16 * nb + c;
                 return (i < i1) & (SINKS ? (j < keys) & (i - j >= a.window) : (unsigned)(i - j) < (unsigned)a.window);
@@ -460,6 +510,11 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
             }
             accumulate<T, DP, NB>(sgo, p, dv);
             accumulate<T, DP, NB>(sqr, dp, dk);
+            }
+            if (kBuffers == 2) {
+                buffer ^= 1;
+                __syncthreads();
+            }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -741,7 +796,7 @@ unsigned row_tiles(int64_t max_len, int rows) {
 template <typename T, int DP, bool BUF>
 struct Kernels {
     static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();       // of O; of dQ, dK and dV
-    static constexpr size_t kLds = TileShape<T, DP>::kLds;
+    static constexpr size_t kLds = TileShape<T, DP>::lds(TileShape<T, DP>::kBuffers), kLdsSinks = TileShape<T, DP>::lds(1);
     static void forward(WindowArgs<T> a, hipStream_t st) {
         a.tiles = row_tiles(a.seq.max_len, 64 * NB);
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(a.tiles * a.heads * a.n_seq), dim3(kThreads), kLds, st, a);
@@ -753,7 +808,7 @@ struct Kernels {
         hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), block, kLds, st, a);
         if (a.sinks > 0) {
             a.tiles = a.segments * ((a.sinks + 15) / 16);
-            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), dim3(64), kLds, st, a);
+            hipLaunchKernelGGL((window_keys_kernel<T, DP, 1, true, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), dim3(64), kLdsSinks, st, a);
             hipLaunchKernelGGL((window_join_kernel<T>), dim3((2 * a.sinks * a.dim + kThreads - 1) / kThreads, a.kv_heads, a.n_seq), block, 0, st, a);
         }
     }
