@@ -153,7 +153,7 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
     const T* qp = STATE ? nullptr : head_ptr(w.q, a.seq, s, first, h);
     T* op = w.o + ((a.seq.starts ? first : (int64_t)s * a.seq.max_len) * a.heads + h) * dim;
     const int sign = w.reverse ? -1 : 1;
-    Staged<T, DP, C::kThreads, BUF> rk, rv, rq;
+    Staged<T, DP, C::kThreads, BUF, C::kLd> rk, rv, rq;
     const auto fetch = [&](int64_t tc) {
         const int64_t at = w.reverse ? len - 1 - tc : tc;
         const int rows = (int)(t1 - tc < kPiece ? t1 - tc : kPiece);

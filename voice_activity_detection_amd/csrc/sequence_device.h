@@ -233,10 +233,11 @@ __device__ __forceinline__ bool piece_not_finite(u32x4 v) {
     return bad;
 }
 
-// 64 rows of one head on their way through a block's registers into an LDS tile.  BUF: by buffer loads (whole_words).
-template <typename T, int DP, int NT, bool BUF>
+// 64 rows of one head on their way through a block's registers into an LDS tile of PITCH elements a row.  BUF: by buffer
+// loads (whole_words).
+template <typename T, int DP, int NT, bool BUF, int PITCH>
 struct Staged {
-    static constexpr int kPer = Elem<T>::kPer16B, kPPR = DP / kPer, kLd = DP + kPer, kPieces = 64 * kPPR / NT, kStep = NT / kPPR;
+    static constexpr int kPer = Elem<T>::kPer16B, kPPR = DP / kPer, kLd = PITCH, kPieces = 64 * kPPR / NT, kStep = NT / kPPR;
     u32x4 r[kPieces];
 
     // Tile row i is row at + i of the head (`back`: at - i) for i < rows, zero from there on; uniform arguments.
@@ -281,9 +282,9 @@ struct Staged {
 };
 
 // A tile's infinities and NaN become zero: every thread of the block cleans the pieces that it staged.
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, int PITCH>
 __device__ __forceinline__ void clean_tile(T* tile) {
-    using S = Staged<T, DP, NT, true>;
+    using S = Staged<T, DP, NT, true, PITCH>;
     const int row0 = threadIdx.x / S::kPPR, c = threadIdx.x % S::kPPR * S::kPer;
 #pragma unroll 1
     for (int n = 0; n < S::kPieces; ++n) {

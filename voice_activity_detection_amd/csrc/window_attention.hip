@@ -53,7 +53,10 @@ struct WindowArgs {
 // then written while the present ones are read, with one barrier between tiles instead of two.
 template <typename T, int DP>
 struct TileShape {
-    static constexpr int kLd = DP + Elem<T>::kPer16B;
+    // The padding spreads the banks (64 of 4 bytes): eight rows' 16-byte pieces at one column, and as many rows' 32-byte
+    // pieces as the transposing read takes them, fall into different ones.  (64 columns of bfloat16 would want 16 elements
+    // as well, but with 8 a fourth block fits the compute unit's LDS: 291 against 335 us on 4 x 16 heads of 8192 rows.)
+    static constexpr int kLd = DP + (sizeof(T) == 4 ? 4 : (DP == 64 ? 8 : 16));
     static constexpr int kTileElems = kTile * kLd;
     static constexpr int kBuffers = 4 * kTileElems * sizeof(T) <= 72 * 1024 ? 2 : 1;
     static constexpr int kExtra = 3 * kTile;          // floats per buffer beside the tiles
@@ -65,7 +68,7 @@ template <typename T, int DP, int NB, int NT, bool BUF>
 __device__ __forceinline__ void load_own(Frag<T> (&f)[NB][DP / 32], const T* p, int64_t st, int first, int len, int dim, T* tiles) {
     constexpr int kLd = TileShape<T, DP>::kLd;
     const int wave = threadIdx.x >> 6;
-    Staged<T, DP, NT, BUF> r;
+    Staged<T, DP, NT, BUF, kLd> r;
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const KeyTiles keys(r0, r1, a.window, a.sinks);
-        Staged<T, DP, kThreads, BUF> rk, rv;
+        Staged<T, DP, kThreads, BUF, C::kLd> rk, rv;
         const auto fetch = [&](int t) {
             const int left = t < keys.end ? len - t : 0;       // no branch: no rows behind the last tile
             rk.fetch(kp, a.k.st, t, left, dim);
@@ -240,23 +243,23 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             }
             T* sk = tiles + 2 * buffer * C::kTileElems;
             T* sv = sk + C::kTileElems;
-            const bool edge = is_edge(t), careful = edge && flags[turn];
-            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
-            turn = after;
-            const bool active = t <= w1 && (w0 - (t + kTile - 1) < a.window || t < a.sinks);      // for this wave
+            // EDGE: some row of the block does not see all of the tile
+            const auto step = [&](auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
+            const bool active = !EDGE || (t <= w1 && (w0 - (t + kTile - 1) < a.window || t < a.sinks));      // for this wave
             f32x4 p[4][NB], dp[4][NB];
             if (active) {
                 scores<T, DP, NB>(sk, qf, p);
                 if (BACK) scores<T, DP, NB>(sv, gf, dp);
             }
-            if (careful) {
+            if (EDGE && flags[turn]) {
                 __syncthreads();
-                clean_tile<T, DP, kThreads>(BACK ? sk : sv);
+                clean_tile<T, DP, kThreads, C::kLd>(BACK ? sk : sv);
                 __syncthreads();
                 met = true;
             }
             if (active) {
-            const bool masked = !(t + kTile - 1 <= w0 && w1 - t < a.window);
+            const bool masked = EDGE && !(t + kTile - 1 <= w0 && w1 - t < a.window);
             if (masked) {
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
@@ -322,6 +325,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 accumulate<T, DP, NB>(sk, dp, acc);
             }
             }
+            };
+            // (the forward pass is faster with one body that asks: 254 against 322 us on 2 x 16 heads of 8192 rows of 128)
+            if (!BACK || is_edge(t))
+                step(std::true_type{});
+            else
+                step(std::false_type{});
+            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
+            turn = after;
             if (C::kBuffers == 2) {
                 buffer ^= 1;
                 __syncthreads();
@@ -417,7 +428,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) dk[b][nb] = dv[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
-        Staged<T, DP, NT, BUF> rq, rg;
+        Staged<T, DP, NT, BUF, C::kLd> rq, rg;
         float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;          // of row threadIdx.x of the tile
         const int steps = n_tiles * group;
         const auto row_of = [&](int step) { return i0 + step % n_tiles * kTile; };
@@ -434,7 +445,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
                 rdelta = row < i1 ? a.delta[at] : 0.0f;
             }
         };
-        const auto is_edge = [&](int t) { return SINKS || !(t >= j0 + kKeys - 1 && t + kTile - 1 - j0 < a.window); };
+        const auto is_edge = [&](int t) { return SINKS || !(t >= j0 + kKeys - 1 && t + kTile - 1 - j0 < a.window && t + kTile <= i1 && j0 + kKeys <= keys); };
         const auto put = [&](int step, int to, int flag) {
             if (step >= steps) return;
             rq.put(tiles + 2 * to * C::kTileElems, dim);
@@ -471,19 +482,18 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
             const float* sm = extras + buffer * C::kExtra;
             const float* sinv = sm + kTile;
             const float* sdelta = sinv + kTile;
-            const bool careful = is_edge(t) && flags[turn];
-            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
-            turn = after;
-            const bool active = w0 < keys && (SINKS || (t + kTile - 1 >= w0 && t - w1 < a.window));
+            const auto work_on = [&](auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
+            const bool active = !EDGE || (w0 < keys && (SINKS || (t + kTile - 1 >= w0 && t - w1 < a.window)));
             f32x4 p[4][NB], dp[4][NB];
             if (active) {
                 scores<T, DP, NB>(sqr, kf, p);
                 scores<T, DP, NB>(sgo, vf, dp);
             }
-            if (careful) {
+            if (EDGE && flags[turn]) {
                 __syncthreads();
-                clean_tile<T, DP, NT>(sqr);
-                clean_tile<T, DP, NT>(sgo);
+                clean_tile<T, DP, NT, C::kLd>(sqr);
+                clean_tile<T, DP, NT, C::kLd>(sgo);
                 __syncthreads();
                 met = true;
             }
@@ -492,7 +502,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
                 const int i = t + row, j = w0 + 16 * nb + c;
                 return (i < i1) & (SINKS ? (j < keys) & (i - j >= a.window) : (unsigned)(i - j) < (unsigned)a.window);
             };
-            const bool masked = SINKS || !(t >= w1 && t + kTile - 1 - w0 < a.window && t + kTile <= i1);
+            const bool masked = EDGE && (SINKS || !(t >= w1 && t + kTile - 1 - w0 < a.window && t + kTile <= i1));
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
                 const f32x4 mm = *reinterpret_cast<const f32x4*>(sm + 16 * kb + 4 * g);
@@ -511,6 +521,13 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
             accumulate<T, DP, NB>(sgo, p, dv);
             accumulate<T, DP, NB>(sqr, dp, dk);
             }
+            };
+            if (is_edge(t))
+                work_on(std::true_type{});
+            else
+                work_on(std::false_type{});
+            if (threadIdx.x == 0) flags[after == 2 ? 0 : after + 1] = 0;
+            turn = after;
             if (kBuffers == 2) {
                 buffer ^= 1;
                 __syncthreads();
@@ -775,9 +792,6 @@ Heads<const T> heads_of(const void* p, const int64_t* s) {
     return {static_cast<const T*>(p), s[0], s[1], s[2]};
 }
 
-template <typename T>
-constexpr int own_blocks() { return sizeof(T) == 2 ? 2 : 1; }     // 16-row blocks of own rows per wave
-
 template <typename F>
 void for_dim(int dim, F f) {
     if (dim <= 32)
@@ -795,7 +809,11 @@ unsigned row_tiles(int64_t max_len, int rows) {
 
 template <typename T, int DP, bool BUF>
 struct Kernels {
-    static constexpr int NB = own_blocks<T>(), NK = DP == 128 ? 1 : own_blocks<T>();       // of O; of dQ, dK and dV
+    // 16-row blocks of own rows per wave.  Two read a streamed tile half as often, one leaves registers for twice the waves: 16
+    // heads of 8192 rows with a window of 1000 (4 sequences of 64 columns; 2 of 128) take 298 and 320 us for O with one and
+    // two blocks at 64 columns, 300 and 235 us at 128; dQ 472 and 469, dK and dV 602 and 541 us at 64 columns, but 61 and 66,
+    // 68 and 92 us on 8 sequences of up to 2000 rows with a window of 300.
+    static constexpr int NB = DP == 128 && sizeof(T) == 2 ? 2 : 1, NK = 1;
     static constexpr size_t kLds = TileShape<T, DP>::lds(TileShape<T, DP>::kBuffers), kLdsSinks = TileShape<T, DP>::lds(1);
     static void forward(WindowArgs<T> a, hipStream_t st) {
         a.tiles = row_tiles(a.seq.max_len, 64 * NB);
