@@ -314,6 +314,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_join_kernel(const float* 
     const int c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4, which = blockIdx.y;
     float v = 0.0f;
     if (c < cols)
+#pragma unroll 8
         for (int p = r; p < parts; p += 16) v += part[((int64_t)p * 2 + which) * cols + c];
     s[r][threadIdx.x & 15] = v;
     __syncthreads();

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 // dK and dV.  SINKS == false: the block's keys against the rows of their window.  SINKS == true: the sink keys against the
 // rows beyond their window, one segment of the rows.
 //
-// The sink keys are few: there a block is one wave with 16 of them, blocks take turns at the segments.
+// The sink keys are few: there a block is one wave with 16 of them, against one segment of the rows of one query head.
 template <typename T, int DP, int NB, bool SINKS, bool BUF>
 __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeof(T) == 4) ? 1 : 2) void window_keys_kernel(WindowArgs<T> a) {
     constexpr int NT = SINKS ? 64 : kThreads;
@@ -409,9 +409,9 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         // the rows [i0, i1) that see the keys
         int i0 = j0, i1;
         if (SINKS) {
-            const int beyond = len > a.window ? len - a.window : 0;
-            const int per = ((beyond + a.segments - 1) / a.segments + kTile - 1) / kTile * kTile;
-            const int64_t lo = a.window + (int64_t)segment * per;
+            const int beyond = len > a.window ? len - a.window : 0, cuts = a.segments / group;
+            const int per = ((beyond + cuts - 1) / cuts + kTile - 1) / kTile * kTile;
+            const int64_t lo = a.window + (int64_t)(segment / group) * per;
             i0 = (int)(lo < len ? lo : len);
             i1 = (int)(lo + per < len ? lo + per : len);
         } else {
@@ -430,11 +430,11 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         const int n_tiles = i1 > i0 ? (i1 - i0 + kTile - 1) / kTile : 0;
         Staged<T, DP, NT, BUF, C::kLd> rq, rg;
         float rm = 0.0f, rinv = 0.0f, rdelta = 0.0f;          // of row threadIdx.x of the tile
-        const int steps = n_tiles * group;
+        const int h0 = hk * group + (SINKS ? segment % group : 0), heads = SINKS ? 1 : group, steps = n_tiles * heads;
         const auto row_of = [&](int step) { return i0 + step % n_tiles * kTile; };
         const auto fetch = [&](int step) {
             if (step >= steps) return;
-            const int h = hk * group + step / n_tiles, t = row_of(step);
+            const int h = h0 + step / n_tiles, t = row_of(step);
             rq.fetch(head_ptr(a.q, a.seq, s, first, h), a.q.st, t, i1 - t, dim);
             rg.fetch(head_ptr(a.go, a.seq, s, first, h), a.go.st, t, i1 - t, dim);
             const int row = t + threadIdx.x;
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
                 const int key = j0 + e / dim, d = e % dim;
                 const int64_t lo = SINKS ? (i0 > key + a.window ? i0 : key + a.window) : key, hi = SINKS ? i1 : (int64_t)key + a.window;
                 float x = 0.0f;
-                for (int h = hk * group; h < (hk + 1) * group; ++h)
+                for (int h = h0; h < h0 + heads; ++h)
                     x += not_finite_sum(head_ptr(a.go, a.seq, s, first, h) + d, a.go.st, lo, hi < i1 ? hi : i1);
                 if (x == 0.0f) continue;
                 if (key < a.sinks)
@@ -584,6 +584,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WindowArgs<T> a) 
     if (key >= len) return;
     const float* p = a.parts + ((int64_t)s * a.kv_heads + hk) * (1 + a.segments) * 2 * n + e;
     float x = 0.0f;
+#pragma unroll 8
     for (int i = 0; i <= a.segments; ++i) x += p[(int64_t)i * 2 * n];
     const int64_t row = (a.seq.starts ? first : (int64_t)s * a.seq.max_len) + key;
     (which ? a.dv : a.dk)[(row * a.kv_heads + hk) * a.dim + d] = (T)x;
@@ -864,13 +865,13 @@ int allow_tiles() {
     return rc != VAD_OK ? rc : Kernels<T, DP, false>::allow();
 }
 
-// Segments of the rows beyond the window for the sink keys' gradients: at least 128 rows each, enough one-wave blocks to fill
-// the chip.
-int sink_segments(int64_t n_seq, int64_t max_len, int kv_heads, int window) {
-    const int64_t beyond = max_len > window ? max_len - window : 0, blocks = n_seq * kv_heads;
+// Segments (cuts of the rows beyond the window times query heads of a key head) for the sink keys' gradients: at least one
+// tile of rows each, enough one-wave blocks to fill the chip.
+int sink_segments(int64_t n_seq, int64_t max_len, int heads, int kv_heads, int window) {
+    const int64_t beyond = max_len > window ? max_len - window : 0, blocks = n_seq * heads;
     int64_t n = (2048 + blocks - 1) / blocks;
-    if (n > beyond / 128) n = beyond / 128;
-    return (int)(n < 1 ? 1 : n);
+    if (n > beyond / kTile) n = beyond / kTile;
+    return (int)(n < 1 ? 1 : n) * (heads / kv_heads);
 }
 
 int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int kv_heads, int dim, int dtype, int64_t window, int sinks) {
@@ -948,7 +949,7 @@ extern "C" size_t vad_window_attention_workspace_bytes(int64_t n_seq, int64_t n_
     using namespace vad;
     if (n_seq <= 0 || n_rows <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || window <= 0 || sinks < 0) return 0;
     size_t floats = (size_t)n_rows * heads;
-    if (sinks > 0) floats += (size_t)n_seq * kv_heads * (1 + sink_segments(n_seq, max_len, kv_heads, (int)window)) * 2 * sinks * dim;
+    if (sinks > 0) floats += (size_t)n_seq * kv_heads * (1 + sink_segments(n_seq, max_len, heads, kv_heads, (int)window)) * 2 * sinks * dim;
     return floats * sizeof(float);
 }
 
@@ -989,7 +990,7 @@ extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q
         a.seq = {starts_dev, n_tokens, max_len};
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
-        a.segments = sink_segments(n_seq, max_len, kv_heads, (int)window);
+        a.segments = sink_segments(n_seq, max_len, heads, kv_heads, (int)window);
         a.whole = whole_words(a.q, dim) && whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.go, dim) && whole_words(a.o, dim) &&
                   whole_words(a.out, dim) && whole_words(a.dk, dim) && whole_words(a.dv, dim);
         return run_backward<T>(a, static_cast<hipStream_t>(stream));
