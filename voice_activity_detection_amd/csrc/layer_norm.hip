@@ -28,8 +28,10 @@ struct Vec<T, 1> {
 };
 
 template <typename T, int VE>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[VE]) {
-    typename Vec<T, VE>::type x = *reinterpret_cast<const typename Vec<T, VE>::type*>(p);
+using Raw = typename Vec<T, VE>::type;
+
+template <typename T, int VE>
+__device__ __forceinline__ void unpack(Raw<T, VE> x, float (&v)[VE]) {
     T e[VE];
     __builtin_memcpy(e, &x, sizeof(x));
 #pragma unroll
@@ -45,7 +47,8 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VE]) {
     *reinterpret_cast<typename Vec<T, VE>::type*>(p) = x;
 }
 
-// Weights are float32 or of x's type (half the bytes); `wide`: 16-byte loads are allowed.
+// Weights are float32 or of x's type.  VE of them from column c on, `absent` where there are none: whole words where the
+// pointer allows (columns come in multiples of VE).
 template <typename T>
 struct Params {
     const void* w;
@@ -53,6 +56,37 @@ struct Params {
     bool f32;
     __device__ __forceinline__ float at(const void* p, int c) const {
         return f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+    }
+    template <int VE>
+    __device__ __forceinline__ void load(const void* p, int c, int cols, float absent, float (&v)[VE]) const {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[i] = absent;
+        if (!p || c >= cols) return;
+        if (f32) {
+            const float* q = static_cast<const float*>(p) + c;
+            if (VE % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < VE; i += 4) {
+                    const u32x4 r = *reinterpret_cast<const u32x4_any*>(q + i);
+                    __builtin_memcpy(v + i, &r, 16);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) v[i] = q[i];
+            }
+        } else {
+            const T* q = static_cast<const T*>(p) + c;
+            if (sizeof(T) == 2 && VE % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0) {
+                const u32x4 r = *reinterpret_cast<const u32x4_any*>(q);
+                T e[VE];
+                __builtin_memcpy(e, &r, 16);
+#pragma unroll
+                for (int i = 0; i < VE; ++i) v[i] = (float)e[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) v[i] = (float)q[i];
+            }
+        }
     }
 };
 
@@ -84,29 +118,35 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T* __restric
     const int64_t step = (int64_t)gridDim.x * per_block;
     float w[NV][VE], b[NV][VE];
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int n = 0; n < NV; ++n) {
+        pr.load(pr.w, (l + n * a.lanes) * VE, a.cols, 1.0f, w[n]);
+        pr.load(pr.b, (l + n * a.lanes) * VE, a.cols, 0.0f, b[n]);
+    }
+    Raw<T, VE> ahead[NV];                      // the next row is on its way while this one is worked on
+    const auto fetch = [&](int64_t base) {
+        const int64_t row = base + threadIdx.x / a.lanes;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const int c = (l + n * a.lanes) * VE + e;
-            w[n][e] = pr.w && c < a.cols ? pr.at(pr.w, c) : 1.0f;
-            b[n][e] = pr.b && c < a.cols ? pr.at(pr.b, c) : 0.0f;
+        for (int n = 0; n < NV; ++n) {
+            const int c = (l + n * a.lanes) * VE;
+            if (row < a.rows && c < a.cols) ahead[n] = *reinterpret_cast<const Raw<T, VE>*>(x + row * a.x_stride + c);
         }
+    };
+#pragma unroll
+    for (int n = 0; n < NV; ++n) ahead[n] = Raw<T, VE>{};
+    fetch((int64_t)blockIdx.x * per_block);
     // every group of a block makes the same number of turns: a whole-block group meets barriers
     for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows; base += step) {
         const int64_t row = base + threadIdx.x / a.lanes;
         const bool live = row < a.rows;
-        const T* xr = x + row * a.x_stride;
         float v[NV][VE];
         float sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (l + n * a.lanes) * VE;
+        for (int n = 0; n < NV; ++n) unpack<T, VE>(ahead[n], v[n]);
+        fetch(base + step);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) v[n][e] = 0.0f;
-            if (live && c < a.cols) load_vec<T, VE>(xr + c, v[n]);
+        for (int n = 0; n < NV; ++n)
 #pragma unroll
             for (int e = 0; e < VE; ++e) sum += v[n][e];
-        }
         const float mean = group_sum(sum, a.lanes, scratch) / (float)a.cols;
         float sq = 0.0f;
 #pragma unroll
@@ -150,13 +190,26 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
     const int64_t step = (int64_t)gridDim.x * per_block;
     float dw[NV][VE], db[NV][VE], w[NV][VE];
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int n = 0; n < NV; ++n) {
+        pr.load(pr.w, (l + n * a.lanes) * VE, a.cols, 1.0f, w[n]);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const int c = (l + n * a.lanes) * VE + e;
-            dw[n][e] = db[n][e] = 0.0f;
-            w[n][e] = c < a.cols ? (pr.w ? pr.at(pr.w, c) : 1.0f) : 0.0f;
+        for (int e = 0; e < VE; ++e) dw[n][e] = db[n][e] = 0.0f;
+    }
+    Raw<T, VE> ahead_x[NV], ahead_g[NV];
+    const auto fetch = [&](int64_t base) {
+        const int64_t row = base + threadIdx.x / a.lanes;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (l + n * a.lanes) * VE;
+            if (row < a.rows && c < a.cols) {
+                ahead_x[n] = *reinterpret_cast<const Raw<T, VE>*>(x + row * a.x_stride + c);
+                ahead_g[n] = *reinterpret_cast<const Raw<T, VE>*>(dy + row * dy_stride + c);
+            }
         }
+    };
+#pragma unroll
+    for (int n = 0; n < NV; ++n) ahead_x[n] = ahead_g[n] = Raw<T, VE>{};
+    fetch((int64_t)blockIdx.x * per_block);
     const float inv = 1.0f / (float)a.cols;
     for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows; base += step) {
         const int64_t row = base + threadIdx.x / a.lanes;
@@ -166,12 +219,13 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int c = (l + n * a.lanes) * VE;
+            unpack<T, VE>(ahead_x[n], v[n]);
+            unpack<T, VE>(ahead_g[n], g[n]);
+        }
+        fetch(base + step);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) v[n][e] = g[n][e] = 0.0f;
-            if (live && c < a.cols) {
-                load_vec<T, VE>(x + row * a.x_stride + c, v[n]);
-                load_vec<T, VE>(dy + row * dy_stride + c, g[n]);
+        for (int n = 0; n < NV; ++n) {
+            if (live && (l + n * a.lanes) * VE < a.cols) {
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
                     v[n][e] = (v[n][e] - mean) * rstd;
