@@ -607,26 +607,28 @@ struct StepArgs {
     bool whole;                     // rows of k, v and the caches are whole words at 4-byte boundaries
 };
 
-// A wave takes 64 / (lanes of a row) slots at a time; a lane keeps 16 bytes of the row for each of GB query heads.
-template <typename T, int DP, int GB>
+// A wave takes kUnroll times 64 / (lanes of a row) consecutive slots at a time; a lane keeps 16 bytes of the row for each of
+// GB query heads.  BUF: rows are whole words at 4-byte boundaries (a.whole).
+template <typename T, int DP, int GB, bool BUF>
 __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
-    constexpr int VE = Elem<T>::kPer16B, kLanes = DP / VE, kRows = 64 / kLanes, kUnroll = 4;
+    constexpr int VE = Elem<T>::kPer16B, kLanes = DP / VE, kRows = 64 / kLanes, kUnroll = 4, kTake = kRows * kUnroll;
+    static_assert(kTake <= 64, "row_buffer covers 64 rows");
     __shared__ float s_ml[kThreads / 64][GB][2];
     __shared__ float s_acc[kThreads / 64][GB][DP];
     const int split = blockIdx.x, hk = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, b = blockIdx.z;
     const int group = a.heads / a.kv_heads;
-    const int lane = lane_id(), wave = threadIdx.x >> 6, d = lane % kLanes * VE, r = lane / kLanes;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = lane % kLanes * VE, r = lane / kLanes;
     const int64_t pos = a.pos[b];
     const int slots = a.sinks + a.window;
     const int n = pos < 0 ? 0 : (int)(pos + 1 < slots ? pos + 1 : slots);
     const int own = pos < 0 ? -1 : (int)(pos < a.sinks ? pos : a.sinks + (pos - a.sinks) % a.window);
     const int per = (n + a.splits - 1) / a.splits;
     const int lo = split * per, hi = lo + per < n ? lo + per : n;
-    const T* kn = a.k.p + b * a.k.sb + hk * a.k.sh;
-    const T* vn = a.v.p + b * a.v.sb + hk * a.v.sh;
     T* ck = a.ck.p + b * a.ck.sb + hk * a.ck.sh;
     T* cv = a.cv.p + b * a.cv.sb + hk * a.cv.sh;
     const float l2scale = a.scale * kLog2e;
+    // the new row takes its slot's place here, whatever the slot holds: no block waits for the one that stores it
+    const u32x4 new_k = load_piece(a.k.p + b * a.k.sb + hk * a.k.sh, d, a.dim, BUF), new_v = load_piece(a.v.p + b * a.v.sb + hk * a.v.sh, d, a.dim, BUF);
     float q[GB][VE], acc[GB][VE], m[GB], sum[GB];
 #pragma unroll
     for (int x = 0; x < GB; ++x) {
@@ -640,36 +642,61 @@ __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
         m[x] = -INFINITY;
         sum[x] = 0.0f;
     }
-    for (int base = lo + wave * kRows; base < hi; base += kThreads / 64 * kRows * kUnroll) {
+    const int words = (a.dim - d) * (int)sizeof(T) / 4;              // of this lane's piece that are the row's
+    for (int base = lo + wave * kTake; base < hi; base += kThreads / 64 * kTake) {
         u32x4 kr[kUnroll], vr[kUnroll];
+        if constexpr (BUF) {
+            const auto kb = row_buffer(ck + (int64_t)base * a.ck.st, a.ck.st, hi - base < kTake ? hi - base : kTake, a.dim);
+            const auto vb = row_buffer(cv + (int64_t)base * a.cv.st, a.cv.st, hi - base < kTake ? hi - base : kTake, a.dim);
+            const int col = d < a.dim ? d * (int)sizeof(T) : 1 << 30;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int slot = base + u * (kThreads / 64) * kRows + r;
-            kr[u] = vr[u] = u32x4{0, 0, 0, 0};
-            if (slot < hi) {
-                const bool mine = slot == own;
-                kr[u] = load_piece(mine ? kn : ck + slot * a.ck.st, d, a.dim, a.whole);
-                vr[u] = load_piece(mine ? vn : cv + slot * a.cv.st, d, a.dim, a.whole);
-                if (mine && chunk == 0) {       // the slot is read from the new row above, by every chunk
-                    store_piece(ck + slot * a.ck.st, d, a.dim, kr[u], a.whole);
-                    store_piece(cv + slot * a.cv.st, d, a.dim, vr[u], a.whole);
+            for (int u = 0; u < kUnroll; ++u) kr[u] = load_piece(kb, (u * kRows + r) * (int)a.ck.st * (int)sizeof(T) + col);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) vr[u] = load_piece(vb, (u * kRows + r) * (int)a.cv.st * (int)sizeof(T) + col);
+            if (a.dim < DP) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        kr[u][i] = i < words ? kr[u][i] : 0u;
+                        vr[u][i] = i < words ? vr[u][i] : 0u;
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const int64_t slot = base + u * kRows + r;
+                kr[u] = vr[u] = u32x4{0, 0, 0, 0};
+                if (slot < hi) {
+                    kr[u] = load_piece(ck + slot * a.ck.st, d, a.dim, false);
+                    vr[u] = load_piece(cv + slot * a.cv.st, d, a.dim, false);
                 }
             }
+        }
+        if (own >= base && own < base + kTake) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (base + u * kRows + r == own) {
+                    kr[u] = new_k;
+                    vr[u] = new_v;
+                    if (chunk == 0 && own < hi) {
+                        store_piece(ck + (int64_t)own * a.ck.st, d, a.dim, new_k, BUF);
+                        store_piece(cv + (int64_t)own * a.cv.st, d, a.dim, new_v, BUF);
+                    }
+                }
         }
         float sc[kUnroll][GB];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             T kk[VE];
             __builtin_memcpy(kk, &kr[u], 16);
-            const bool live = base + u * (kThreads / 64) * kRows + r < hi;
+            const bool live = base + u * kRows + r < hi;
 #pragma unroll
             for (int x = 0; x < GB; ++x) {
                 float t = 0.0f;
 #pragma unroll
                 for (int e = 0; e < VE; ++e) t = fmaf(q[x][e], (float)kk[e], t);
-#pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) t += __shfl_xor(t, o);
-                sc[u][x] = live ? t : -INFINITY;
+                sc[u][x] = live ? lanes_sum(t, kLanes) : -INFINITY;
             }
         }
 #pragma unroll
@@ -751,8 +778,10 @@ __global__ __launch_bounds__(128) void window_step_join_kernel(StepArgs<T> a) {
     const float* p = a.parts + head * a.splits * (a.dim + 2);
     const int stride = a.dim + 2;
     float now = -INFINITY, total = 0.0f, value = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < a.splits; ++i) now = fmaxf(now, p[i * stride]);
     const float ref = now == -INFINITY ? 0.0f : now;
+#pragma unroll 8
     for (int i = 0; i < a.splits; ++i) {
         const float f = __builtin_amdgcn_exp2f(p[i * stride] - ref);
         total = fmaf(p[i * stride + 1], f, total);
@@ -1017,12 +1046,19 @@ int run_step(StepArgs<T> a, int64_t batch, hipStream_t st) {
     const dim3 grid(a.splits, a.kv_heads * a.chunks, (unsigned)batch), block(kThreads);
     for_dim(a.dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
+        const auto launch = [&](auto heads) {
+            constexpr int GB = decltype(heads)::value;
+            if (a.whole)
+                hipLaunchKernelGGL((window_step_kernel<T, DP, GB, true>), grid, block, 0, st, a);
+            else
+                hipLaunchKernelGGL((window_step_kernel<T, DP, GB, false>), grid, block, 0, st, a);
+        };
         if (gb == 4)
-            hipLaunchKernelGGL((window_step_kernel<T, DP, 4>), grid, block, 0, st, a);
+            launch(std::integral_constant<int, 4>{});
         else if (gb == 2)
-            hipLaunchKernelGGL((window_step_kernel<T, DP, 2>), grid, block, 0, st, a);
+            launch(std::integral_constant<int, 2>{});
         else
-            hipLaunchKernelGGL((window_step_kernel<T, DP, 1>), grid, block, 0, st, a);
+            launch(std::integral_constant<int, 1>{});
     });
     VAD_HIP_CHECK(hipGetLastError());
     if (a.splits > 1) {
