@@ -9,8 +9,8 @@
 // the backward walks starting from the gradient of the final state and ending at a times that of the initial state.
 //
 // Where sequences and heads alone do not fill the chip, a sequence is cut into spans walked by blocks of their own: a
-// first launch computes each span's state from k and v alone, a second one joins them along the sequence, and the
-// walk of every span starts from its joined state.
+// first launch computes each span's state from k and v alone, and the walk of every span starts from those before it --
+// added up by its block, or, where the spans are many, by a launch in between that goes along the sequence once.
 //
 // Wave w of a block owns columns 16 w .. 16 w + 15 of the state and of the outputs.  The state stays in float32; for
 // bfloat16 inputs its update multiplies v by the decay in float32 and splits the product into bfloat16 terms -- three, which
@@ -44,6 +44,7 @@ struct WalkArgs {
     const float* log_decay;
     float* spans;                      // [walk][seq][head][span][dim][dim]
     int n_seq, heads, dim, n_spans;
+    bool joined;                       // spans hold the states that they start from, not those that they leave
     bool whole;                        // all rows are whole words at 4-byte boundaries
 };
 
@@ -140,13 +141,31 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
             const int row = 16 * b + 4 * g + i;
             float x = 0.0f;
             if (!STATE && row < dim && col < dim) {
-                if (a.n_spans > 1)
+                if (a.joined)
                     x = spans[row * dim + col];
                 else if (w.s0)
                     x = w.s0[head * elems + (w.s0_transposed ? col * dim + row : row * dim + col)] * (w.reverse ? 1.0f : power(l2, 1.0f));
             }
             H[b][i] = x;
         }
+
+    if (!STATE && a.n_spans > 1 && !a.joined) {
+        const float keep = power(l2, (float)per);
+        const float* before = spans - (int64_t)span * elems;
+#pragma unroll 1
+        for (int u = 0; u < span; ++u, before += elems) {
+            f32x4 own[DP / 16];
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * b + 4 * g + i;
+                    own[b][i] = row < dim && col < dim ? before[row * dim + col] : 0.0f;
+                }
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) H[b] = H[b] * keep + own[b];
+        }
+    }
 
     const T* kp = head_ptr(w.k, a.seq, s, first, h);
     const T* vp = head_ptr(w.v, a.seq, s, first, h);
@@ -410,10 +429,14 @@ __global__ __launch_bounds__(256) void decay_step_kernel(Heads<const T> q, Heads
     if (t < 32 && oc < dim) o[head * dim + oc] = (T)(scale * ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])));
 }
 
-// Spans per sequence: enough blocks to fill the chip, spans of at least four pieces.
+constexpr int kJoinFrom = 8;
+
+// Spans per sequence.  A compute unit holds three walks of 64 columns, 768 in all.  512 walks and more go without spans
+// (24 ragged sequences of up to 2000 rows, 8 heads, trained, 1536 and 576 walks: 215 us; cut in two 231), fewer are cut into
+// 768 (4 x 16 heads of 8192 rows: 105 us; into 512 117, into 1536 115), of at least four pieces.
 int span_count(int64_t n_seq, int64_t max_len, int64_t heads, int walks) {
-    const int64_t blocks = n_seq * heads * walks, want = 768;
-    int64_t n = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    const int64_t blocks = n_seq * heads * walks;
+    int64_t n = blocks >= 512 ? 1 : (768 + blocks - 1) / blocks;
     const int64_t most = max_len / (4 * kPiece);
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n);
@@ -451,9 +474,11 @@ int run_walks(const WalkArgs<T>& a, int walks, hipStream_t st) {
     if (a.n_spans > 1) {
         launch_walk<T, true>(a, walks, st);
         VAD_HIP_CHECK(hipGetLastError());
-        const int64_t blocks = ((int64_t)a.dim * a.dim + 255) / 256 * a.n_seq * a.heads;
-        hipLaunchKernelGGL((decay_join_kernel<T>), dim3((unsigned)blocks, (unsigned)walks), dim3(256), 0, st, a);
-        VAD_HIP_CHECK(hipGetLastError());
+        if (a.joined) {
+            const int64_t blocks = ((int64_t)a.dim * a.dim + 255) / 256 * a.n_seq * a.heads;
+            hipLaunchKernelGGL((decay_join_kernel<T>), dim3((unsigned)blocks, (unsigned)walks), dim3(256), 0, st, a);
+            VAD_HIP_CHECK(hipGetLastError());
+        }
     }
     launch_walk<T, false>(a, walks, st);
     VAD_HIP_CHECK(hipGetLastError());
@@ -477,6 +502,7 @@ int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* 
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
+    a.joined = n_spans > kJoinFrom;
     a.whole = whole_words(a.walk[0].q, dim) && whole_words(a.walk[0].k, dim) && whole_words(a.walk[0].v, dim) && whole_words(a.walk[0].o, dim);
     return run_walks(a, 1, st);
 }
@@ -497,6 +523,7 @@ int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t*
     a.heads = heads;
     a.dim = dim;
     a.n_spans = n_spans;
+    a.joined = n_spans > kJoinFrom;
     a.whole = whole_words(Q, dim) && whole_words(K, dim) && whole_words(V, dim) && whole_words(G, dim);
     for (const Walk<T>& w : a.walk) a.whole = a.whole && whole_words(w.o, dim);
     return run_walks(a, 3, st);
