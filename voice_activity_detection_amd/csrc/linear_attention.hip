@@ -431,13 +431,14 @@ __global__ __launch_bounds__(256) void decay_step_kernel(Heads<const T> q, Heads
 
 constexpr int kJoinFrom = 8;
 
-// Spans per sequence.  A compute unit holds three walks of 64 columns, 768 in all.  512 walks and more go without spans
-// (24 ragged sequences of up to 2000 rows, 8 heads, trained, 1536 and 576 walks: 215 us; cut in two 231), fewer are cut into
-// 768 (4 x 16 heads of 8192 rows: 105 us; into 512 117, into 1536 115), of at least four pieces.
-int span_count(int64_t n_seq, int64_t max_len, int64_t heads, int walks) {
-    const int64_t blocks = n_seq * heads * walks;
-    int64_t n = blocks >= 512 ? 1 : (768 + blocks - 1) / blocks;
-    const int64_t most = max_len / (4 * kPiece);
+// Spans per sequence: none where the walks fill half of the chip, else as many as fill it -- a compute unit holds three
+// walks of up to 64 columns, two of more -- down to one piece each.  24 ragged sequences of up to 2000 rows, 8 heads, trained
+// (192 and 576 walks): 198 us, with the backward walks cut in two as well 231.  4 x 16 heads of 8192 rows: 104 us with 768
+// walks, 117 with 512, 115 with 1536.  One sequence of 300 rows and 8 heads: 16 us, with spans of four pieces and more 21.
+int span_count(int64_t n_seq, int64_t max_len, int64_t heads, int dim, int walks) {
+    const int64_t blocks = n_seq * heads * walks, fill = dim > 64 ? 512 : 768;
+    int64_t n = blocks >= 512 ? 1 : (fill + blocks - 1) / blocks;
+    const int64_t most = (max_len + kPiece - 1) / kPiece;
     if (n > most) n = most;
     return (int)(n < 1 ? 1 : n);
 }
@@ -567,7 +568,7 @@ int ensure_linear_attention_attrs() {
 extern "C" size_t vad_linear_attention_workspace_bytes(int64_t n_seq, int64_t max_len, int heads, int dim, int backward) {
     using namespace vad;
     if (n_seq <= 0 || max_len <= 0 || heads <= 0 || dim <= 0) return 0;
-    const int walks = backward ? 3 : 1, spans = span_count(n_seq, max_len, heads, walks);
+    const int walks = backward ? 3 : 1, spans = span_count(n_seq, max_len, heads, dim, walks);
     return spans > 1 ? (size_t)walks * n_seq * heads * spans * dim * dim * sizeof(float) : 0;
 }
 
@@ -590,7 +591,7 @@ extern "C" int vad_linear_attention_forward(const void* q_dev, const int64_t* q_
     VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
     rc = ensure_linear_attention_attrs();
     if (rc != VAD_OK) return rc;
-    const int spans = span_count(n_seq, max_len, heads, 1);
+    const int spans = span_count(n_seq, max_len, heads, dim, 1);
     const Sequences seq = {starts_dev, n_tokens, max_len};
     hipStream_t st = static_cast<hipStream_t>(stream);
     float* ws = static_cast<float*>(workspace_dev);
@@ -621,7 +622,7 @@ extern "C" int vad_linear_attention_backward(const void* q_dev, const int64_t* q
     VAD_REQUIRE(workspace_bytes >= need && (!need || workspace_dev), "workspace of %zu bytes is too small: %zu", workspace_bytes, need);
     rc = ensure_linear_attention_attrs();
     if (rc != VAD_OK) return rc;
-    const int spans = span_count(n_seq, max_len, heads, 3);
+    const int spans = span_count(n_seq, max_len, heads, dim, 3);
     const Sequences seq = {starts_dev, n_tokens, max_len};
     hipStream_t st = static_cast<hipStream_t>(stream);
     float* ws = static_cast<float*>(workspace_dev);
