@@ -63,24 +63,28 @@ struct TileShape {
     static constexpr size_t lds(int buffers) { return (size_t)buffers * (2 * kTileElems * sizeof(T) + kExtra * sizeof(float)) + 4 * sizeof(int); }
 };
 
-// Own rows first .. first + 64 NB - 1 of a head (zero from row `len` on) as fragments: by way of the block's two tiles.
+// Own rows first .. first + 64 NB - 1 of a head (zero from row `len` on) as fragments: requested early, then by way of the
+// block's first two tiles.
 template <typename T, int DP, int NB, int NT, bool BUF>
-__device__ __forceinline__ void load_own(Frag<T> (&f)[NB][DP / 32], const T* p, int64_t st, int first, int len, int dim, T* tiles) {
-    constexpr int kLd = TileShape<T, DP>::kLd;
-    const int wave = threadIdx.x >> 6;
-    Staged<T, DP, NT, BUF, kLd> r;
-    __syncthreads();
+struct Own {
+    static constexpr int kLd = TileShape<T, DP>::kLd;
+    Staged<T, DP, NT, BUF, kLd> r[NB];
+    __device__ __forceinline__ void fetch(const T* p, int64_t st, int first, int len, int dim) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        r.fetch(p, st, first + 64 * n, len - first - 64 * n, dim);
-        r.put(tiles + n * kTile * kLd, dim);
+        for (int n = 0; n < NB; ++n) r[n].fetch(p, st, first + 64 * n, len - first - 64 * n, dim);
     }
-    __syncthreads();
+    __device__ __forceinline__ void take(Frag<T> (&f)[NB][DP / 32], T* tiles, int dim) {
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+        for (int n = 0; n < NB; ++n) r[n].put(tiles + n * kTile * kLd, dim);
+        __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) f[nb][d] = frag_natural(tiles, kLd, 16 * (NB * wave + nb), 32 * d);
-}
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) f[nb][d] = frag_natural(tiles, kLd, 16 * (NB * wave + nb), 32 * d);
+    }
+};
 
 // acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
 // own row.
@@ -180,11 +184,24 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
         Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
         f32x4 acc[DP / 16][NB];
         float m[NB], sum[NB], delta[NB];
-        load_own<T, DP, NB, kThreads, BUF>(qf, qp, a.q.st, r0, len, dim, tiles);
+        const KeyTiles keys(r0, r1, a.window, a.sinks);
+        Staged<T, DP, kThreads, BUF, C::kLd> rk, rv;
+        const auto fetch = [&](int t) {
+            const int left = t < keys.end ? len - t : 0;       // no branch: no rows behind the last tile
+            rk.fetch(kp, a.k.st, t, left, dim);
+            rv.fetch(vp, a.v.st, t, left, dim);
+        };
+        Own<T, DP, NB, kThreads, BUF> own_q;
+        own_q.fetch(qp, a.q.st, r0, len, dim);
         if (BACK) {
+            Own<T, DP, NB, kThreads, BUF> own_g, own_o;
+            own_g.fetch(gp, a.go.st, r0, len, dim);
+            own_o.fetch(a.o + (row_base * a.heads + h) * dim, (int64_t)a.heads * dim, r0, len, dim);
+            fetch(keys.first());
             Frag<T> of[NB][DP / 32];
-            load_own<T, DP, NB, kThreads, BUF>(gf, gp, a.go.st, r0, len, dim, tiles);
-            load_own<T, DP, NB, kThreads, BUF>(of, a.o + (row_base * a.heads + h) * dim, (int64_t)a.heads * dim, r0, len, dim, tiles);
+            own_q.take(qf, tiles, dim);
+            own_g.take(gf, tiles, dim);
+            own_o.take(of, tiles, dim);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float x = 0.0f;
@@ -194,6 +211,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                     for (int j = 0; j < 8; ++j) x = fmaf((float)gf[nb][d][j], (float)of[nb][d][j], x);
                 delta[nb] = groups_sum(x);
             }
+        } else {
+            fetch(keys.first());
+            own_q.take(qf, tiles, dim);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -210,21 +230,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        const KeyTiles keys(r0, r1, a.window, a.sinks);
-        Staged<T, DP, kThreads, BUF, C::kLd> rk, rv;
-        const auto fetch = [&](int t) {
-            const int left = t < keys.end ? len - t : 0;       // no branch: no rows behind the last tile
-            rk.fetch(kp, a.k.st, t, left, dim);
-            rv.fetch(vp, a.v.st, t, left, dim);
-        };
         const auto is_edge = [&](int t) { return !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window); };
         const auto put = [&](int t, int to, int flag) {
             rk.put(tiles + 2 * to * C::kTileElems, dim);
             rv.put(tiles + (2 * to + 1) * C::kTileElems, dim);
             if (is_edge(t) && (BACK ? rk : rv).not_finite()) flags[flag] = 1;
         };
-        fetch(keys.first());
-        __syncthreads();                                       // the own rows' fragments and the last tiles are read
+        __syncthreads();                                       // the own rows' fragments are read
         if (C::kBuffers == 2) {
             put(keys.first(), buffer, turn);
             fetch(keys.next(keys.first()));
@@ -421,8 +433,9 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
         const int keys = SINKS ? (a.sinks < len ? a.sinks : len) : len;
         Frag<T> kf[NB][DP / 32], vf[NB][DP / 32];
         f32x4 dk[DP / 16][NB], dv[DP / 16][NB];
-        load_own<T, DP, NB, NT, BUF>(kf, kp, a.k.st, j0, keys, dim, tiles);
-        load_own<T, DP, NB, NT, BUF>(vf, vp, a.v.st, j0, keys, dim, tiles);
+        Own<T, DP, NB, NT, BUF> own_k, own_v;
+        own_k.fetch(kp, a.k.st, j0, keys, dim);
+        if (!SINKS) own_v.fetch(vp, a.v.st, j0, keys, dim);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -459,7 +472,10 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
             if (is_edge(row_of(step)) && (rq.not_finite() || rg.not_finite())) flags[flag] = 1;
         };
         if (!SINKS) fetch(0);
-        __syncthreads();                                       // the own rows' fragments and the last tiles are read
+        own_k.take(kf, tiles, dim);
+        if (SINKS) own_v.fetch(vp, a.v.st, j0, keys, dim);     // one wave stages whole tiles: one of them at a time in its registers
+        own_v.take(vf, tiles, dim);
+        __syncthreads();                                       // the own rows' fragments are read
         if (kBuffers == 2) {
             put(0, buffer, turn);
             fetch(1);
