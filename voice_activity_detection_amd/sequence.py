@@ -18,7 +18,7 @@ import math
 import operator
 
 import torch
-from torch._C import _cuda_getCurrentRawStream
+from torch._C import _cuda_getCurrentRawStream, _cuda_getDevice
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -43,7 +43,7 @@ def _strides(*s):
 
 def _call(fn, device, *args):
     """fn on the current stream of ``device`` (an index), with that device as the current one."""
-    if device == torch.cuda.current_device():
+    if device == _cuda_getDevice():
         rc = fn(*args, _cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -53,7 +53,7 @@ def _call(fn, device, *args):
 
 
 def _scratch(n, like):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _check_tensor(name, t, dtype=None, device=None):
@@ -122,6 +122,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _norm_forward(x, weight, bias, eps, False)[0]
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(n, cols):
+    return _lib.lib().vad_layer_norm_workspace_bytes(n, cols)
+
+
 def _as_rows(x):
     """(rows, cols) with dense columns: a view of x where its strides allow, else a copy."""
     if x.dim() == 2 and x.stride(1) == 1:
@@ -134,13 +139,13 @@ def _norm_forward(x, weight, bias, eps, keep):
     rows = _as_rows(x)
     n, cols = rows.shape
     y = x.new_empty(x.shape)
-    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+    stats = x.new_empty((n, 2), dtype=torch.float32) if keep else None
     wt = 0
     if weight is not None:
-        weight = weight.contiguous()
+        weight = weight if weight.is_contiguous() else weight.contiguous()
         wt = _DTYPES[weight.dtype]
     if bias is not None:
-        bias = bias.contiguous()
+        bias = bias if bias.is_contiguous() else bias.contiguous()
         wt = _DTYPES[bias.dtype]
     _call(_lib.lib().vad_layer_norm_forward, x.get_device(), rows.data_ptr(), n, cols, rows.stride(0), _ptr(weight), _ptr(bias),
           _DTYPES[x.dtype], wt, eps, y.data_ptr(), _ptr(stats))
@@ -159,17 +164,17 @@ class _LayerNorm(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows, dyr = _as_rows(x), _as_rows(dy)
         n, cols = rows.shape
         dx = x.new_empty(x.shape) if need_x else None
-        dw = torch.empty(cols, dtype=ctx.param, device=x.device) if need_w else None
-        db = torch.empty(cols, dtype=ctx.param, device=x.device) if need_b else None
-        L = _lib.lib()
-        size = L.vad_layer_norm_workspace_bytes(n, cols) if need_w or need_b else 0
+        dw = stats.new_empty(cols, dtype=ctx.param) if need_w else None
+        db = stats.new_empty(cols, dtype=ctx.param) if need_b else None
+        size = _norm_workspace(n, cols) if need_w or need_b else 0
         ws = _scratch(size, x)
-        weight = weight if weight is None else weight.contiguous()
-        _call(L.vad_layer_norm_backward, x.get_device(), rows.data_ptr(), dyr.data_ptr(), n, cols, rows.stride(0), dyr.stride(0),
+        if weight is not None and not weight.is_contiguous():
+            weight = weight.contiguous()
+        _call(_lib.lib().vad_layer_norm_backward, x.get_device(), rows.data_ptr(), dyr.data_ptr(), n, cols, rows.stride(0), dyr.stride(0),
               _ptr(weight), _DTYPES[x.dtype], 0 if ctx.param is None else _DTYPES[ctx.param], stats.data_ptr(), _ptr(dx), _ptr(dw),
               _ptr(db), _ptr(ws), size)
         return dx, dw, db, None
@@ -286,7 +291,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, starts=None, ma
 
 def _decay_forward(q, k, v, state, log_decay, starts, scale, lay):
     o = lay.output(q)
-    out = torch.empty(lay.state_shape, dtype=torch.float32, device=q.device)
+    out = q.new_empty(lay.state_shape, dtype=torch.float32)
     (q, qs), (k, ks), (v, vs) = lay.operand(q), lay.operand(k), lay.operand(v)
     state = state if state is None else state.contiguous()
     size = lay.decay_workspace[0]
@@ -403,7 +408,7 @@ def window_attention(q, k, v, window, sinks=0, scale=None, starts=None, max_len=
 
 def _window_forward(q, k, v, starts, window, sinks, scale, lay, keep):
     o = lay.output(q)
-    stats = torch.empty((lay.n_rows, lay.heads, 2), dtype=torch.float32, device=q.device) if keep else None
+    stats = q.new_empty((lay.n_rows, lay.heads, 2), dtype=torch.float32) if keep else None
     (q, qs), (k, ks), (v, vs) = lay.operand(q), lay.operand(k), lay.operand(v)
     _call(_lib.lib().vad_window_attention_forward, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(starts),
           *lay.sequences, lay.heads, lay.kv_heads, lay.dim, _DTYPES[q.dtype], window, sinks, scale, o.data_ptr(), _ptr(stats))
