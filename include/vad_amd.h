@@ -416,7 +416,8 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *   rows         q, k, v and the gradients of outputs are read through strides in ELEMENTS given on the host: {sequence,
  *                row, head} (steps: {batch, head}, caches: {batch, slot, head}); the head dimension is dense.  Any alignment
  *                works; rows of whole 4-byte words at 4-byte boundaries take wide loads.
- *                Row strides and dense rows (heads * dim) are below VAD_MAX_ROW_STRIDE.  Outputs are dense (rows, heads, dim).
+ *                Row strides (not those of caches) and dense rows (heads * dim) are below
+ *                VAD_MAX_ROW_STRIDE.  Outputs are dense (rows, heads, dim).
  *   sequences    starts_dev == NULL: n_seq sequences of max_len rows each.  Otherwise the rows of all sequences are packed
  *                behind one another in n_tokens rows and starts_dev holds n_seq + 1 ascending int64 on the device, sequence s
  *                being rows starts[s] .. starts[s+1] - 1 (empty ones allowed).  The table is NOT validated: entries are clamped

@@ -641,7 +641,7 @@ __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = lane % kLanes * VE, r = lane / kLanes;
     const int64_t pos = a.pos[b];
     const int slots = a.sinks + a.window;
-    const int n = pos < 0 ? 0 : (int)(pos + 1 < slots ? pos + 1 : slots);
+    const int n = pos < 0 ? 0 : (int)(pos < slots ? pos + 1 : slots);
     const int own = pos < 0 ? -1 : (int)(pos < a.sinks ? pos : a.sinks + (pos - a.sinks) % a.window);
     const int per = (n + a.splits - 1) / a.splits;
     const int lo = split * per, hi = lo + per < n ? lo + per : n;
@@ -1129,7 +1129,9 @@ extern "C" int vad_window_attention_step(const void* q_dev, const int64_t* q_str
         const int group = heads / kv_heads, gb = step_heads(group);
         a.chunks = (group + gb - 1) / gb;
         a.splits = step_splits(batch, kv_heads, a.chunks, sinks + window);
-        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim);
+        // (a cache may be laid out with any slot stride: row_buffer takes those below VAD_MAX_ROW_STRIDE)
+        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim) &&
+                  a.ck.st < VAD_MAX_ROW_STRIDE && a.cv.st < VAD_MAX_ROW_STRIDE;
         return run_step<T>(a, batch, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
