@@ -423,6 +423,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *                being rows starts[s] .. starts[s+1] - 1 (empty ones allowed).  The table is NOT validated: entries are clamped
  *                into 0 .. n_tokens.  Output rows before the first and behind the last sequence are set to zero.  max_len is
  *                then a hint that sizes the launch; longer sequences are still computed in full.
+ *                At most 2^30 rows, fewer than 2^22 pairs of sequence (of a batch) and head, 65535 sequences for windows.
  *   masked rows  what lies outside a row's mask -- later rows, rows beyond the window, unfilled cache slots, rows of no
  *                sequence -- has no influence on it, also where it holds infinities or NaN.
  *   repeatability  no atomics: the same call gives the same bits.
@@ -481,7 +482,8 @@ int vad_linear_attention_step(const void* q_dev, const int64_t* q_strides, const
 /*
  * Attention with a sliding window and sinks: row i sees key j when j <= i and (i - j < window or j < sinks);
  * o_i = softmax over the visible keys of (scale q_i . k_j) v_j.  heads query heads share kv_heads key heads: query head h
- * reads key head h / (heads / kv_heads).  sinks <= VAD_MAX_SINKS, scale > 0, at most 2^30 rows.
+ * reads key head h / (heads / kv_heads).  sinks <= VAD_MAX_SINKS, scale > 0,
+ * window <= 2^30.
  *   stats_dev       (rows, heads, 2) float32 softmax statistics for the backward pass; may be NULL in the forward call
  * Backward: o_dev the forward call's output; dk_dev / dv_dev (rows, kv_heads, dim).
  * workspace_dev: vad_window_attention_workspace_bytes(..., n_rows = rows of q, ...).

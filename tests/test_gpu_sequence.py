@@ -581,6 +581,141 @@ def test_offsets_past_32_bits(vad):
     assert torch.equal(far_o, vad.window_attention_step(qq, kk, kk, ka, ka.clone(), pos, 70)) and torch.equal(near, ka)
 
 
+def test_hints_windows_and_strides_at_their_ends(vad):
+    """A hint shorter than the sequences, a window longer than any, one key head for all, expanded rows, rows far apart."""
+    g = _gen(51)
+    q, k, v, do = (_rand(g, 700, 3, 40) for _ in range(4))
+    starts = torch.tensor([0, 600, 700], device='cuda')
+    log_decay = _decays(3)
+
+    def run(q, k, v, **hint):
+        leaf = [t.detach().requires_grad_() for t in (q, k, v)]
+        o, s = vad.linear_attention(*leaf, log_decay, starts=starts, **hint)
+        outs = [o, s, *torch.autograd.grad(o, leaf, do)]
+        for window, sinks in ((90, 5), (1 << 30, 0), (1 << 30, 64), (1, 0), (1, 17)):
+            w = vad.window_attention(*leaf, window, sinks, starts=starts, **hint)
+            outs += [w, *torch.autograd.grad(w, leaf, do)]
+        return outs
+
+    want = run(q, k, v)
+    for hint in (0, 1, 65, 600, 10 ** 12):
+        for a, b in zip(run(q, k, v, max_len=hint), want):
+            assert torch.allclose(a, b, rtol=1e-4, atol=1e-4)
+    # every window of a whole sequence and more is the same causal attention, sinks or not
+    for a, b in zip(want[9:13], want[13:17]):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-4)
+    # a window of one row without sinks answers with that row's value.  Its weight p is 2 to the rounding error of s - max, not 1
+    # to the bit, so the answer is (p v) (1 / p): half a unit for either product, a whole one for the reciprocal, 2^-24 (1 + 1 + 2)
+    assert ((want[17] - v).abs() <= 2.0 ** -22 * v.abs()).all()
+    # keys and values expanded over heads (stride 0): the gradient of the shared head is the heads' sum
+    one = _rand(g, 700, 1, 40).requires_grad_()
+    wide = one.detach().expand(700, 3, 40).clone().requires_grad_()
+    a = torch.autograd.grad(vad.window_attention(q, one.expand(700, 3, 40), one.expand(700, 3, 40), 90, 5, starts=starts), one, do)[0]
+    b = torch.autograd.grad(vad.window_attention(q, wide, wide, 90, 5, starts=starts), wide, do)[0]
+    c = torch.autograd.grad(vad.window_attention(q, one, one, 90, 5, starts=starts), one, do)[0]
+    assert torch.allclose(a, b.sum(1, keepdim=True), rtol=1e-4, atol=1e-4) and torch.allclose(a, c, rtol=1e-4, atol=1e-4)
+    # one row for all rows
+    row = _rand(g, 1, 3, 40).expand(700, 3, 40)
+    for x, y in zip(run(row, row, row), run(*[row.contiguous()] * 3)):
+        assert torch.equal(x, y)
+    assert torch.equal(vad.layer_norm(row), vad.layer_norm(row.contiguous()))
+    # rows farther apart than a kernel's offsets reach are brought together first
+    far = torch.empty(4, 1 << 22, device='cuda').as_strided((1, 4, 3, 40), (0, 1 << 22, 40, 1))
+    far.copy_(q[None, :4])
+    assert torch.equal(vad.window_attention(far, far, far, 2), vad.window_attention(*[q[None, :4]] * 3, 2))
+    assert torch.equal(vad.linear_attention(far, far, far, log_decay)[0], vad.linear_attention(*[q[None, :4]] * 3, log_decay)[0])
+    empty = torch.empty(0, 40, device='cuda', requires_grad=True)
+    w, b = torch.ones(40, device='cuda', requires_grad=True), torch.zeros(40, device='cuda', requires_grad=True)
+    assert all(not t.any() for t in torch.autograd.grad(vad.layer_norm(empty, w, b).sum(), (w, b)))
+
+
+def test_many_short_sequences(vad):
+    """65535 sequences of 0 .. 2 rows without a hint: more tiles than a launch holds."""
+    n = 65535
+    lengths = torch.arange(n) % 3
+    starts = torch.cat((torch.zeros(1, dtype=torch.int64), lengths.cumsum(0))).cuda()
+    rows = int(starts[-1])
+    g = _gen(61)
+    q, k, v, do = (_rand(g, rows, 2, 4) for _ in range(4))
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    o = vad.window_attention(*leaf, 7, 1, starts=starts)
+    grads = torch.autograd.grad(o, leaf, do)
+    first = (starts[:-1][lengths.cuda() > 0])
+    assert torch.allclose(o[first], v[first], rtol=1e-6, atol=1e-6)
+    pairs = first[1::2]                                     # sequences of two rows
+    sc = (q[pairs + 1][:, None] * torch.stack((k[pairs], k[pairs + 1]), 1)).sum(-1, keepdim=True) / 2
+    want = (torch.softmax(sc, 1) * torch.stack((v[pairs], v[pairs + 1]), 1)).sum(1)
+    assert torch.allclose(o[pairs + 1], want, rtol=1e-5, atol=1e-5)
+    short = torch.tensor([0, 0, 1, 3], device='cuda')
+    cut = [t.detach()[:3].clone().requires_grad_() for t in (q, k, v)]
+    cut_grads = torch.autograd.grad(vad.window_attention(*cut, 7, 1, starts=short), cut, do[:3])
+    assert all(torch.allclose(a[:3], b, rtol=1e-5, atol=1e-5) for a, b in zip(grads, cut_grads))
+    o, s = vad.linear_attention(*leaf, _decays(2), starts=starts)
+    assert torch.allclose(s[1], k[0][:, :, None] * v[0][:, None, :], rtol=1e-6, atol=1e-6) and not s[0].any()
+    with pytest.raises(vad.VadError, match='sequence count'):
+        vad.window_attention(*[torch.zeros(1, 2, 4, device='cuda')] * 3, 7, starts=torch.zeros(65537, dtype=torch.int64, device='cuda'))
+
+
+def test_in_place_updates_are_seen_by_autograd(vad):
+    """A state or cache that a graph has saved and a step has overwritten since: an error, not a wrong gradient."""
+    g = _gen(71)
+    x = _rand(g, 1, 5, 2, 8).requires_grad_()
+    row = x.detach()[:, 0]
+    log_decay = _decays(2)
+    state = torch.zeros(1, 2, 8, 8, device='cuda')
+    o, _ = vad.linear_attention(x, x, x, log_decay, state=state)
+    vad.linear_attention_step(row, row, row, log_decay, state)
+    with pytest.raises(RuntimeError, match='inplace'):
+        o.sum().backward()
+    ck, cv = (_rand(g, 1, 5, 2, 8) for _ in range(2))
+    pos = torch.tensor([9], device='cuda')
+    for write in (lambda: vad.window_attention_step(row, row, row, ck, cv, pos, 4, 1),
+                  lambda: vad.window_cache_fill(x.detach(), x.detach(), ck, cv, 4, 1)):
+        o = vad.window_attention(x, ck, cv, 4, 1)
+        write()
+        with pytest.raises(RuntimeError, match='inplace'):
+            o.sum().backward()
+    with torch.inference_mode():
+        s, c, d = (torch.zeros(*n, device='cuda') for n in ((1, 2, 8, 8), (1, 5, 2, 8), (1, 5, 2, 8)))
+        vad.linear_attention_step(row, row, row, log_decay, s)
+        vad.window_attention_step(row, row, row, c, d, vad.window_cache_fill(x, x, c, d, 4, 1), 4, 1)
+        assert s.any() and c.any()
+
+
+def test_two_streams_at_once(vad):
+    """The same calls on two streams at the same time, each with its own tensors and scratch memory."""
+    def work(seed):
+        g = _gen(seed)
+        q, k, v, do = (_rand(g, 4000, 4, 64, dtype=torch.bfloat16) for _ in range(4))
+        leaf = [t.requires_grad_() for t in (q, k, v)]
+        log_decay = _decays(4)
+        cache = torch.zeros(2, 1, 4016, 4, 64, dtype=torch.bfloat16, device='cuda')
+
+        def run():
+            o, s = vad.linear_attention(*leaf, log_decay, starts=starts)
+            w = vad.window_attention(*leaf, 200, 16, starts=starts)
+            grads = (*torch.autograd.grad(o, leaf, do), *torch.autograd.grad(w, leaf, do))
+            with torch.no_grad():
+                pos = vad.window_cache_fill(k[None], v[None], cache[0], cache[1], 4000, 16)
+                step = vad.window_attention_step(q[:1], k[:1], v[:1], cache[0], cache[1], pos, 4000, 16)
+            return [o, s, w, *grads, step]
+        return run
+
+    starts = torch.tensor([0, 3000, 4000], device='cuda')
+    runs = [work(81), work(82)]
+    want = [[t.clone() for t in run()] for run in runs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for run, stream in zip(runs, streams):
+            with torch.cuda.stream(stream):
+                got.append(run())
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_nothing_is_written_behind_a_head(vad):
     """Caches, states and outputs of head sizes that end inside a 16-byte piece, between guard values."""
     g = _gen(41)
@@ -689,6 +824,8 @@ def test_device_refusals(vad):
         (lambda: vad.window_attention_step(q[0], q[0], q[0], *[torch.zeros(10, 5, 4, 32, device='cuda')] * 2, torch.zeros(10, dtype=torch.int64, device='cuda'), 5, 1), 'cache_k'),
         (lambda: vad.window_attention_step(q[0], q[0], q[0], torch.zeros(10, 6, 4, 32, device='cuda'), torch.zeros(1, 6, 4, 32, device='cuda').expand(10, 6, 4, 32),
                                            torch.zeros(10, dtype=torch.int64, device='cuda'), 5, 1), 'broadcast'),
+        (lambda: vad.window_cache_fill(q, q, *[torch.zeros(1, 6, 4, 32, device='cuda')] * 2, 5, 1), 'same memory'),
+        (lambda: vad.window_cache_fill(q.clone().requires_grad_(), q, *[torch.zeros(1, 6, 4, 32, device='cuda') for _ in range(2)], 5, 1), 'no gradient'),
     ]
     for call, needle in bad:
         with pytest.raises(ValueError, match=needle):

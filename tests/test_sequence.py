@@ -68,6 +68,11 @@ def test_c_entry_points_refuse_before_any_device_work(L):
         ('vad_window_attention_forward', win(max_len=1 << 31), b'length'),
         ('vad_window_attention_forward', win(o=None), b'null pointer'),
         ('vad_window_attention_backward', (*hd, ok, ok, s3, ok, None, 1, 0, 4, 2, 1, 4, 0, 3, 0, 1.0, ok, ok, ok, ok, 8, None), b'too small'),
+        ('vad_window_attention_forward', win(n_seq=60000, heads=60000, kv=60000), b'too many'),
+        ('vad_linear_attention_forward', fwd(t=(ok, s3, ok, _strides(1, 1 << 22, 1), ok, s3)), b'row stride'),
+        ('vad_linear_attention_forward', fwd(heads=1 << 20, dim=8), b'rows of'),
+        ('vad_linear_attention_forward', fwd(max_len=1 << 31), b'length'),
+        ('vad_linear_attention_step', (ok, s2, ok, s2, ok, s2, 1 << 21, 2, 4, 0, ok, 1.0, ok, ok, None), b'too many'),
         ('vad_window_attention_step', step(dtype=-1), b'dtype'),
         ('vad_window_attention_step', step(pos=None), b'null pointer'),
         ('vad_window_attention_step', step(window=100000), b'too small'),

@@ -535,7 +535,9 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(dim >= 1 && dim <= VAD_MAX_HEAD_DIM, "head dimension %d out of range 1..%d", dim, VAD_MAX_HEAD_DIM);
     VAD_REQUIRE(heads >= 1, "heads must be positive, got %d", heads);
     VAD_REQUIRE(n_seq >= 0 && n_tokens >= 0 && max_len >= 0, "negative sequence count or length");
-    VAD_REQUIRE(n_seq <= 0x7FFFFFFF / heads / 64, "too many sequences for one launch");
+    VAD_REQUIRE(n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
+    // a step launches up to four blocks of 256 threads for each, and a launch's threads are counted in 32 bits
+    VAD_REQUIRE(n_seq < (1 << 22) / heads, "too many sequences for one launch");
     VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
     return VAD_OK;
 }

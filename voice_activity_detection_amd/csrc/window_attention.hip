@@ -843,6 +843,8 @@ Heads<const T> heads_of(const void* p, const int64_t* s) {
     return {static_cast<const T*>(p), s[0], s[1], s[2]};
 }
 
+constexpr int64_t kMostBlocks = ((int64_t)1 << 32) / kThreads - 1;
+
 template <typename F>
 void for_dim(int dim, F f) {
     if (dim <= 32)
@@ -853,9 +855,11 @@ void for_dim(int dim, F f) {
         f(std::integral_constant<int, 128>{});
 }
 
-unsigned row_tiles(int64_t max_len, int rows) {
-    const int64_t n = (max_len + rows - 1) / rows;
-    return (unsigned)(n < 1 ? 1 : n);
+// Blocks per head and sequence: one per tile of own rows, fewer (each then takes several) where a launch, whose threads are
+// counted in 32 bits, could not hold them.
+unsigned row_tiles(int64_t max_len, int rows, int64_t heads) {
+    const int64_t n = (max_len + rows - 1) / rows, most = kMostBlocks / heads;
+    return (unsigned)(n < 1 ? 1 : (n < most ? n : most));
 }
 
 template <typename T, int DP, bool BUF>
@@ -867,12 +871,12 @@ struct Kernels {
     static constexpr int NB = DP == 128 && sizeof(T) == 2 ? 2 : 1, NK = 1;
     static constexpr size_t kLds = TileShape<T, DP>::lds(TileShape<T, DP>::kBuffers), kLdsSinks = TileShape<T, DP>::lds(1);
     static void forward(WindowArgs<T> a, hipStream_t st) {
-        a.tiles = row_tiles(a.seq.max_len, 64 * NB);
+        a.tiles = row_tiles(a.seq.max_len, 64 * NB, (int64_t)a.heads * a.n_seq);
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(a.tiles * a.heads * a.n_seq), dim3(kThreads), kLds, st, a);
     }
     static void backward(WindowArgs<T> a, hipStream_t st) {
         const dim3 block(kThreads);
-        a.tiles = row_tiles(a.seq.max_len, 64 * NK);
+        a.tiles = row_tiles(a.seq.max_len, 64 * NK, (int64_t)a.heads * a.n_seq);
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NK, true, BUF>), dim3(a.tiles * a.heads * a.n_seq), block, kLds, st, a);
         hipLaunchKernelGGL((window_keys_kernel<T, DP, NK, false, BUF>), dim3(a.tiles * a.kv_heads * a.n_seq), block, kLds, st, a);
         if (a.sinks > 0) {
@@ -932,7 +936,7 @@ int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int
     VAD_REQUIRE(sinks >= 0 && sinks <= VAD_MAX_SINKS, "sinks %d out of range 0..%d", sinks, VAD_MAX_SINKS);
     VAD_REQUIRE(n_seq >= 0 && n_seq <= 65535, "sequence count %lld out of range 0..65535", (long long)n_seq);
     VAD_REQUIRE(n_tokens >= 0 && max_len >= 0 && n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
-    VAD_REQUIRE((max_len / 64 + 1) * heads * n_seq <= 0x7FFFFFFF, "too many rows for one launch");
+    VAD_REQUIRE(n_seq * heads <= kMostBlocks / 2, "too many sequences for one launch");
     VAD_REQUIRE((int64_t)heads * dim < VAD_MAX_ROW_STRIDE, "rows of %lld elements are too long", (long long)heads * dim);
     return VAD_OK;
 }

@@ -52,6 +52,11 @@ def _call(fn, device, *args):
         _lib.check(rc)
 
 
+def _written(*tensors):
+    """Tensors that a call updates in place: a graph that saved one of them then refuses its backward pass."""
+    torch._C._increment_version(tensors)
+
+
 def _scratch(n, like):
     return like.new_empty(n, dtype=torch.uint8) if n else None
 
@@ -375,6 +380,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None):
     q, qs, k, ks, v, vs = _step_operands(q, k, v)
     _call(_lib.lib().vad_linear_attention_step, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, batch, heads, dim,
           _DTYPES[q.dtype], log_decay.data_ptr(), scale, state.data_ptr(), o.data_ptr())
+    _written(state)
     return o
 
 
@@ -450,6 +456,11 @@ def _cache_table(name, shape, stride, batch, slots, kv_heads, dim):
     return _strides(*stride[:3])
 
 
+def _check_apart(k, v):
+    if k.data_ptr() == v.data_ptr() and k.numel():
+        raise ValueError('cache_k and cache_v are the same memory')
+
+
 def _check_cache(name, c, like, batch, slots, kv_heads, dim):
     if type(c) is not torch.Tensor or c.dtype is not like.dtype or c.get_device() != like.get_device():
         _check_tensor(name, c, like.dtype, like.device)
@@ -478,6 +489,7 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, window, sinks=0, scale
     _check_tensor('pos', pos, torch.int64, q.device)
     if pos.dim() != 1 or pos.size(0) != batch or not pos.is_contiguous():
         raise ValueError('pos must be a contiguous tensor of shape (%d,), got %s' % (batch, tuple(pos.shape)))
+    _check_apart(cache_k, cache_v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or cache_k.requires_grad or cache_v.requires_grad):
         raise ValueError('window_attention_step has no gradient: call it under torch.no_grad(), or use window_attention')
     o = q.new_empty(q.shape)
@@ -487,19 +499,24 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, window, sinks=0, scale
     _call(_lib.lib().vad_window_attention_step, q.get_device(), q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, cache_k.data_ptr(),
           cks, cache_v.data_ptr(), cvs, pos.data_ptr(), batch, heads, kv_heads, dim, _DTYPES[q.dtype], window, sinks, scale, o.data_ptr(),
           _ptr(ws), size)
+    _written(cache_k, cache_v)
     return o
 
 
 def window_cache_fill(k, v, cache_k, cache_v, window, sinks=0, starts=None):
     """Keys and values of whole sequences into rolling caches, as the steps after them expect it: (batch, length, kv_heads,
     dim), or packed with ``starts``.  Slots that no row belongs to stay as they are.  Returns ``pos`` (batch,) int64: the
-    lengths."""
+    lengths.  Inference only."""
     lay = _layout(k, k, v, starts, None, True)
     window, sinks, _ = _check_window(window, sinks, None, lay.dim)
     cks = _check_cache('cache_k', cache_k, k, lay.n_seq, sinks + window, lay.heads, lay.dim)
     cvs = _check_cache('cache_v', cache_v, k, lay.n_seq, sinks + window, lay.heads, lay.dim)
+    _check_apart(cache_k, cache_v)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or cache_k.requires_grad or cache_v.requires_grad):
+        raise ValueError('window_cache_fill has no gradient: call it under torch.no_grad()')
     pos = torch.empty(lay.n_seq, dtype=torch.int64, device=k.device)
     (k, ks), (v, vs) = lay.operand(k), lay.operand(v)
     _call(_lib.lib().vad_window_cache_fill, k.get_device(), k.data_ptr(), ks, v.data_ptr(), vs, _ptr(starts), *lay.sequences, lay.heads,
           lay.dim, _DTYPES[k.dtype], window, sinks, cache_k.data_ptr(), cks, cache_v.data_ptr(), cvs, pos.data_ptr())
+    _written(cache_k, cache_v)
     return pos
