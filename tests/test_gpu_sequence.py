@@ -283,6 +283,22 @@ def test_window_attention(vad, dtype, lengths, heads, kv_heads, dim, window, sin
     assert all(torch.equal(a, b) for a, b in zip(grads, grads2))
 
 
+@pytest.mark.parametrize('length,dim,window,sinks', [(200, 64, 2, 0), (200, 30, 4, 1), (150, 128, 3, 0), (300, 64, 100, 4), (300, 16, 300, 0)])
+def test_window_attention_gradients_keep_bfloat16(vad, length, dim, window, sinks):
+    """Each result takes two roundings to bfloat16 -- of the weights (P or dS), of itself -- and nothing else that counts.  A
+    rounding is off by up to 2^-8, evenly spread: 2^-8 / sqrt(3) in the mean square, two of them sqrt(2 / 3) 2^-8."""
+    g = _gen(91)
+    q, k, v, do = (_rand(g, 1, length, 2, dim, dtype=torch.bfloat16) for _ in range(4))
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    o = vad.window_attention(*leaf, window, sinks)
+    got = (o, *torch.autograd.grad(o, leaf, do))
+    for h in range(2):
+        exact = [t.detach()[0, :, h].double().requires_grad_() for t in (q, k, v)]
+        want = ref.window_sequence(*exact, window, sinks, dim ** -0.5)['o']
+        for a, b in zip(got, (want, *torch.autograd.grad(want, exact, do[0, :, h].double()))):
+            assert float((a.detach()[0, :, h].double() - b.detach()).norm()) <= (2 / 3) ** 0.5 * 2.0 ** -8 * float(b.detach().norm())
+
+
 def test_window_attention_gradients_against_differences(vad):
     g = _gen(4)
     q = _rand(g, 1, 150, 4, 30)

@@ -281,14 +281,15 @@ struct Staged {
     }
 };
 
-// A tile's infinities and NaN become zero: every thread of the block cleans the pieces that it staged.
+// The infinities and NaN in a tile's first `rows` rows become zero: every thread of the block cleans pieces of it.
 template <typename T, int DP, int NT, int PITCH>
-__device__ __forceinline__ void clean_tile(T* tile) {
+__device__ __forceinline__ void clean_tile(T* tile, int rows) {
     using S = Staged<T, DP, NT, true, PITCH>;
     const int row0 = threadIdx.x / S::kPPR, c = threadIdx.x % S::kPPR * S::kPer;
 #pragma unroll 1
     for (int n = 0; n < S::kPieces; ++n) {
         T* p = tile + (row0 + n * S::kStep) * S::kLd + c;
+        if (row0 + n * S::kStep >= rows) break;
 #pragma unroll
         for (int e = 0; e < S::kPer; ++e)
             if (!(fabsf((float)p[e]) < INFINITY)) p[e] = (T)0.0f;

@@ -86,12 +86,12 @@ struct Own {
     }
 };
 
-// acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of the 64 streamed rows for this lane's
+// acc (columns of the tile down, own rows along the lanes) += tile^T p, p the weights of 16 KB streamed rows for this lane's
 // own row.
-template <typename T, int DP, int NB>
-__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB], f32x4 (&acc)[DP / 16][NB]) {
+template <typename T, int DP, int NB, int KB>
+__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[KB][NB], f32x4 (&acc)[DP / 16][NB]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < KB / 2; ++t) {
         Frag<T> f[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
@@ -100,6 +100,30 @@ __device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[4][NB
             const Frag<T> x = frag_columns(tile, TileShape<T, DP>::kLd, 32 * t, 16 * b);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) acc[b][nb] = mma(x, f[nb], acc[b][nb]);
+        }
+    }
+}
+
+// The same for two sets of weights, each piece of the tile read once.
+template <typename T, int DP, int NB, int KB>
+__device__ __forceinline__ void accumulate(const T* tile, const f32x4 (&p)[KB][NB], f32x4 (&acc)[DP / 16][NB], const f32x4 (&p2)[KB][NB],
+                                           f32x4 (&acc2)[DP / 16][NB]) {
+#pragma unroll
+    for (int t = 0; t < KB / 2; ++t) {
+        Frag<T> f[NB], f2[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            to_frag(p[2 * t][nb], p[2 * t + 1][nb], f[nb]);
+            to_frag(p2[2 * t][nb], p2[2 * t + 1][nb], f2[nb]);
+        }
+#pragma unroll
+        for (int b = 0; b < DP / 16; ++b) {
+            const Frag<T> x = frag_columns(tile, TileShape<T, DP>::kLd, 32 * t, 16 * b);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                acc[b][nb] = mma(x, f[nb], acc[b][nb]);
+                acc2[b][nb] = mma(x, f2[nb], acc2[b][nb]);
+            }
         }
     }
 }
@@ -116,11 +140,11 @@ __device__ __forceinline__ float not_finite_sum(const T* p, int64_t st, int64_t 
     return sum;
 }
 
-// s = tile own^T for the 64 streamed rows
-template <typename T, int DP, int NB>
-__device__ __forceinline__ void scores(const T* tile, const Frag<T> (&own)[NB][DP / 32], f32x4 (&s)[4][NB]) {
+// s = tile own^T for 16 KB streamed rows
+template <typename T, int DP, int NB, int KB>
+__device__ __forceinline__ void scores(const T* tile, const Frag<T> (&own)[NB][DP / 32], f32x4 (&s)[KB][NB]) {
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
+    for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) s[kb][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -173,6 +197,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
     const int64_t row_base = a.seq.starts ? first : (int64_t)s * a.seq.max_len;
     const float l2scale = a.scale * kLog2e;
     constexpr int kRows = 64 * NB;
+    // delta of bfloat16 outputs is off by their rounding and that of the weights behind them, 2^-8 of dO O, which is not small
+    // beside dP - delta where few keys share a row.  The sum of a row's dS tells by how much, and dQ is off by that times the
+    // mean key: one more product, 50 -> 62 us on 24 ragged sequences of up to 2000 rows (8 heads of 64, window 300), for gradients
+    // at 2^-8.7 of the exact ones in place of 2^-7.8 (window 2) and 2^-8.5 (window 300).
+    constexpr bool kRefine = BACK && sizeof(T) == 2;
+    // with 128 columns half a tile's scores at a time, or registers run out: 463 -> 420 us on 2 x 16 heads of 8192 rows, window 1000
+    // (64 columns: 456 -> 466 us on twice the sequences, 32: 274 -> 289)
+    constexpr int kHalves = kRefine && DP == 128 ? 2 : 1, kPart = kTile / kHalves;
     zero_outside(a.out, (int64_t)a.heads * dim, h * dim, dim, a.seq, s, a.n_seq, part, a.tiles);
     // flags[turn]: the tile in hand holds infinities or NaN; the next tile's is set and the last one's cleared meanwhile
     if (threadIdx.x < 3) flags[threadIdx.x] = 0;
@@ -182,8 +214,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
         const int r0 = (int)r0_64, r1 = (len - r0 < kRows ? len - r0 : kRows) + r0 - 1;
         const int w0 = r0 + 16 * NB * wave, w1 = w0 + 16 * NB - 1;
         Frag<T> qf[NB][DP / 32], gf[NB][DP / 32];
-        f32x4 acc[DP / 16][NB];
-        float m[NB], sum[NB], delta[NB];
+        f32x4 acc[DP / 16][NB], mean[DP / 16][NB];
+        float m[NB], sum[NB], delta[NB], off[NB];
         const KeyTiles keys(r0, r1, a.window, a.sinks);
         Staged<T, DP, kThreads, BUF, C::kLd> rk, rv;
         const auto fetch = [&](int t) {
@@ -225,10 +257,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 const int64_t at = (row_base + row) * a.heads + h;
                 m[nb] = live ? a.stats[2 * at] : 0.0f;
                 sum[nb] = live ? a.stats[2 * at + 1] : 0.0f;
-                if (live && g == 0) a.delta[at] = delta[nb];
             }
+            off[nb] = 0.0f;
 #pragma unroll
-            for (int b = 0; b < DP / 16; ++b) acc[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int b = 0; b < DP / 16; ++b) acc[b][nb] = mean[b][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const auto is_edge = [&](int t) { return !(t + kTile - 1 <= r0 && r0 + kRows - 1 - t < a.window); };
         const auto put = [&](int t, int to, int flag) {
@@ -259,17 +291,21 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             const auto step = [&](auto edge) {
             constexpr bool EDGE = decltype(edge)::value;
             const bool active = !EDGE || (t <= w1 && (w0 - (t + kTile - 1) < a.window || t < a.sinks));      // for this wave
-            f32x4 p[4][NB], dp[4][NB];
+#pragma unroll 1
+            for (int half = 0; half < kHalves; ++half) {
+            T* pk = sk + half * kPart * C::kLd;
+            T* pv = sv + half * kPart * C::kLd;
+            f32x4 p[kPart / 16][NB], dp[kPart / 16][NB];
             if (active) {
                 // products ahead of the other waves' softmax: 258 -> 248 us at 128 columns
                 __builtin_amdgcn_s_setprio(1);
-                scores<T, DP, NB>(sk, qf, p);
-                if (BACK) scores<T, DP, NB>(sv, gf, dp);
+                scores<T, DP, NB>(pk, qf, p);
+                if (BACK) scores<T, DP, NB>(pv, gf, dp);
                 __builtin_amdgcn_s_setprio(0);
             }
             if (EDGE && flags[turn]) {
                 __syncthreads();
-                clean_tile<T, DP, kThreads, C::kLd>(BACK ? sk : sv);
+                clean_tile<T, DP, kThreads, C::kLd>(BACK ? pk : pv, kPart);
                 __syncthreads();
                 met = true;
             }
@@ -277,12 +313,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             const bool masked = EDGE && !(t + kTile - 1 <= w0 && w1 - t < a.window);
             if (masked) {
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
+                for (int kb = 0; kb < kPart / 16; ++kb)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int j = t + 16 * kb + 4 * g + i, gap = w0 + 16 * nb + c - j;
+                            const int j = t + half * kPart + 16 * kb + 4 * g + i, gap = w0 + 16 * nb + c - j;
                             const bool sees = ((unsigned)gap < (unsigned)a.window) | ((gap >= 0) & (j < a.sinks));
                             p[kb][nb][i] = sees ? p[kb][nb][i] : -INFINITY;
                         }
@@ -296,7 +332,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 for (int nb = 0; nb < NB; ++nb) {
                     top[nb] = p[0][nb][0];
 #pragma unroll
-                    for (int kb = 0; kb < 4; ++kb)
+                    for (int kb = 0; kb < kPart / 16; ++kb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top[nb] = fmaxf(top[nb], p[kb][nb][i]);
                     top[nb] = groups_max(top[nb]) * l2scale;
@@ -318,7 +354,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                     const float base = m[nb] == -INFINITY ? 0.0f : m[nb];
                     float part = 0.0f;
 #pragma unroll
-                    for (int kb = 0; kb < 4; ++kb)
+                    for (int kb = 0; kb < kPart / 16; ++kb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             p[kb][nb][i] = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -base));
@@ -327,19 +363,28 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                     sum[nb] += part;
                 }
                 __builtin_amdgcn_s_setprio(1);
-                accumulate<T, DP, NB>(sv, p, acc);
+                accumulate<T, DP, NB>(pv, p, acc);
                 __builtin_amdgcn_s_setprio(0);
             } else {
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
+                for (int kb = 0; kb < kPart / 16; ++kb)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float x = __builtin_amdgcn_exp2f(fmaf(p[kb][nb][i], l2scale, -m[nb])) * sum[nb];
-                            dp[kb][nb][i] = (p[kb][nb][i] == -INFINITY) & masked ? 0.0f : x * (dp[kb][nb][i] - delta[nb]) * a.scale;
+                            const float y = (p[kb][nb][i] == -INFINITY) & masked ? 0.0f : x * (dp[kb][nb][i] - delta[nb]);
+                            if (kRefine) {
+                                p[kb][nb][i] = x;
+                                off[nb] += y;
+                            }
+                            dp[kb][nb][i] = y * a.scale;
                         }
-                accumulate<T, DP, NB>(sk, dp, acc);
+                if (kRefine)
+                    accumulate<T, DP, NB>(pk, dp, acc, p, mean);
+                else
+                    accumulate<T, DP, NB>(pk, dp, acc);
+            }
             }
             }
             };
@@ -366,6 +411,15 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                     a.stats[2 * at] = m[nb];
                     a.stats[2 * at + 1] = f;
                 }
+            }
+            if (BACK) {
+                if (kRefine) {
+                    off[nb] = groups_sum(off[nb]);
+                    const float back = off[nb] * a.scale;
+#pragma unroll
+                    for (int b = 0; b < DP / 16; ++b) acc[b][nb] -= mean[b][nb] * back;
+                }
+                if (row < len && g == 0) a.delta[at] = delta[nb] + off[nb];
             }
             if (row < len) {
 #pragma unroll
@@ -513,8 +567,8 @@ __global__ __launch_bounds__(SINKS ? 64 : kThreads, DP == 128 && (SINKS || sizeo
             }
             if (EDGE && flags[turn]) {
                 __syncthreads();
-                clean_tile<T, DP, NT, C::kLd>(sqr);
-                clean_tile<T, DP, NT, C::kLd>(sgo);
+                clean_tile<T, DP, NT, C::kLd>(sqr, kTile);
+                clean_tile<T, DP, NT, C::kLd>(sgo, kTile);
                 __syncthreads();
                 met = true;
             }
