@@ -440,7 +440,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *   weight_dev, bias_dev   cols values of weight_dtype (VAD_DTYPE_F32 or dtype), each may be NULL
  *   y_dev           (rows, cols) dense
  *   stats_dev       (rows, 2) mean and 1 / sqrt(var + eps) for the backward pass; may be NULL
- * Backward: dx_dev (rows, cols) dense, dweight_dev / dbias_dev cols values of weight_dtype; each of the three may be NULL.
+ * Backward (eps as in the forward call): dx_dev (rows, cols) dense, dweight_dev / dbias_dev cols values of weight_dtype; each of the three may be NULL.
  * workspace_dev: vad_layer_norm_workspace_bytes(rows, cols), needed for dweight / dbias.
  */
 size_t vad_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
@@ -448,7 +448,7 @@ int vad_layer_norm_forward(const void* x_dev, int64_t rows, int64_t cols, int64_
                            const void* weight_dev, const void* bias_dev, int dtype, int weight_dtype, float eps,
                            void* y_dev, float* stats_dev, void* stream);
 int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, int64_t rows, int64_t cols, int64_t x_stride,
-                            int64_t dy_stride, const void* weight_dev, int dtype, int weight_dtype,
+                            int64_t dy_stride, const void* weight_dev, int dtype, int weight_dtype, float eps,
                             const float* stats_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
                             void* workspace_dev, size_t workspace_bytes, void* stream);
 

@@ -70,6 +70,25 @@ def test_layer_norm(vad, dtype, rows, cols):
     _close(grads[2], want[3], dy.double().abs().sum(0), rows_n, torch.float32, 'db')
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_layer_norm_of_two_columns(vad, dtype):
+    """dx is what eps leaves of g, a millionth here: right to a few roundings of g, not of g less its projection.  Four or so
+    on the way to 1 / sqrt(var + eps), three times over, and four more; x - mean is exact to 2 ulp of x."""
+    g = _gen(7)
+    x = (_rand(g, 100, 2) * 2 + 0.5)
+    x[0] = 1.0                                              # no variance: all of g - mean g
+    x = x.to(dtype).requires_grad_()
+    w = (1 + _rand(g, 2, scale=0.3))
+    dy = _rand(g, 100, 2, dtype=dtype)
+    for view in (x, x[:, [1, 0]], torch.cat((x, x), 1)[:, 1:3]):           # the last: rows that end inside a word
+        dx = torch.autograd.grad(vad.layer_norm(view, w), view, dy)[0]
+        want = ref.layer_norm(view.detach(), w, None, 1e-5, dy)[1]
+        xd = view.detach().double()
+        r = 1 / torch.sqrt(xd.var(1, unbiased=False, keepdim=True) + 1e-5)
+        mag = 1e-5 * r ** 3 * (dy.double() * w).abs().sum(1, keepdim=True) * (1 + (xd.abs().amax(1, keepdim=True) * r) ** 2)
+        _close(dx, want, mag.expand_as(xd), 30 * ULP, dtype, 'dx')
+
+
 def test_layer_norm_parameters_shapes_and_strides(vad):
     g = _gen(5)
     x = _rand(g, 4, 6, 48)

@@ -43,9 +43,10 @@ def test_c_entry_points_refuse_before_any_device_work(L):
         ('vad_layer_norm_forward', (ok, -1, 4, 4, None, None, 0, 0, 1e-5, ok, None, None), b'out of range'),
         ('vad_layer_norm_forward', (ok, 1, 4, 4, None, None, 0, 0, math.nan, ok, None, None), b'eps'),
         ('vad_layer_norm_forward', (None, 1, 4, 4, None, None, 0, 0, 1e-5, ok, None, None), b'null pointer'),
-        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, ok, ok, ok, ok, ok, 8, None), b'too small'),
-        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, None, ok, ok, ok, ok, 32, None), b'null pointer'),
-        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, ok, ok, ok, ok, None, 32, None), b'workspace'),
+        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, 1e-5, ok, ok, ok, ok, ok, 8, None), b'too small'),
+        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, 1e-5, None, ok, ok, ok, ok, 32, None), b'null pointer'),
+        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, 1e-5, ok, ok, ok, ok, None, 32, None), b'workspace'),
+        ('vad_layer_norm_backward', (ok, ok, 1, 4, 4, 4, None, 0, 0, -1.0, ok, ok, ok, ok, ok, 32, None), b'eps'),
         ('vad_linear_attention_forward', fwd(dtype=5), b'dtype'),
         ('vad_linear_attention_forward', fwd(dim=129), b'head dimension'),
         ('vad_linear_attention_forward', fwd(dim=0), b'head dimension'),

@@ -166,7 +166,7 @@ def lib():
     L.vad_layer_norm_forward.restype = i32
     L.vad_layer_norm_forward.argtypes = [c_void, c_i64, c_i64, c_i64, c_void, c_void, i32, i32, f32, c_void, c_void, c_void]
     L.vad_layer_norm_backward.restype = i32
-    L.vad_layer_norm_backward.argtypes = [c_void, c_void] + [c_i64] * 4 + [c_void, i32, i32] + [c_void] * 5 + [size, c_void]
+    L.vad_layer_norm_backward.argtypes = [c_void, c_void] + [c_i64] * 4 + [c_void, i32, i32, f32] + [c_void] * 5 + [size, c_void]
     heads = [c_void, c_void]                                    # a tensor and its strides
     seq = [c_void, c_i64, c_i64, c_i64]                         # starts, n_seq, n_tokens, max_len
     L.vad_linear_attention_workspace_bytes.restype = size

@@ -240,12 +240,14 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
         s1 = group_sum(s1, a.lanes, scratch) * inv;
         s2 = group_sum(s2, a.lanes, scratch) * inv;
         if (!live || !dx) continue;
+        // Of two columns g - mean g is a multiple of xh, and eps / (var + eps) of it is left: formed as that, not as a difference.
+        const bool pair = a.cols == 2;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int c = (l + n * a.lanes) * VE;
             if (c < a.cols) {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) g[n][e] = rstd * (g[n][e] - s1 - v[n][e] * s2);
+                for (int e = 0; e < VE; ++e) g[n][e] = rstd * (pair ? (g[n][e] - s1) * (a.eps * rstd * rstd) : g[n][e] - s1 - v[n][e] * s2);
                 store_vec<T, VE>(dx + row * a.cols + c, g[n]);
             }
         }
@@ -451,11 +453,11 @@ int run_forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, con
 
 template <typename T>
 int run_backward(const void* x, const void* dy, int64_t rows, int64_t cols, int64_t x_stride, int64_t dy_stride, const void* w,
-                 int w_f32, const float* stats, void* dx, void* dw, void* db, float* part, hipStream_t st) {
+                 int w_f32, float eps, const float* stats, void* dx, void* dw, void* db, float* part, hipStream_t st) {
     const Shape sh = row_shape((int)cols, sizeof(T),
                                reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx) |
                                    (uintptr_t)(x_stride * sizeof(T)) | (uintptr_t)(dy_stride * sizeof(T)));
-    Rows a = {rows, x_stride, (int)cols, sh.lanes, 0.0f};
+    Rows a = {rows, x_stride, (int)cols, sh.lanes, eps};
     Params<T> pr = {w, nullptr, w_f32 != 0};
     const T* xp = static_cast<const T*>(x);
     const T* gp = static_cast<const T*>(dy);
@@ -513,7 +515,7 @@ extern "C" int vad_layer_norm_forward(const void* x_dev, int64_t rows, int64_t c
 }
 
 extern "C" int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, int64_t rows, int64_t cols, int64_t x_stride,
-                                       int64_t dy_stride, const void* weight_dev, int dtype, int weight_dtype,
+                                       int64_t dy_stride, const void* weight_dev, int dtype, int weight_dtype, float eps,
                                        const float* stats_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
                                        void* workspace_dev, size_t workspace_bytes, void* stream) {
     using namespace vad;
@@ -522,6 +524,7 @@ extern "C" int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, in
     VAD_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 28) && x_stride >= 0 && dy_stride >= 0,
                 "rows %lld, cols %lld, x_stride %lld or dy_stride %lld out of range", (long long)rows, (long long)cols,
                 (long long)x_stride, (long long)dy_stride);
+    VAD_REQUIRE(eps >= 0.0f && eps < INFINITY, "eps must be finite and not negative");
     VAD_REQUIRE(rows == 0 || (x_dev && dy_dev && stats_dev), "null pointer argument");
     VAD_REQUIRE((!dweight_dev && !dbias_dev) || workspace_bytes >= vad_layer_norm_workspace_bytes(rows, cols),
                 "workspace of %zu bytes is too small", workspace_bytes);
@@ -531,7 +534,7 @@ extern "C" int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, in
     if (rows == 0 && !dweight_dev && !dbias_dev) return VAD_OK;
     return dtype == VAD_DTYPE_F32
                ? run_backward<float>(x_dev, dy_dev, rows, cols, x_stride, dy_stride, weight_dev, weight_dtype == VAD_DTYPE_F32,
-                                     stats_dev, dx_dev, dweight_dev, dbias_dev, part, st)
+                                     eps, stats_dev, dx_dev, dweight_dev, dbias_dev, part, st)
                : run_backward<__bf16>(x_dev, dy_dev, rows, cols, x_stride, dy_stride, weight_dev, weight_dtype == VAD_DTYPE_F32,
-                                      stats_dev, dx_dev, dweight_dev, dbias_dev, part, st);
+                                      eps, stats_dev, dx_dev, dweight_dev, dbias_dev, part, st);
 }

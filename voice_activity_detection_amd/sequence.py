@@ -162,6 +162,7 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         y, stats = _norm_forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
+        ctx.eps = eps
         ctx.param = None if weight is None and bias is None else (weight if weight is not None else bias).dtype
         return y
 
@@ -180,7 +181,7 @@ class _LayerNorm(torch.autograd.Function):
         if weight is not None and not weight.is_contiguous():
             weight = weight.contiguous()
         _call(_lib.lib().vad_layer_norm_backward, x.get_device(), rows.data_ptr(), dyr.data_ptr(), n, cols, rows.stride(0), dyr.stride(0),
-              _ptr(weight), _DTYPES[x.dtype], 0 if ctx.param is None else _DTYPES[ctx.param], stats.data_ptr(), _ptr(dx), _ptr(dw),
+              _ptr(weight), _DTYPES[x.dtype], 0 if ctx.param is None else _DTYPES[ctx.param], ctx.eps, stats.data_ptr(), _ptr(dx), _ptr(dw),
               _ptr(db), _ptr(ws), size)
         return dx, dw, db, None
 
