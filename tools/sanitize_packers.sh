@@ -9,5 +9,5 @@ out=${TMPDIR:-/tmp}/vad_pack_sanitize
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O1 -g -std=c++17 -Xarch_host -fsanitize=address -Xarch_host -fsanitize=undefined \
     -Xarch_host -fno-omit-frame-pointer -Xclang -target-feature -Xclang -packed-fp32-ops \
     -I"$root/include" -I"$root/voice_activity_detection_amd/csrc" -o "$out" "$root/tests/c_client/pack_sanitize.cpp" \
-    "$root"/voice_activity_detection_amd/csrc/{abi,mfcc,rnn,densenet,nicknet,nicknet_stream,overlay,sweep,seq}.hip 2>&1 | grep -v "packed-fp32-ops" || true
+    "$root"/voice_activity_detection_amd/csrc/{abi,mfcc,rnn,densenet,nicknet,nicknet_stream,overlay,sweep,seq,layer_norm,linear_attention,window_attention}.hip 2>&1 | grep -v "packed-fp32-ops" || true
 "$out"

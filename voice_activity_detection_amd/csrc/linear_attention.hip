@@ -12,10 +12,15 @@
 // first launch computes each span's state from k and v alone, and the walk of every span starts from those before it --
 // added up by its block, or, where the spans are many, by a launch in between that goes along the sequence once.
 //
+// Measured, bfloat16 heads of 64: 4 x 16 heads of 8192 rows in 104 us (states of the spans 30, their join 7, walk 67: 268 MB
+// at 2.6 TB/s, where a copy takes 57 us -- latency along a walk and vector work on its 64 x 64 weights bound it, not memory);
+// 24 ragged sequences of up to 2000 rows and 8 heads, with gradients, 198 us.  A step of 64 x 16 states of 128 x 128 22.7 us:
+// 134 MB read and written, 5.9 TB/s with what the last cache keeps.
+//
 // Wave w of a block owns columns 16 w .. 16 w + 15 of the state and of the outputs.  The state stays in float32; for
 // bfloat16 inputs its update multiplies v by the decay in float32 and splits the product into bfloat16 terms -- three, which
-// is exact, where the state is handed out or crosses spans, two (2^-17) where it only feeds outputs of 8 bits; the weights a^(i-j) (q . k) and the copy of the state that q is
-// multiplied with are rounded to bfloat16 once.
+// is exact, where the state is handed out or crosses spans, two (2^-17) where it only feeds outputs of 8 bits.  The weights
+// a^(i-j) (q . k) and the copy of the state that q is multiplied with are rounded to bfloat16 once.
 
 #include <mutex>
 
