@@ -664,8 +664,13 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WindowArgs<T> a) 
     if (key >= len) return;
     const float* p = a.parts + ((int64_t)s * a.kv_heads + hk) * (1 + a.segments) * 2 * n + e;
     float x = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i <= a.segments; ++i) x += p[(int64_t)i * 2 * n];
+    for (int i = 0; i <= a.segments; i += 16) {
+        float part[16];                                        // asked for together, added in order
+#pragma unroll
+        for (int u = 0; u < 16; ++u) part[u] = i + u <= a.segments ? p[(int64_t)(i + u) * 2 * n] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) x += part[u];
+    }
     const int64_t row = (a.seq.starts ? first : (int64_t)s * a.seq.max_len) + key;
     (which ? a.dv : a.dk)[(row * a.kv_heads + hk) * a.dim + d] = (T)x;
 }
