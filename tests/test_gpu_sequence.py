@@ -664,6 +664,24 @@ def test_hints_windows_and_strides_at_their_ends(vad):
     assert all(not t.any() for t in torch.autograd.grad(vad.layer_norm(empty, w, b).sum(), (w, b)))
 
 
+@pytest.mark.parametrize('dim,window,sinks', [(40, 300, 5), (30, 256, 0), (64, 1000, 64)])
+def test_large_launches_agree_with_small_ones(vad, dim, window, sinks):
+    """Many rows take wider blocks than few do.  Either form is off by 2^-8 of every weight's term and of the result."""
+    g = _gen(101)
+    n = 8200
+    q, k, v = (_rand(g, 2, n, heads, dim, dtype=torch.bfloat16) for heads in (17, 1, 1))
+    k[:, 8000:], v[:, 8100:] = math.nan, math.inf
+    o = vad.window_attention(q, k, v, window, sinks)
+    alone = torch.cat([vad.window_attention(q[i:i + 1], k[i:i + 1], v[i:i + 1], window, sinks) for i in range(2)])
+    size = vad.window_attention(q[:, :8000], k[:, :8000], v[:, :8000].abs(), window, sinks).float()
+    a, b = o[:, :8000].float(), alone[:, :8000].float()
+    assert ((a - b).abs() <= 2.0 ** -7 * (size * (1 + 2.0 ** -6) + b.abs())).all()
+    assert o[:, 8000:].isnan().all() and alone[:, 8000:].isnan().all()
+    starts = torch.tensor([0, n, 2 * n], device='cuda')
+    packed = vad.window_attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), window, sinks, starts=starts, max_len=n)
+    assert torch.equal(packed.view_as(o).nan_to_num(), o.nan_to_num())
+
+
 def test_many_short_sequences(vad):
     """65535 sequences of 0 .. 2 rows without a hint: more tiles than a launch holds."""
     n = 65535

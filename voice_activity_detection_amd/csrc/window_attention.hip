@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             T* pv = sv + half * kPart * C::kLd;
             f32x4 p[kPart / 16][NB], dp[kPart / 16][NB];
             if (active) {
-                // products ahead of the other waves' softmax: 258 -> 248 us at 128 columns
+                // products ahead of the other waves' softmax: 228 -> 223 us at 128 columns, 299 -> 295 at 64
                 __builtin_amdgcn_s_setprio(1);
                 scores<T, DP, NB>(pk, qf, p);
                 if (BACK) scores<T, DP, NB>(pv, gf, dp);
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
             }
             }
             };
-            // (the forward pass is faster with one body that asks: 254 against 322 us on 2 x 16 heads of 8192 rows of 128)
+            // (the forward pass is faster with one body that asks: 256 against 325 us on 2 x 16 heads of 8192 rows of 128)
             if (!BACK || is_edge(t))
                 step(std::true_type{});
             else
@@ -928,15 +928,30 @@ unsigned row_tiles(int64_t max_len, int rows, int64_t heads) {
 
 template <typename T, int DP, bool BUF>
 struct Kernels {
-    // 16-row blocks of own rows per wave.  Two read a streamed tile half as often, one leaves registers for twice the waves: 16
-    // heads of 8192 rows with a window of 1000 (4 sequences of 64 columns; 2 of 128) take 298 and 320 us for O with one and
-    // two blocks at 64 columns, 300 and 235 us at 128; dQ 472 and 469, dK and dV 602 and 541 us at 64 columns, but 61 and 66,
-    // 68 and 92 us on 8 sequences of up to 2000 rows with a window of 300.
-    static constexpr int NB = DP == 128 && sizeof(T) == 2 ? 2 : 1, NK = 1;
+    // 16-row blocks of own rows per wave.  Two read a streamed tile half as often, one makes twice the blocks and leaves registers
+    // for more waves.  O takes two where they still make two rounds of blocks and the window's middle outweighs its edges, and at 128
+    // columns always: 4 sequences (2 of 128 columns) of 8192 rows, 16 heads, window 1000: 270 us with two and 315 with one at 64 columns,
+    // 172 and 186 at 32, 223 and 268 at 128; a single one 82 and 82; 8 sequences of up to 2000 rows, 8 heads, window 300: 47 and 41 us; 32
+    // of up to 1000 rows, 16 heads, window 100: 95 and 91.  dQ (503 and 456 us at 64 columns), dK and dV (528
+    // and 527; 100 and 68 on the short ones) take one: at 128 columns two do not fit the registers.
+    static constexpr int NK = 1;
     static constexpr size_t kLds = TileShape<T, DP>::lds(TileShape<T, DP>::kBuffers), kLdsSinks = TileShape<T, DP>::lds(1);
-    static void forward(WindowArgs<T> a, hipStream_t st) {
+    static bool two_blocks(const WindowArgs<T>& a) {
+        const int64_t dense = (int64_t)a.n_seq * a.seq.max_len, rows = a.seq.starts && a.seq.n_tokens < dense ? a.seq.n_tokens : dense;
+        return rows / 128 * a.heads >= 2048 && a.window >= 256;
+    }
+    template <int NB>
+    static void rows(WindowArgs<T> a, hipStream_t st) {
         a.tiles = row_tiles(a.seq.max_len, 64 * NB, (int64_t)a.heads * a.n_seq);
         hipLaunchKernelGGL((window_rows_kernel<T, DP, NB, false, BUF>), dim3(a.tiles * a.heads * a.n_seq), dim3(kThreads), kLds, st, a);
+    }
+    static void forward(const WindowArgs<T>& a, hipStream_t st) {
+        if constexpr (sizeof(T) == 4)
+            rows<1>(a, st);
+        else if constexpr (DP == 128)
+            rows<2>(a, st);
+        else
+            two_blocks(a) ? rows<2>(a, st) : rows<1>(a, st);
     }
     static void backward(WindowArgs<T> a, hipStream_t st) {
         const dim3 block(kThreads);
@@ -950,7 +965,9 @@ struct Kernels {
         }
     }
     static int allow() {
-        const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NB, false, BUF>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NK, true, BUF>),
+        constexpr int kOne = sizeof(T) == 2 && DP == 128 ? 2 : 1, kTwo = sizeof(T) == 2 ? 2 : 1;
+        const void* f[] = {reinterpret_cast<const void*>(&window_rows_kernel<T, DP, kOne, false, BUF>), reinterpret_cast<const void*>(&window_rows_kernel<T, DP, kTwo, false, BUF>),
+                           reinterpret_cast<const void*>(&window_rows_kernel<T, DP, NK, true, BUF>),
                            reinterpret_cast<const void*>(&window_keys_kernel<T, DP, NK, false, BUF>), reinterpret_cast<const void*>(&window_keys_kernel<T, DP, 1, true, BUF>)};
         for (const void* k : f) VAD_HIP_CHECK(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds));
         return VAD_OK;
