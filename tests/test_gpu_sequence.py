@@ -889,3 +889,27 @@ def test_device_refusals(vad):
     first = torch.autograd.grad(vad.layer_norm(leaf).square().sum(), leaf, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         torch.autograd.grad(first.sum(), leaf)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('window,sinks', [(129, 0), (190, 3), (650, 64)])
+def test_window_step_with_infinities_in_the_new_row(vad, dtype, window, sinks):
+    """An infinite value in the new row reaches the output as that infinity from every slot, those next to the ends of the
+    parts that a cache is cut into among them; the other columns stay finite."""
+    g = _gen(window)
+    slots, dim = sinks + window, 128
+    ck, cv = (_rand(g, 1, slots, 2, dim, dtype=dtype) for _ in range(2))
+    q = _rand(g, slots, 2, dim, dtype=dtype)
+    k, v = (_rand(g, slots, 2, dim, dtype=dtype) for _ in range(2))
+    v[:, :, 3], v[:, :, 70] = math.inf, -math.inf
+    rest = torch.ones(dim, dtype=torch.bool, device='cuda')
+    rest[3] = rest[70] = False
+    for slot in range(sinks, slots):
+        pos = torch.tensor([slot + window], device='cuda')
+        kk, vv = ck.clone(), cv.clone()
+        i = slice(slot, slot + 1)
+        o = vad.window_attention_step(q[i], k[i], v[i], kk, vv, pos, window, sinks)[0].float()
+        assert (o[:, 3] == math.inf).all() and (o[:, 70] == -math.inf).all(), slot
+        p = torch.softmax((kk[0].double() * q[i].double()).sum(-1) * dim ** -0.5, 0)              # slots, heads
+        want = (p[..., None] * vv[0].double())[..., rest].sum(0)
+        assert float((o[:, rest].double() - want).abs().max()) < 1e-5 + 2 * U[dtype] * float(want.abs().max()), slot

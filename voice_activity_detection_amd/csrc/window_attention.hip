@@ -758,13 +758,14 @@ __global__ __launch_bounds__(kThreads) void window_step_kernel(StepArgs<T> a) {
                 }
             }
         }
-        if (own >= base && own < base + kTake) {
+        // (slots from hi on are the next split's: a weight of zero would still make NaN of an infinity)
+        if (own >= base && own < base + kTake && own < hi) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u)
                 if (base + u * kRows + r == own) {
                     kr[u] = new_k;
                     vr[u] = new_v;
-                    if (chunk == 0 && own < hi) {
+                    if (chunk == 0) {
                         store_piece(ck + (int64_t)own * a.ck.st, d, a.dim, new_k, BUF);
                         store_piece(cv + (int64_t)own * a.cv.st, d, a.dim, new_v, BUF);
                     }
