@@ -913,3 +913,99 @@ def test_window_step_with_infinities_in_the_new_row(vad, dtype, window, sinks):
         p = torch.softmax((kk[0].double() * q[i].double()).sum(-1) * dim ** -0.5, 0)              # slots, heads
         want = (p[..., None] * vv[0].double())[..., rest].sum(0)
         assert float((o[:, rest].double() - want).abs().max()) < 1e-5 + 2 * U[dtype] * float(want.abs().max()), slot
+
+
+def _outer_sums(keys, values, queries, a, scale, back=False):
+    """S_t = a S_{t-1} + keys_t values_t^T row by row, o_t = scale queries_t S_t, one product at a time in float64; `back`: from
+    the last row to the first.  The S behind the last row taken and the rows o."""
+    s, out = torch.zeros(keys.size(1), values.size(1), dtype=torch.float64, device=keys.device), []
+    order = range(keys.size(0))
+    for t in reversed(order) if back else order:
+        s = a * s + keys[t, :, None] * values[t, None, :]
+        out.append(scale * (queries[t, :, None] * s).sum(0))
+    return s, torch.stack(out[::-1] if back else out)
+
+
+def _same_kinds(got, want, what):
+    """Infinities of the same sign, NaN and finite values in the same places."""
+    got = got.double()
+    assert torch.equal(got.isnan(), want.isnan()), what
+    for sign in (math.inf, -math.inf):
+        assert torch.equal(got == sign, want == sign), what
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('length,dim', [(50, 64), (150, 30), (1000, 64), (300, 128)])
+def test_linear_attention_infinite_keys(vad, dtype, length, dim):
+    """An infinite key makes infinities of the state's row and of what its queries read, NaN only where the recurrence itself has
+    one; infinite output gradients do the same to dk, in either type."""
+    g = _gen(length + dim)
+    # values that a few bits hold and no product that vanishes: the lower terms of a split float32 are zero
+    q, k, v, do = (torch.randint(1, 5, (1, length, 2, dim), generator=g, device='cuda').to(dtype) / 4 for _ in range(4))
+    signs = torch.randint(0, 2, (4, 1, length, 2, dim), generator=g, device='cuda') * 2 - 1
+    q, k, v, do = (t * s for t, s in zip((q, k, v, do), signs))
+    log_decay = torch.tensor([0.0, -0.01], device='cuda')
+
+    def spoilt(t):
+        bad = t.clone()
+        bad[0, 20, 0, 5], bad[0, length - 3, 1, dim - 1] = math.inf, -math.inf
+        return bad
+
+    bad = spoilt(k)
+    o, s = vad.linear_attention(q, bad, v, log_decay, scale=0.5)
+    leaf = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(vad.linear_attention(*leaf, log_decay, scale=0.5)[0], leaf, spoilt(do))
+    for h, a in enumerate(log_decay.double().exp().tolist()):
+        x = [t[0, :, h].double() for t in (q, bad, v, spoilt(do))]
+        ws, wo = _outer_sums(x[1], x[2], x[0], a, 0.5)
+        assert ws.isinf().any() and not ws.isnan().any()
+        _same_kinds(s[0, h], ws, 'state')
+        _same_kinds(o[0, :, h], wo, 'o')
+        _same_kinds(grads[1][0, :, h], _outer_sums(x[3], x[0], x[2], a, 0.5, back=True)[1], 'dk')
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('length,dim', [(50, 64), (150, 30), (1000, 70), (300, 128)])
+def test_linear_attention_infinite_values(vad, dtype, length, dim):
+    """An infinite value where nothing is negative is an infinity in the state's column and in the rows behind it, and one of the
+    output's gradient is one in dv, at any head size: no order of the sums makes NaN of it."""
+    g = _gen(length + dim)
+    q, k, v, do = (torch.randint(1, 5, (1, length, 2, dim), generator=g, device='cuda').to(dtype) / 4 for _ in range(4))
+    log_decay = torch.tensor([0.0, -0.01], device='cuda')
+    bad, bad_do = v.clone(), do.clone()
+    bad[0, 20, 0, 5], bad[0, length - 3, 1, dim - 1] = math.inf, math.inf
+    bad_do[0, length - 20, 0, 5], bad_do[0, 2, 1, dim - 1] = math.inf, math.inf
+    o, s = vad.linear_attention(q, k, bad, log_decay, scale=0.5)
+    leaf = [t.clone().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(vad.linear_attention(*leaf, log_decay, scale=0.5)[0], leaf, bad_do)
+    for h, a in enumerate(log_decay.double().exp().tolist()):
+        x = [t[0, :, h].double() for t in (q, k, bad, bad_do)]
+        ws, wo = _outer_sums(x[1], x[2], x[0], a, 0.5)
+        assert ws.isinf().any() and not ws.isnan().any() and not wo.isnan().any()
+        _same_kinds(s[0, h], ws, 'state')
+        _same_kinds(o[0, :, h], wo, 'o')
+        _same_kinds(grads[2][0, :, h], _outer_sums(x[0], x[3], x[1], a, 0.5, back=True)[1], 'dv')
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [30, 64, 128])
+def test_infinities_are_found_in_every_column(vad, dtype, dim):
+    """One infinity or NaN per sequence, each in another column, of k and of v."""
+    g = _gen(dim)
+    n = torch.arange(dim, device='cuda')
+    q, k, v = (torch.randint(1, 5, (dim, 70, 1, dim), generator=g, device='cuda').to(dtype) / 4 for _ in range(3))
+    log_decay = torch.tensor([-0.01], device='cuda')
+    for value in (math.inf, -math.inf, math.nan):
+        kk, vv = k.clone(), v.clone()
+        kk[n, n * 7 % 64, 0, n] = value
+        vv[n, n * 5 % 64, 0, n] = value
+        for a, b, axis, row in ((kk, v, 1, n * 7 % 64), (k, vv, 2, n * 5 % 64)):
+            o, s = vad.linear_attention(q, a, b, log_decay)
+            hit = torch.zeros(dim, dim, dim, dtype=torch.bool, device='cuda')
+            hit[n, n] = True
+            hit = hit if axis == 1 else hit.transpose(1, 2)
+            want = torch.full_like(s[:, 0], value)
+            assert torch.equal(s[:, 0].isfinite(), ~hit)
+            assert torch.equal(s[:, 0][hit].isnan(), want[hit].isnan()) and (value != value or torch.equal(s[:, 0][hit], want[hit]))
+            w = vad.window_attention(q, a, b, 20)
+            assert torch.isfinite(w[row < 50, 69]).all() and not torch.isfinite(o[:, 69]).all()

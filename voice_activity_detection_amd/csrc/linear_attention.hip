@@ -98,12 +98,12 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&f)[3]) {
 }
 
 // Waves per SIMD that the registers are shared out for.
-template <typename T, int DP>
-constexpr int walk_waves() { return sizeof(T) == 2 && DP < 128 ? 3 : 2; }
+template <typename T, int DP, bool STATE>
+constexpr int walk_waves() { return sizeof(T) == 2 && STATE ? 4 : (sizeof(T) == 2 && DP < 128 ? 3 : 2); }
 
 // BUF: rows are whole words at 4-byte boundaries (a.whole).
 template <typename T, int DP, bool STATE, bool BUF>
-__global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kernel(WalkArgs<T> a) {
+__global__ __launch_bounds__(DP * 4, (walk_waves<T, DP, STATE>())) void decay_walk_kernel(WalkArgs<T> a) {
     using C = WalkShape<T, DP>;
     extern __shared__ char lds_raw[];
     T* sk = reinterpret_cast<T*>(lds_raw);
@@ -206,7 +206,8 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
         rv.put(sv, dim);
         if (!STATE) {
             rq.put(sq_, dim);
-            if (rv.not_finite()) flags[turn] = 1;
+            // (of bfloat16 keys as well, 67 -> 69 us on 4 x 16 heads of 8192 rows)
+            if (rv.not_finite() | (sizeof(T) == 2 && rk.not_finite())) flags[turn] = 1;
         }
         __syncthreads();
         const bool careful = !STATE && flags[turn];
@@ -260,9 +261,9 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
 
         // the state behind the piece
         const bool last = tc + kPiece >= t1;
-        const bool finish = !STATE && last && t1 == len && w.s1;
-        if (!last || STATE || finish) {
-            const bool less = finish && !w.reverse;                        // the forward walk hands out S, not a S
+        const bool finish = !STATE && last && t1 == len && w.s1, updates = !last || STATE || finish;
+        const bool less = finish && !w.reverse;                            // the forward walk hands out S, not a S
+        if (updates && !careful) {
             const float keep = n == kPiece && !less ? a32 * a32 : power(l2, (float)(n - (less ? 1 : 0)));
 #pragma unroll
             for (int b = 0; b < DP / 16; ++b) H[b] *= keep;
@@ -332,7 +333,48 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP>())) void decay_walk_kern
                 if (row < n) store_quad(oc + sign * row * a.heads * dim, 16 * wave + 4 * g, dim, o[rb], BUF);
             }
         }
+        if (careful && updates) {
+            // Row by row: the matrix product would also multiply infinities and NaN by what is only there for its shape -- the zeros
+            // behind a head's columns, the lower terms of a split value, zero or of the other sign -- and 0 * inf is NaN.
+            const float keep = power(l2, (float)(n - (less ? 1 : 0)));
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) H[b] *= keep;
+#pragma unroll 1
+            for (int row = 0; row < n; ++row) {
+                const float x = (float)sv[row * C::kLd + col] * (w.update * power(l2, (float)(n - row - (less ? 1 : 0))));
+#pragma unroll
+                for (int b = 0; b < DP / 16; ++b) {
+                    const Quad<T> y = *reinterpret_cast<const Quad<T>*>(sk + row * C::kLd + 16 * b + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) H[b][i] = 16 * b + 4 * g + i < dim ? fmaf((float)y[i], x, H[b][i]) : 0.0f;
+                }
+            }
+        }
         __syncthreads();
+    }
+    if (STATE && sizeof(T) == 2) {
+        // A NaN in a span's state: perhaps an infinity's meeting with a lower term.  Once more, row by row.
+        bool spoilt = false;
+#pragma unroll
+        for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) spoilt |= H[b][i] != H[b][i];
+        if (__any(spoilt)) {
+#pragma unroll
+            for (int b = 0; b < DP / 16; ++b) H[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int64_t t = t0; t < t1 && col < dim; ++t) {
+                const int64_t at = w.reverse ? len - 1 - t : t;
+                const float x = (float)vp[at * w.v.st + col] * (w.update * power(l2, (float)(t1 - t)));
+#pragma unroll
+                for (int b = 0; b < DP / 16; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = 16 * b + 4 * g + i;
+                        if (d < dim) H[b][i] = fmaf((float)kp[at * w.k.st + d], x, H[b][i]);
+                    }
+            }
+        }
     }
     float* out = STATE ? spans : (t1 == len && w.s1 ? w.s1 + head * elems : nullptr);
     if (out) {

@@ -219,18 +219,30 @@ __device__ __forceinline__ u32x4 load_piece(__amdgpu_buffer_rsrc_t b, int offset
     return __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0);
 }
 
-// Whether any of the values in a 16-byte piece is an infinity or a NaN.
-template <typename T>
-__device__ __forceinline__ bool piece_not_finite(u32x4 v) {
-    bool bad = false;
+// Whether any of the values in some 16-byte pieces is an infinity or a NaN.  Times zero they are NaN, and two bfloat16 take one
+// instruction for that; of float32 the largest bit pattern without its sign says it.
+template <typename T, int N>
+__device__ __forceinline__ bool any_not_finite(const u32x4 (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (sizeof(T) == 4)
-            bad |= (v[i] & 0x7F800000u) == 0x7F800000u;
-        else
-            bad |= ((v[i] & 0x7F800000u) == 0x7F800000u) | ((v[i] & 0x7F80u) == 0x7F80u);
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = max(top, v[n][i] & 0x7FFFFFFFu);
+        return top >= 0x7F800000u;
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 zero = {(__bf16)0.0f, (__bf16)0.0f};
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned word = v[n][i];
+                sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, word), zero, sum, false);
+            }
+        return sum != sum;
     }
-    return bad;
 }
 
 // 64 rows of one head on their way through a block's registers into an LDS tile of PITCH elements a row.  BUF: by buffer
@@ -273,12 +285,7 @@ struct Staged {
 #pragma unroll
         for (int n = 0; n < kPieces; ++n) *reinterpret_cast<u32x4*>(tile + (row0 + n * kStep) * kLd + c) = r[n];
     }
-    __device__ __forceinline__ bool not_finite() const {
-        bool bad = false;
-#pragma unroll
-        for (int n = 0; n < kPieces; ++n) bad |= piece_not_finite<T>(r[n]);
-        return bad;
-    }
+    __device__ __forceinline__ bool not_finite() const { return any_not_finite<T>(r); }
 };
 
 // The infinities and NaN in a tile's first `rows` rows become zero: every thread of the block cleans pieces of it.
