@@ -12,6 +12,8 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from oracle import sequence_ref as ref
 
@@ -1009,3 +1011,38 @@ def test_infinities_are_found_in_every_column(vad, dtype, dim):
             assert torch.equal(s[:, 0][hit].isnan(), want[hit].isnan()) and (value != value or torch.equal(s[:, 0][hit], want[hit]))
             w = vad.window_attention(q, a, b, 20)
             assert torch.isfinite(w[row < 50, 69]).all() and not torch.isfinite(o[:, 69]).all()
+
+
+def test_derivatives_and_recordings_that_cannot_pass_are_refused(vad):
+    """Forward-mode derivatives, also of an output's gradient, and calls that a tracer would not record: an error in place of a
+    result that lacks them.  Plain tensors in a dual level are computed."""
+    g = _gen(5)
+    q, k, v = (_rand(g, 1, 10, 2, 16) for _ in range(3))
+    log_decay = _decays(2)
+    calls = [lambda x: vad.layer_norm(x), lambda x: vad.linear_attention(x, k, v, log_decay)[0], lambda x: vad.window_attention(x, k, v, 4)]
+    with forward_ad.dual_level():
+        for call in calls:
+            for x in (q, q.clone().requires_grad_()):
+                with pytest.raises(ValueError, match='forward-mode'):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+            leaf = q.clone().requires_grad_()
+            o = call(leaf)
+            assert forward_ad.unpack_dual(o).tangent is None
+            with pytest.raises(ValueError, match='forward-mode'):
+                torch.autograd.grad(o, leaf, forward_ad.make_dual(torch.ones_like(o), torch.ones_like(o)))
+    row, pos = q[0], torch.zeros(10, dtype=torch.int64, device='cuda')
+    state, cache = torch.zeros(10, 2, 16, 16, device='cuda'), torch.zeros(2, 10, 4, 2, 16, device='cuda')
+    one = torch.zeros(2, 1, 4, 2, 16, device='cuda')
+    calls += [lambda x: vad.linear_attention_step(x[0], row, row, log_decay, state),
+              lambda x: vad.window_attention_step(x[0], row, row, cache[0], cache[1], pos, 4), lambda x: vad.window_cache_fill(x, v, one[0], one[1], 4)]
+    for call in calls:
+        with pytest.raises(ValueError, match='traced'):
+            torch.jit.trace(call, (q,), check_trace=False)
+        with pytest.raises(ValueError, match='traced'):
+            make_fx(call)(q)
+    assert not state.any() and not cache.any() and not one.any()
+    for transform in (lambda call: torch.vmap(call)(q[None]), lambda call: torch.func.jvp(call, (q,), (q,)),
+                      lambda call: torch.func.grad(lambda x: call(x).sum())(q)):
+        for call in calls[:3]:
+            with pytest.raises((RuntimeError, ValueError)):
+                transform(call)

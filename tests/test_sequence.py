@@ -6,6 +6,7 @@ import math
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import voice_activity_detection_amd as pkg
 from oracle import sequence_ref as ref
@@ -145,3 +146,21 @@ def test_plain_layer_norm():
     y = torch.nn.functional.layer_norm(leaf[0], (9,), leaf[1], leaf[2], 1e-5)
     for got, want in zip(ref.layer_norm(x, w, b, 1e-5, dy), (y, *torch.autograd.grad(y, leaf, dy))):
         assert torch.allclose(got, want.detach(), rtol=1e-11, atol=1e-12)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not ask for a gradient, and a result without its tangent would read as a derivative of zero."""
+    q = torch.zeros(1, 4, 2, 8)
+    row, ld, state, cache = q[0], torch.zeros(2), torch.zeros(4, 2, 8, 8), torch.zeros(4, 4, 2, 8)
+    pos, w = torch.zeros(4, dtype=torch.int64), torch.ones(8)
+    calls = [(pkg.layer_norm, [q, w, w]), (pkg.linear_attention, [q, q, q, ld]), (pkg.linear_attention_step, [row, row, row, ld, state]),
+             (lambda a, b, c: pkg.window_attention(a, b, c, 3), [q, q, q]), (lambda *t: pkg.linear_attention(q, q, q, ld, state=t[0]), [state]),
+             (lambda a, b, c, d, e: pkg.window_attention_step(a, b, c, d, e, pos, 4), [row, row, row, cache, cache]),
+             (lambda a, b, c, d: pkg.window_cache_fill(a, b, c, d, 4), [q, q, cache, cache])]
+    with forward_ad.dual_level():
+        for call, args in calls:
+            for i, t in enumerate(args):
+                with pytest.raises(ValueError, match='forward-mode'):
+                    call(*args[:i], forward_ad.make_dual(t, torch.ones_like(t)), *args[i + 1:])
+            with pytest.raises(ValueError, match='CUDA tensor'):        # others are as welcome as outside
+                call(*args)

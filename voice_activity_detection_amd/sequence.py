@@ -19,6 +19,8 @@ import operator
 
 import torch
 from torch._C import _cuda_getCurrentRawStream, _cuda_getDevice
+from torch._C import _len_torch_dispatch_stack as _dispatch_modes
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -43,6 +45,8 @@ def _strides(*s):
 
 def _call(fn, device, *args):
     """fn on the current stream of ``device`` (an index), with that device as the current one."""
+    if _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        _refuse_tracing(None)
     if device == _cuda_getDevice():
         rc = fn(*args, _cuda_getCurrentRawStream(device))
     else:
@@ -83,6 +87,21 @@ def _check_like(q, k, v):
     _check_tensor('v', v, q.dtype, q.device)
 
 
+def _refuse_tangents(*tensors):
+    """Derivatives in forward mode: a dual tensor does not ask for a gradient, and the kernels write plain tensors -- the result's
+    tangent would read as zero.  (Called only inside a dual level.)"""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError('the sequence operators have no forward-mode derivatives')
+
+
+def _refuse_tracing(size):
+    """Calls under torch.jit.trace, where sizes are tensors, or make_fx (``_call``): a trace records torch's operators, and of these
+    calls only the empty tensor that they write into."""
+    if type(size) is not int:
+        raise ValueError('calls of the sequence operators cannot be traced')
+
+
 def _dense(t):
     return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
 
@@ -93,6 +112,8 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(*grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 
@@ -104,9 +125,12 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     ``weight`` / ``bias``  (x.size(-1),) float32 or of x's type, both of the same one; None: ones / zeros.
     Gradients reach x, weight and bias."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, bias)
     _check_tensor('x', x)
     if x.dim() < 1 or x.size(-1) < 1:
         raise ValueError('x needs a last dimension of at least one value, got %s' % (tuple(x.shape),))
+    _refuse_tracing(x.size(-1))
     if not 0.0 <= eps < math.inf:
         raise ValueError('eps must be finite and not negative, got %r' % (eps,))
     for name, p in (('weight', weight), ('bias', bias)):
@@ -192,6 +216,8 @@ class _Layout:
     """What the shapes of a call over whole sequences say; one object per combination, see ``_layout``."""
 
     def __init__(self, qs, ks, vs, n_starts, max_len, shared):
+        if qs:
+            _refuse_tracing(qs[-1])
         for name, s in (('q', qs), ('k', ks), ('v', vs)):
             if len(s) != (4 if n_starts is None else 3):
                 raise ValueError('%s must be (batch, length, heads, dim), or (rows, heads, dim) with starts; got %s' % (name, tuple(s)))
@@ -283,6 +309,8 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, starts=None, ma
                    every sequence's last row, the one ``linear_attention_step`` goes on from.
     ``max_len``    longest sequence of a packed call, a hint that sizes the launch.
     Gradients reach q, k, v and state."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q, k, v, log_decay, state)
     lay = _layout(q, k, v, starts, max_len, False)
     _check_decay(log_decay, lay.heads, q)
     scale = _scale(scale, lay.dim)
@@ -340,6 +368,8 @@ class _LinearAttention(torch.autograd.Function):
 
 @functools.lru_cache(maxsize=256)
 def _step_shapes(qs, ks, vs, shared):
+    if qs:
+        _refuse_tracing(qs[-1])
     for name, s in (('q', qs), ('k', ks), ('v', vs)):
         if len(s) != 3:
             raise ValueError('%s must be (batch, heads, dim), got %s' % (name, tuple(s)))
@@ -367,6 +397,8 @@ def _step_operands(q, k, v):
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """One row of ``linear_attention`` per sequence: q, k, v (batch, heads, dim); ``state`` (batch, heads, dim, dim) float32,
     contiguous, is updated in place.  Returns o (batch, heads, dim).  Inference only."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q, k, v, log_decay, state)
     _check_like(q, k, v)
     batch, heads, _, dim, state_shape = _step_shapes(q.shape, k.shape, v.shape, False)
     _check_decay(log_decay, heads, q)
@@ -406,6 +438,8 @@ def window_attention(q, k, v, window, sinks=0, scale=None, starts=None, max_len=
     ``k``, ``v``  may have fewer heads than q: query head h reads key head ``h // (heads // kv_heads)``.
     ``scale``   positive, dim ** -0.5 unless given.  ``max_len`` as in ``linear_attention``.
     Returns a tensor of q's shape; gradients reach q, k and v."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q, k, v)
     lay = _layout(q, k, v, starts, max_len, True)
     window, sinks, scale = _check_window(window, sinks, scale, lay.dim)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -482,6 +516,8 @@ def window_attention_step(q, k, v, cache_k, cache_v, pos, window, sinks=0, scale
     ``pos``    (batch,) int64 CUDA tensor: rows the sequence has had before this one; not changed.  Where it is negative
                the output is zero and the cache stays as it is.
     Returns o (batch, heads, dim).  Inference only."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q, k, v, cache_k, cache_v)
     _check_like(q, k, v)
     batch, heads, kv_heads, dim, _ = _step_shapes(q.shape, k.shape, v.shape, True)
     window, sinks, scale = _check_window(window, sinks, scale, dim)
@@ -508,6 +544,8 @@ def window_cache_fill(k, v, cache_k, cache_v, window, sinks=0, starts=None):
     """Keys and values of whole sequences into rolling caches, as the steps after them expect it: (batch, length, kv_heads,
     dim), or packed with ``starts``.  Slots that no row belongs to stay as they are.  Returns ``pos`` (batch,) int64: the
     lengths.  Inference only."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(k, v, cache_k, cache_v)
     lay = _layout(k, k, v, starts, None, True)
     window, sinks, _ = _check_window(window, sinks, None, lay.dim)
     cks = _check_cache('cache_k', cache_k, k, lay.n_seq, sinks + window, lay.heads, lay.dim)
