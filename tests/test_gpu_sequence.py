@@ -1046,3 +1046,33 @@ def test_derivatives_and_recordings_that_cannot_pass_are_refused(vad):
         for call in calls[:3]:
             with pytest.raises((RuntimeError, ValueError)):
                 transform(call)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('cols', [30, 900, 1024, 1025, 5000, 20001])
+def test_layer_norm_of_far_rows(vad, dtype, cols):
+    """Rows far from zero: the mean's own rounding stays out of the deviations, in either direction.  A sum of n terms of size s is
+    off by at most n 2^-24 s; taken again over the deviations, what is left of the mean's error is n 2^-24 of them and, of the
+    offset, (n 2^-24)^2."""
+    g = _gen(cols)
+    n = (cols / 64 + 10 if cols <= 4096 else 180) * ULP               # values down a lane and levels across, as in test_layer_norm
+    w, b = 1 + _rand(g, cols, scale=0.3), _rand(g, cols)
+    for offset in (1e2, 1e4, 1e6):
+        x = (_rand(g, 6, cols) + offset).to(dtype)
+        x[0], x[1], x[2] = offset, offset + 0.3, -1.37 * offset       # no variance
+        x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+        dy = _rand(g, 6, cols, dtype=dtype)
+        y = vad.layer_norm(x, w, b)
+        grads = torch.autograd.grad(y, (x, w, b), dy)
+        want = ref.layer_norm(x.detach(), w.detach(), b.detach(), 1e-5, dy)
+        xd = x.detach().double()
+        c = xd - xd.mean(1, keepdim=True)
+        r = 1 / torch.sqrt((c * c).mean(1, keepdim=True) + 1e-5)
+        xh = (c * r).abs()
+        # deviations off by n of their mean size and by their own rounding; r by the same, relatively, three roundings more
+        mag_xh = xh.mean(1, keepdim=True) + 8 * xh + n * xd.abs().amax(1, keepdim=True) * r
+        _close(y.detach(), want[0], mag_xh * w.detach().abs() + b.detach().abs(), 2 * n, dtype, 'y at %g' % offset)
+        gw = (dy.double() * w.detach()).abs()
+        mag = r * (gw + gw.mean(1, keepdim=True) + (xh + mag_xh) * (gw * (xh + mag_xh)).mean(1, keepdim=True)) * 4
+        _close(grads[0], want[1], mag, 2 * n, dtype, 'dx at %g' % offset)
+        _close(grads[1], want[2], (dy.double().abs() * (xh + mag_xh)).sum(0), 2 * n + 70 * ULP, torch.float32, 'dw at %g' % offset)

@@ -5,10 +5,16 @@
 //
 // Both directions are bound by memory: forward moves x and y once, backward x, dy and dx.  A row is held in the
 // registers of a group of lanes -- 1 .. 64 lanes of a wave, or a whole block -- so that the variance is taken around the
-// exact mean without reading the row again.  The backward pass adds dy xh and dy of all rows of a group in registers
-// (a lane keeps its columns from row to row); the groups of a block are added through LDS, the blocks by a second
-// kernel, each in a fixed order: no atomics, the same bits from call to call.  Rows too long for registers are read
-// three times, which the cache serves, and their weight gradients are summed by columns.
+// mean without reading the row again.  The mean of n values s away from zero is off by up to n 2^-24 s, as much as the
+// deviations themselves where a row lies far out: what is left of it is summed over the deviations and taken off
+// them, here and again in the backward pass, whose mean has been rounded to a float32 (one more sum across lanes: 7.0 -> 7.6 us
+// forward for 120000 rows of 24 float32, 42 -> 44 us backward for 32768 of 1024 bfloat16, others within the noise).
+//
+// The backward pass adds dy xh and dy of all rows of a group in registers (a lane keeps its columns from row to row);
+// the groups of a block are added through LDS, the blocks by a second kernel, each in a fixed order: no atomics, the
+// same bits from call to call.  Rows of more vectors than a block holds in registers -- 2048, of 16 bytes where the row's
+// length and alignment allow and else of less, down to one value -- are read four times, which the cache serves, and
+// their weight gradients are summed by columns.
 //
 // Measured: 32768 rows of 1024 bfloat16 23 us forward (134 MB, 5.8 TB/s: some of it stays in the last cache) and 41 + 4 us
 // backward (201 MB, 4.9 TB/s, and the join); 120000 rows of 24 float32 7.3 us (23 MB); 2048 rows of 900 float32 5.8 us
@@ -138,6 +144,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T* __restric
 #pragma unroll
     for (int n = 0; n < NV; ++n) ahead[n] = Raw<T, VE>{};
     fetch((int64_t)blockIdx.x * per_block);
+    const float inv = 1.0f / (float)a.cols;
     // every group of a block makes the same number of turns: a whole-block group meets barriers
     for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows; base += step) {
         const int64_t row = base + threadIdx.x / a.lanes;
@@ -152,13 +159,24 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T* __restric
 #pragma unroll
             for (int e = 0; e < VE; ++e) sum += v[n][e];
         const float mean = group_sum(sum, a.lanes, scratch) / (float)a.cols;
-        float sq = 0.0f;
+        float left = 0.0f, sq = 0.0f;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if ((l + n * a.lanes) * VE < a.cols) {
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
                     v[n][e] -= mean;
+                    left += v[n][e];
+                }
+            }
+        }
+        left = group_sum(left, a.lanes, scratch) * inv;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            if ((l + n * a.lanes) * VE < a.cols) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    v[n][e] -= left;
                     sq = fmaf(v[n][e], v[n][e], sq);
                 }
             }
@@ -166,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_kernel(const T* __restric
         const float rstd = 1.0f / sqrtf(group_sum(sq, a.lanes, scratch) / (float)a.cols + a.eps);
         if (!live) continue;
         if (stats && l == 0) {
-            stats[2 * row] = mean;
+            stats[2 * row] = mean + left;
             stats[2 * row + 1] = rstd;
         }
         T* yr = y + row * a.cols;
@@ -220,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
         const bool live = row < a.rows;
         const float mean = live ? stats[2 * row] : 0.0f, rstd = live ? stats[2 * row + 1] : 0.0f;
         float v[NV][VE], g[NV][VE];
-        float s1 = 0.0f, s2 = 0.0f;
+        float left = 0.0f, s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             unpack<T, VE>(ahead_x[n], v[n]);
@@ -232,7 +250,18 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
             if (live && (l + n * a.lanes) * VE < a.cols) {
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
-                    v[n][e] = (v[n][e] - mean) * rstd;
+                    v[n][e] -= mean;
+                    left += v[n][e];
+                }
+            }
+        }
+        left = group_sum(left, a.lanes, scratch) * inv;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            if (live && (l + n * a.lanes) * VE < a.cols) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    v[n][e] = (v[n][e] - left) * rstd;
                     dw[n][e] = fmaf(g[n][e], v[n][e], dw[n][e]);
                     db[n][e] += g[n][e];
                     g[n][e] *= w[n][e];
@@ -299,7 +328,15 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_kernel(const T* __re
     for (int c = threadIdx.x; c < 2 * a.cols; c += kThreads) out[c] = sums[c];
 }
 
-// Rows longer than a block's registers: three passes over the row.
+// What is left of a row's mean behind `mean`, by a whole block.
+template <typename T>
+__device__ __forceinline__ float mean_left(const T* x, float mean, int cols, float* scratch) {
+    float sum = 0.0f;
+    for (int c = threadIdx.x; c < cols; c += kThreads) sum += (float)x[c] - mean;
+    return group_sum(sum, kThreads, scratch) / (float)cols;
+}
+
+// Rows of more vectors than a block holds in registers: four passes over the row.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void layer_norm_long_kernel(const T* __restrict__ x, Rows a, Params<T> pr, T* __restrict__ y,
                                                                    float* __restrict__ stats) {
@@ -308,42 +345,54 @@ __global__ __launch_bounds__(kThreads) void layer_norm_long_kernel(const T* __re
         const T* xr = x + row * a.x_stride;
         float sum = 0.0f, sq = 0.0f;
         for (int c = threadIdx.x; c < a.cols; c += kThreads) sum += (float)xr[c];
-        const float mean = group_sum(sum, kThreads, scratch) / (float)a.cols;
+        const float mean = group_sum(sum, kThreads, scratch) / (float)a.cols, left = mean_left(xr, mean, a.cols, scratch);
         for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-            const float d = (float)xr[c] - mean;
+            const float d = (float)xr[c] - mean - left;
             sq = fmaf(d, d, sq);
         }
         const float rstd = 1.0f / sqrtf(group_sum(sq, kThreads, scratch) / (float)a.cols + a.eps);
         if (stats && threadIdx.x == 0) {
-            stats[2 * row] = mean;
+            stats[2 * row] = mean + left;
             stats[2 * row + 1] = rstd;
         }
         for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-            y[row * a.cols + c] = (T)fmaf(((float)xr[c] - mean) * rstd, pr.w ? pr.at(pr.w, c) : 1.0f, pr.b ? pr.at(pr.b, c) : 0.0f);
+            y[row * a.cols + c] = (T)fmaf(((float)xr[c] - mean - left) * rstd, pr.w ? pr.at(pr.w, c) : 1.0f, pr.b ? pr.at(pr.b, c) : 0.0f);
         }
     }
 }
 
+// left[row] for the weights' gradients of long rows.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void layer_norm_left_kernel(const T* __restrict__ x, Rows a, const float* __restrict__ stats,
+                                                                   float* __restrict__ left) {
+    __shared__ float scratch[kThreads / 64];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float m = mean_left(x + row * a.x_stride, stats[2 * row], a.cols, scratch);
+        if (threadIdx.x == 0) left[row] = m;
+    }
+}
+
+// left: that of every row where it is known, else null.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void layer_norm_grad_long_kernel(const T* __restrict__ x, const T* __restrict__ dy, Rows a,
                                                                         int64_t dy_stride, Params<T> pr, const float* __restrict__ stats,
-                                                                        T* __restrict__ dx) {
+                                                                        const float* __restrict__ left, T* __restrict__ dx) {
     __shared__ float scratch[kThreads / 64];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* xr = x + row * a.x_stride;
         const T* gr = dy + row * dy_stride;
-        const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+        const float mean = stats[2 * row], rstd = stats[2 * row + 1], rest = left ? left[row] : mean_left(xr, mean, a.cols, scratch);
         float s1 = 0.0f, s2 = 0.0f;
         for (int c = threadIdx.x; c < a.cols; c += kThreads) {
             const float g = (float)gr[c] * (pr.w ? pr.at(pr.w, c) : 1.0f);
             s1 += g;
-            s2 = fmaf(g, ((float)xr[c] - mean) * rstd, s2);
+            s2 = fmaf(g, ((float)xr[c] - mean - rest) * rstd, s2);
         }
         s1 = group_sum(s1, kThreads, scratch) / (float)a.cols;
         s2 = group_sum(s2, kThreads, scratch) / (float)a.cols;
         for (int c = threadIdx.x; c < a.cols; c += kThreads) {
             const float g = (float)gr[c] * (pr.w ? pr.at(pr.w, c) : 1.0f);
-            dx[row * a.cols + c] = (T)(rstd * (g - s1 - ((float)xr[c] - mean) * rstd * s2));
+            dx[row * a.cols + c] = (T)(rstd * (g - s1 - ((float)xr[c] - mean - rest) * rstd * s2));
         }
     }
 }
@@ -352,13 +401,13 @@ __global__ __launch_bounds__(kThreads) void layer_norm_grad_long_kernel(const T*
 template <typename T>
 __global__ __launch_bounds__(kThreads) void layer_norm_columns_kernel(const T* __restrict__ x, const T* __restrict__ dy, Rows a,
                                                                       int64_t dy_stride, const float* __restrict__ stats,
-                                                                      float* __restrict__ part) {
+                                                                      const float* __restrict__ left, float* __restrict__ part) {
     const int c = blockIdx.x * kThreads + threadIdx.x;
     if (c >= a.cols) return;
     float dw = 0.0f, db = 0.0f;
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float g = (float)dy[row * dy_stride + c];
-        dw = fmaf(g, ((float)x[row * a.x_stride + c] - stats[2 * row]) * stats[2 * row + 1], dw);
+        dw = fmaf(g, ((float)x[row * a.x_stride + c] - stats[2 * row] - left[row]) * stats[2 * row + 1], dw);
         db += g;
     }
     float* out = part + (int64_t)blockIdx.y * 2 * a.cols;
@@ -475,12 +524,13 @@ int run_backward(const void* x, const void* dy, int64_t rows, int64_t cols, int6
         VAD_LN_LAUNCH(layer_norm_grad_kernel, T, dim3((unsigned)parts), dim3(kThreads), lds, st, xp, gp, a, dy_stride, pr, stats, dxp,
                       sums ? part : nullptr);
     } else {
-        if (dx)
-            hipLaunchKernelGGL((layer_norm_grad_long_kernel<T>), dim3((unsigned)row_blocks(rows, kThreads, 256 * 8)), dim3(kThreads),
-                               0, st, xp, gp, a, dy_stride, pr, stats, dxp);
+        const dim3 grid((unsigned)row_blocks(rows, kThreads, 256 * 8));
+        float* left = sums ? part + (int64_t)parts * 2 * cols : nullptr;
+        if (sums) hipLaunchKernelGGL((layer_norm_left_kernel<T>), grid, dim3(kThreads), 0, st, xp, a, stats, left);
+        if (dx) hipLaunchKernelGGL((layer_norm_grad_long_kernel<T>), grid, dim3(kThreads), 0, st, xp, gp, a, dy_stride, pr, stats, left, dxp);
         if (sums)
             hipLaunchKernelGGL((layer_norm_columns_kernel<T>), dim3((unsigned)((cols + kThreads - 1) / kThreads), (unsigned)parts),
-                               dim3(kThreads), 0, st, xp, gp, a, dy_stride, stats, part);
+                               dim3(kThreads), 0, st, xp, gp, a, dy_stride, stats, left, part);
     }
     VAD_HIP_CHECK(hipGetLastError());
     if (sums) {
@@ -496,7 +546,9 @@ int run_backward(const void* x, const void* dy, int64_t rows, int64_t cols, int6
 
 extern "C" size_t vad_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return (size_t)(rows < vad::kMaxParts ? rows : vad::kMaxParts) * 2 * (size_t)cols * sizeof(float);
+    // rows of more than one value a vector and thread may be too long for registers: their means' remainders as well
+    const size_t left = cols > vad::kMaxVecs * vad::kThreads ? (size_t)rows : 0;
+    return ((size_t)(rows < vad::kMaxParts ? rows : vad::kMaxParts) * 2 * (size_t)cols + left) * sizeof(float);
 }
 
 extern "C" int vad_layer_norm_forward(const void* x_dev, int64_t rows, int64_t cols, int64_t x_stride, const void* weight_dev,
