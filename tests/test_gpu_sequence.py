@@ -1076,3 +1076,33 @@ def test_layer_norm_of_far_rows(vad, dtype, cols):
         mag = r * (gw + gw.mean(1, keepdim=True) + (xh + mag_xh) * (gw * (xh + mag_xh)).mean(1, keepdim=True)) * 4
         _close(grads[0], want[1], mag, 2 * n, dtype, 'dx at %g' % offset)
         _close(grads[1], want[2], (dy.double().abs() * (xh + mag_xh)).sum(0), 2 * n + 70 * ULP, torch.float32, 'dw at %g' % offset)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_single_rows_of_any_stride(vad, dtype):
+    """One row has no row stride, whatever its tensor says: a slice of a longer batch, one frame of many channels kept time first,
+    heads laid out behind the row."""
+    g = _gen(15)
+    log_decay = torch.tensor([-0.1], device='cuda').expand(64).contiguous()
+    wide = torch.zeros(2, 8192, 16, 64, dtype=dtype, device='cuda')[0:1, 0]
+    frame = torch.zeros(1, 8192, 32, 16, dtype=dtype, device='cuda').transpose(0, 1)
+    inside = torch.zeros(3, 4, 32, 1, dtype=dtype, device='cuda').permute(0, 3, 1, 2)
+    assert wide.stride(0) >= 1 << 22 and frame.stride(1) >= 1 << 22 and inside.stride(1) == 1
+    for t in (wide, frame, inside):
+        t.copy_(_rand(g, *t.shape, dtype=dtype))
+        starts = torch.tensor([0, 1], device='cuda') if t.dim() == 3 else None
+        heads, dim, n = t.size(-2), t.size(-1), 1 if t.dim() == 3 else t.size(0)
+
+        def run(x, gy):
+            leaf = [x.detach().requires_grad_() for _ in range(3)]
+            o, s = vad.linear_attention(*leaf, log_decay[:heads], starts=starts)
+            w = vad.window_attention(*leaf, 5, 1, starts=starts)
+            ck, cv = (torch.zeros(n, 6, heads, dim, dtype=dtype, device='cuda') for _ in range(2))
+            with torch.no_grad():
+                pos = vad.window_cache_fill(x, x, ck, cv, 5, 1, starts=starts)
+            return [o, s, w, ck, cv, pos, *torch.autograd.grad(o, leaf, gy), *torch.autograd.grad(w, leaf, gy)]
+
+        plain = t.clone(memory_format=torch.contiguous_format)
+        plain = plain.as_strided(plain.shape, torch.empty(plain.shape).stride())
+        for a, b in zip(run(t, t), run(plain, plain)):
+            assert torch.equal(a, b)

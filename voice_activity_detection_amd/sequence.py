@@ -230,6 +230,7 @@ class _Layout:
         if self.heads % self.kv_heads or (not shared and self.heads != self.kv_heads):
             raise ValueError('%d query heads cannot use %d key heads' % (self.heads, self.kv_heads))
         self.packed = n_starts is not None
+        self.one_row = qs[-3] <= 1          # its stride says nothing, and a copy would not change it
         if self.packed:
             self.n_seq, self.n_rows = n_starts - 1, qs[0]
             if max_len is not None and max_len < 0:
@@ -244,12 +245,13 @@ class _Layout:
         self.table = functools.lru_cache(maxsize=64)(self._table)
 
     def _table(self, s):
-        return _strides(*((0,) + s[:2] if self.packed else s[:3]))
+        sequence, row, head = (0, *s[:2]) if self.packed else s[:3]
+        return _strides(sequence, self.dim if self.one_row else row, head)
 
     def operand(self, t):
         """t with a dense head dimension, and its {sequence, row, head} strides."""
         t = _dense(t)
-        if t.stride(-3) >= MAX_ROW_STRIDE:
+        if t.stride(-3) >= MAX_ROW_STRIDE and not self.one_row:
             t = t.contiguous()
         return t, self.table(t.stride())
 
