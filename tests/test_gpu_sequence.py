@@ -1106,3 +1106,17 @@ def test_single_rows_of_any_stride(vad, dtype):
         plain = plain.as_strided(plain.shape, torch.empty(plain.shape).stride())
         for a, b in zip(run(t, t), run(plain, plain)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_caches_of_one_slot_at_any_stride(vad, dtype):
+    """A cache of one slot has no slot stride: what the slot held before, NaN here, does not come back as that of a next one."""
+    g = _gen(16)
+    q, k, v = (_rand(g, 3, 2, 64, dtype=dtype) for _ in range(3))
+    pos = torch.tensor([0, 5, 9], device='cuda')
+    caches = [torch.full((3, 2, 64, 1), math.nan, dtype=dtype, device='cuda').permute(0, 3, 1, 2) for _ in range(2)]
+    caches += [torch.full((3, 2, 64), math.nan, dtype=dtype, device='cuda').as_strided((3, 1, 2, 64), (128, 0, 64, 1)) for _ in range(2)]
+    assert caches[0].stride(1) == 1
+    for ck, cv in (caches[:2], caches[2:]):
+        o = vad.window_attention_step(q, k, v, ck, cv, pos, 1)
+        assert torch.equal(o, v) and torch.equal(ck[:, 0], k) and torch.equal(cv[:, 0], v)

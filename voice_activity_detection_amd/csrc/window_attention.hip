@@ -1215,9 +1215,10 @@ extern "C" int vad_window_attention_step(const void* q_dev, const int64_t* q_str
         const int group = heads / kv_heads, gb = step_heads(group);
         a.chunks = (group + gb - 1) / gb;
         a.splits = step_splits(batch, kv_heads, a.chunks, sinks + window);
-        // (a cache may be laid out with any slot stride: row_buffer takes those below VAD_MAX_ROW_STRIDE)
-        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim) &&
-                  a.ck.st < VAD_MAX_ROW_STRIDE && a.cv.st < VAD_MAX_ROW_STRIDE;
+        // A cache may be laid out with any slot stride.  A buffer takes those below VAD_MAX_ROW_STRIDE, and ends with the last slot
+        // only where slots lie behind one another: that of a single slot may be anything.
+        a.whole = whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.ck, dim) && whole_words(a.cv, dim);
+        for (const int64_t st : {a.ck.st, a.cv.st}) a.whole = a.whole && st >= dim && st < VAD_MAX_ROW_STRIDE;
         return run_step<T>(a, batch, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
