@@ -8,6 +8,7 @@ values; the softmax's dS carries two (the weight itself, and rowsum(dO O) formed
 terms is off by at most n 2^-24 mag.  A softmax weight inherits the absolute error of its score, (dim + 4) 2^-24 `size`, once
 from itself and once from the sum it is divided by; powers of the decay are exponentials of at most 87 (larger ones vanish):
 90 2^-24."""
+import ctypes
 import math
 
 import pytest
@@ -1120,3 +1121,32 @@ def test_caches_of_one_slot_at_any_stride(vad, dtype):
     for ck, cv in (caches[:2], caches[2:]):
         o = vad.window_attention_step(q, k, v, ck, cv, pos, 1)
         assert torch.equal(o, v) and torch.equal(ck[:, 0], k) and torch.equal(cv[:, 0], v)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_overlapping_rows(vad, dtype):
+    """One row for all, and rows that share memory, reach no further than copies of them: an infinite key stays one infinity in the
+    state's row."""
+    g = _gen(17)
+    n, dim = 70, 64
+    log_decay = torch.zeros(1, device='cuda')
+    q, v = (_rand(g, 1, n, 1, dim, dtype=dtype).abs() + 0.5 for _ in range(2))
+    row = _rand(g, 1, 1, 1, dim, dtype=dtype)
+    row[..., 7] = math.inf
+    run = _rand(g, n + dim, dtype=dtype)
+    run[3 * dim // 2] = math.inf
+    for k in (row.expand(1, n, 1, dim), run.as_strided((1, n, 1, dim), (n + dim, 1, dim, 1))):
+        for got, want in zip(vad.linear_attention(q, k, v, log_decay), vad.linear_attention(q, k.contiguous(), v, log_decay)):
+            assert torch.equal(got.nan_to_num(), want.nan_to_num()) and torch.equal(got.isnan(), want.isnan())
+        s = vad.linear_attention(q, k, v, log_decay)[1]
+        assert s.isinf().any() and not s.isnan().any()
+        # the entry point itself, which Python calls with copies of such rows
+        L, strides = vad.lib(), [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+        size = L.vad_linear_attention_workspace_bytes(1, n, 1, dim, 0)
+        ws, o, state = torch.empty(size, dtype=torch.uint8, device='cuda'), torch.empty_like(v), torch.empty_like(s)
+        rc = L.vad_linear_attention_forward(q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[2], None, 1, 0, n, 1, dim,
+                                            dtype is torch.bfloat16, log_decay.data_ptr(), dim ** -0.5, None, o.data_ptr(), state.data_ptr(),
+                                            ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(state, s) and torch.equal(o.nan_to_num(), vad.linear_attention(q, k, v, log_decay)[0].nan_to_num())
+        for got, want in zip(vad.linear_attention(q, v, k, log_decay), vad.linear_attention(q, v, k.contiguous(), log_decay)):
+            assert torch.equal(got.nan_to_num(), want.nan_to_num()) and torch.equal(got.isnan(), want.isnan())

@@ -551,7 +551,7 @@ int run_forward(const void* q, const int64_t* qs, const void* k, const int64_t* 
     a.dim = dim;
     a.n_spans = n_spans;
     a.joined = n_spans > kJoinFrom;
-    a.whole = whole_words(a.walk[0].q, dim) && whole_words(a.walk[0].k, dim) && whole_words(a.walk[0].v, dim) && whole_words(a.walk[0].o, dim);
+    a.whole = whole_rows(a.walk[0].q, dim) && whole_rows(a.walk[0].k, dim) && whole_rows(a.walk[0].v, dim) && whole_words(a.walk[0].o, dim);
     return run_walks(a, 1, st);
 }
 
@@ -572,7 +572,7 @@ int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t*
     a.dim = dim;
     a.n_spans = n_spans;
     a.joined = n_spans > kJoinFrom;
-    a.whole = whole_words(Q, dim) && whole_words(K, dim) && whole_words(V, dim) && whole_words(G, dim);
+    a.whole = whole_rows(Q, dim) && whole_rows(K, dim) && whole_rows(V, dim) && whole_rows(G, dim);
     for (const Walk<T>& w : a.walk) a.whole = a.whole && whole_words(w.o, dim);
     return run_walks(a, 3, st);
 }

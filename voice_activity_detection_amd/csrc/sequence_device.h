@@ -203,6 +203,12 @@ bool whole_words(const Heads<T>& x, int dim) {
     const uint64_t at = reinterpret_cast<uintptr_t>(x.p) | (uint64_t)(x.sb * sizeof(T)) | (uint64_t)(x.st * sizeof(T)) | (uint64_t)(x.sh * sizeof(T));
     return at % 4 == 0 && dim * sizeof(T) % 4 == 0;
 }
+// The same of rows that a buffer can end behind: it leaves out what lies behind the last row, which rows that overlap -- one
+// for all, or windows over one run of values -- would find in the rows before it.
+template <typename T>
+bool whole_rows(const Heads<T>& x, int dim) {
+    return x.st >= dim && whole_words(x, dim);
+}
 template <typename T>
 bool whole_words(const T* p, int dim) {
     return reinterpret_cast<uintptr_t>(p) % 4 == 0 && dim * sizeof(T) % 4 == 0;

@@ -1074,7 +1074,7 @@ extern "C" int vad_window_attention_forward(const void* q_dev, const int64_t* q_
         a.seq = {starts_dev, n_tokens, max_len};
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
-        a.whole = whole_words(a.q, dim) && whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.out, dim);
+        a.whole = whole_rows(a.q, dim) && whole_rows(a.k, dim) && whole_rows(a.v, dim) && whole_words(a.out, dim);
         return run_forward<T>(a, static_cast<hipStream_t>(stream));
     };
     return dtype == VAD_DTYPE_F32 ? run(0.0f) : run((__bf16)0.0f);
@@ -1127,7 +1127,7 @@ extern "C" int vad_window_attention_backward(const void* q_dev, const int64_t* q
         a.n_seq = (int)n_seq, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
         a.window = (int)window, a.sinks = sinks, a.scale = scale;
         a.segments = sink_segments(n_seq, max_len, heads, kv_heads, (int)window);
-        a.whole = whole_words(a.q, dim) && whole_words(a.k, dim) && whole_words(a.v, dim) && whole_words(a.go, dim) && whole_words(a.o, dim) &&
+        a.whole = whole_rows(a.q, dim) && whole_rows(a.k, dim) && whole_rows(a.v, dim) && whole_rows(a.go, dim) && whole_words(a.o, dim) &&
                   whole_words(a.out, dim) && whole_words(a.dk, dim) && whole_words(a.dv, dim);
         return run_backward<T>(a, static_cast<hipStream_t>(stream));
     };

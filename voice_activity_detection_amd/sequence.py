@@ -249,9 +249,10 @@ class _Layout:
         return _strides(sequence, self.dim if self.one_row else row, head)
 
     def operand(self, t):
-        """t with a dense head dimension, and its {sequence, row, head} strides."""
+        """t with a dense head dimension, and its {sequence, row, head} strides.  Rows too far apart for the kernels are brought
+        together; rows that overlap, which they would read value by value, are taken apart."""
         t = _dense(t)
-        if t.stride(-3) >= MAX_ROW_STRIDE and not self.one_row:
+        if not self.dim <= t.stride(-3) < MAX_ROW_STRIDE and not self.one_row:
             t = t.contiguous()
         return t, self.table(t.stride())
 
