@@ -1150,3 +1150,23 @@ def test_overlapping_rows(vad, dtype):
         assert rc == 0 and torch.equal(state, s) and torch.equal(o.nan_to_num(), vad.linear_attention(q, k, v, log_decay)[0].nan_to_num())
         for got, want in zip(vad.linear_attention(q, v, k, log_decay), vad.linear_attention(q, v, k.contiguous(), log_decay)):
             assert torch.equal(got.nan_to_num(), want.nan_to_num()) and torch.equal(got.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('at', [3, 100, 200])
+def test_window_attention_infinite_keys_in_dq(vad, dtype, at):
+    """A key with an infinity has a score of an infinity or NaN for every row that sees it.  Where that is minus infinity its weight
+    is zero and dS K is zero times infinity, wherever the key stands in its tile; rows that do not see it stay finite."""
+    g = _gen(18)
+    n, window, sinks = 300, 90, 4
+    q, do = (_rand(g, 1, n, 2, 64, dtype=dtype).abs() + 0.1 for _ in range(2))
+    k, v = (_rand(g, 1, n, 1, 64, dtype=dtype) for _ in range(2))
+    k[0, at, 0, 9] = -math.inf
+    leaf = [t.requires_grad_() for t in (q, k, v)]
+    o = vad.window_attention(*leaf, window, sinks)
+    dq = torch.autograd.grad(o, leaf, do)[0]
+    rows = torch.arange(n, device='cuda')
+    sees = (rows >= at) & ((rows - at < window) | (at < sinks)) & (rows > 0)
+    assert dq[0, sees][..., 9].isnan().all()
+    others = torch.arange(64, device='cuda') != 9
+    assert torch.isfinite(o).all() and torch.isfinite(dq[0, ~sees]).all() and torch.isfinite(dq[0, sees][..., others]).all()

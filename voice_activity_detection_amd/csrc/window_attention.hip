@@ -22,8 +22,9 @@
 // A row outside a key's window must not feel what that key holds.  Scores are replaced, not multiplied, where the mask
 // says so.  Where a partly visible tile holds an infinity or a NaN, which the matrix product would multiply by zero, it is
 // taken out of the tile once the scores are formed.  A visible one still reaches its rows: through a weight that its own
-// score has made NaN, or, where no score depends on it (V in O, dO in dV), by a pass over the block's outputs at its end,
-// which costs a block that meets one milliseconds and the others nothing.
+// score has made NaN, or, where no score depends on it (V in O, dO in dV) or the score may be minus infinity and its weight
+// zero (K in dQ), by a pass over the block's outputs at its end, which costs a block that meets one milliseconds and the
+// others nothing.
 
 #include <mutex>
 #include <type_traits>
@@ -431,13 +432,16 @@ __global__ __launch_bounds__(kThreads, 2) void window_rows_kernel(WindowArgs<T> 
                 for (int b = 0; b < DP / 16; ++b) store_quad(a.out + at * dim, 16 * b + 4 * g, dim, acc[b][nb] * f, BUF);
             }
         }
-        if (!BACK && met) {
+        if (met) {
             __syncthreads();
+            const T* p = BACK ? kp : vp;
+            const int64_t st = BACK ? a.k.st : a.v.st;
             for (int e = threadIdx.x; e < (r1 - r0 + 1) * dim; e += kThreads) {
                 const int row = r0 + e / dim, d = e % dim, lo = row - a.window + 1 > 0 ? row - a.window + 1 : 0;
-                const float x = not_finite_sum(vp + d, a.v.st, lo, (int64_t)row + 1) + not_finite_sum(vp + d, a.v.st, 0, lo < a.sinks ? lo : a.sinks);
+                const float x = not_finite_sum(p + d, st, lo, (int64_t)row + 1) + not_finite_sum(p + d, st, 0, lo < a.sinks ? lo : a.sinks);
                 T* o = a.out + ((row_base + row) * a.heads + h) * dim + d;
-                if (x != 0.0f) *o = (T)((float)*o + x);
+                // dS of such a key is zero or NaN, and so dS K is NaN
+                if (x != 0.0f) *o = BACK ? (T)NAN : (T)((float)*o + x);
             }
             met = false;
         }
