@@ -455,6 +455,7 @@ int vad_layer_norm_backward(const void* x_dev, const void* dy_dev, int64_t rows,
 /*
  * Linear attention with a decay per head:  S_t = exp(log_decay) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t.
  *   log_decay_dev   heads float32, <= 0.  Not validated: values are clamped into -87 .. 0.
+ *   scale           finite
  *   state_in_dev    (n_seq, heads, dim, dim) float32, S before the first row ([key dim][value dim]); NULL = zero
  *   state_out_dev   S behind the last row (state_in for an empty sequence); may be NULL, must not be state_in_dev
  * Backward: do_dev the gradient of o, dstate_out_dev that of state_out (NULL = zero); dq_dev / dk_dev / dv_dev dense,

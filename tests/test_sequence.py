@@ -164,3 +164,16 @@ def test_forward_mode_derivatives_are_refused():
                     call(*args[:i], forward_ad.make_dual(t, torch.ones_like(t)), *args[i + 1:])
             with pytest.raises(ValueError, match='CUDA tensor'):        # others are as welcome as outside
                 call(*args)
+
+
+def test_scales_past_float32_are_refused(L):
+    """A scale that a double holds and a float32 does not would come out as infinity."""
+    buf = np.zeros(256, np.float32)
+    ok = buf.ctypes.data
+    s3, s2 = _strides(1, 1, 1), _strides(1, 1)
+    hd = (ok, s3) * 3
+    for scale in (1e39, -1e39, math.inf, math.nan):
+        for name, args in (('vad_linear_attention_forward', (*hd, None, 1, 0, 4, 1, 4, 0, ok, scale, None, ok, None, None, 0, None)),
+                           ('vad_linear_attention_backward', (*hd, ok, s3, None, 1, 0, 4, 1, 4, 0, ok, scale, None, None, ok, ok, ok, None, None, 0, None)),
+                           ('vad_linear_attention_step', (ok, s2, ok, s2, ok, s2, 1, 1, 4, 0, ok, scale, ok, ok, None))):
+            assert getattr(L, name)(*args) == -1 and b'scale' in L.vad_last_error(), (name, scale)

@@ -577,10 +577,11 @@ int run_backward(const void* q, const int64_t* qs, const void* k, const int64_t*
     return run_walks(a, 3, st);
 }
 
-int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int dim, int dtype) {
+int check_heads(int64_t n_seq, int64_t n_tokens, int64_t max_len, int heads, int dim, int dtype, float scale) {
     VAD_REQUIRE(dtype == VAD_DTYPE_F32 || dtype == VAD_DTYPE_BF16, "dtype must be VAD_DTYPE_F32 or VAD_DTYPE_BF16, got %d", dtype);
     VAD_REQUIRE(dim >= 1 && dim <= VAD_MAX_HEAD_DIM, "head dimension %d out of range 1..%d", dim, VAD_MAX_HEAD_DIM);
     VAD_REQUIRE(heads >= 1, "heads must be positive, got %d", heads);
+    VAD_REQUIRE(fabsf(scale) < INFINITY, "scale must be finite in float32");
     VAD_REQUIRE(n_seq >= 0 && n_tokens >= 0 && max_len >= 0, "negative sequence count or length");
     VAD_REQUIRE(n_tokens <= (1 << 30) && max_len <= (1 << 30), "length out of range");
     // a step launches up to four blocks of 256 threads for each, and a launch's threads are counted in 32 bits
@@ -627,7 +628,7 @@ extern "C" int vad_linear_attention_forward(const void* q_dev, const int64_t* q_
                                             const float* log_decay_dev, float scale, const float* state_in_dev, void* o_dev,
                                             float* state_out_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     using namespace vad;
-    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype);
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype, scale);
     if (rc != VAD_OK) return rc;
     VAD_REQUIRE(q_strides && k_strides && v_strides && log_decay_dev, "null pointer argument");
     if (n_seq == 0) return VAD_OK;
@@ -658,7 +659,7 @@ extern "C" int vad_linear_attention_backward(const void* q_dev, const int64_t* q
                                              const float* dstate_out_dev, void* dq_dev, void* dk_dev, void* dv_dev,
                                              float* dstate_in_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     using namespace vad;
-    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype);
+    int rc = check_heads(n_seq, n_tokens, max_len, heads, dim, dtype, scale);
     if (rc != VAD_OK) return rc;
     VAD_REQUIRE(q_strides && k_strides && v_strides && do_strides && log_decay_dev, "null pointer argument");
     if (n_seq == 0) return VAD_OK;
@@ -688,7 +689,7 @@ extern "C" int vad_linear_attention_step(const void* q_dev, const int64_t* q_str
                                          const void* v_dev, const int64_t* v_strides, int64_t batch, int heads, int dim, int dtype,
                                          const float* log_decay_dev, float scale, float* state_dev, void* o_dev, void* stream) {
     using namespace vad;
-    int rc = check_heads(batch, 0, 0, heads, dim, dtype);
+    int rc = check_heads(batch, 0, 0, heads, dim, dtype, scale);
     if (rc != VAD_OK) return rc;
     if (batch == 0) return VAD_OK;
     VAD_REQUIRE(q_dev && k_dev && v_dev && q_strides && k_strides && v_strides && log_decay_dev && state_dev && o_dev, "null pointer argument");
