@@ -415,7 +415,7 @@ int vad_threshold_sweep_noalloc_f32(const float* score_dev, int64_t score_stride
  *                are float32.
  *   rows         q, k, v and the gradients of outputs are read through strides in ELEMENTS given on the host: {sequence,
  *                row, head} (steps: {batch, head}, caches: {batch, slot, head}); the head dimension is dense.  Any alignment
- *                works; rows of whole 4-byte words at 4-byte boundaries take wide loads.
+ *                works; rows of whole 4-byte words at 4-byte boundaries, none of which overlap, take wide loads.
  *                Row strides (not those of caches) and dense rows (heads * dim) are below
  *                VAD_MAX_ROW_STRIDE.  Outputs are dense (rows, heads, dim).
  *   sequences    starts_dev == NULL: n_seq sequences of max_len rows each.  Otherwise the rows of all sequences are packed

@@ -16,9 +16,10 @@
 // length and alignment allow and else of less, down to one value -- are read four times, which the cache serves, and
 // their weight gradients are summed by columns.
 //
-// Measured: 32768 rows of 1024 bfloat16 23 us forward (134 MB, 5.8 TB/s: some of it stays in the last cache) and 41 + 4 us
-// backward (201 MB, 4.9 TB/s, and the join); 120000 rows of 24 float32 7.3 us (23 MB); 2048 rows of 900 float32 5.8 us
-// forward, 13.4 + 4.1 us backward, where launches and the sums of 256 blocks count as much as the 22 MB.
+// Measured: 32768 rows of 1024 bfloat16 23 us forward (134 MB, 5.8 TB/s: some of it stays in the last cache) and 43 + 4 us
+// backward (201 MB, 4.7 TB/s, and the join); 120000 rows of 24 float32 7.6 us (23 MB); 2048 rows of 900 float32 5.5 us
+// forward, 13.5 + 3.9 us backward: 512 blocks of one row a wave, whose sums are 3.7 MB written and read again beside the 22 MB.
+// Rows too long for registers: 2048 of 8191 bfloat16 47 us forward and 63 backward, of 8192 (in registers) 16 and 48.
 
 #include "sequence_device.h"
 

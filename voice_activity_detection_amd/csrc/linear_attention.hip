@@ -12,10 +12,11 @@
 // first launch computes each span's state from k and v alone, and the walk of every span starts from those before it --
 // added up by its block, or, where the spans are many, by a launch in between that goes along the sequence once.
 //
-// Measured, bfloat16 heads of 64: 4 x 16 heads of 8192 rows in 104 us (states of the spans 30, their join 7, walk 67: 268 MB
-// at 2.6 TB/s, where a copy takes 57 us -- latency along a walk and vector work on its 64 x 64 weights bound it, not memory);
-// 24 ragged sequences of up to 2000 rows and 8 heads, with gradients, 198 us.  A step of 64 x 16 states of 128 x 128 22.7 us:
-// 134 MB read and written, 5.9 TB/s with what the last cache keeps.
+// Measured, bfloat16 heads of 64: 4 x 16 heads of 8192 rows in 99 us (states of the spans 27, their join 6, walk 65: 268 MB
+// at 2.7 TB/s, where a copy takes 57 us -- latency along a walk and vector work on its 64 x 64 weights bound it, not memory);
+// 24 ragged sequences of up to 2000 rows and 8 heads, with gradients, 189 us.  A step of 64 x 16 states of 128 x 128 22.9 us:
+// 134 MB read and written, 5.9 TB/s with what the last cache keeps.  (Passes in a row; the comparisons beside the choices below
+// were taken in turn on a card that had just been idle, where the same kernels are up to a tenth slower.)
 //
 // Wave w of a block owns columns 16 w .. 16 w + 15 of the state and of the outputs.  The state stays in float32; for
 // bfloat16 inputs its update multiplies v by the decay in float32 and splits the product into bfloat16 terms -- three, which
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP, STATE>())) void decay_wa
         rv.put(sv, dim);
         if (!STATE) {
             rq.put(sq_, dim);
-            // (of bfloat16 keys as well, 67 -> 69 us on 4 x 16 heads of 8192 rows)
+            // (of bfloat16 keys as well: 67 -> 69 us on 4 x 16 heads of 8192 rows)
             if (rv.not_finite() | (sizeof(T) == 2 && rk.not_finite())) flags[turn] = 1;
         }
         __syncthreads();
@@ -353,7 +354,8 @@ __global__ __launch_bounds__(DP * 4, (walk_waves<T, DP, STATE>())) void decay_wa
         __syncthreads();
     }
     if (STATE && sizeof(T) == 2) {
-        // A NaN in a span's state: perhaps an infinity's meeting with a lower term.  Once more, row by row.
+        // A NaN in a span's state: perhaps an infinity's meeting with a lower term.  Once more, row by row: 1 ms where one
+        // of 4 x 8192 rows is NaN, and nothing where none is.
         bool spoilt = false;
 #pragma unroll
         for (int b = 0; b < DP / 16; ++b)

@@ -14,17 +14,19 @@
 // in registers.  The few sink keys are seen by every later row; their share of dK and dV is a second kernel over
 // segments of the rows, joined in a fixed order.
 //
-// Bound by matrix products and the exponentials beside them.  Measured, bfloat16: 2 x 16 heads of 128 over 8192 rows, window
-// 1000, O in 223 .. 248 us (540 .. 600 TFLOP/s of visible pairs); 8 ragged sequences of up to 2000 rows, 8 query heads of 64 on 2
-// key heads, window 300: O 41, dQ 62, dK and dV 66, those of 4 sinks 12 + 8 us.  The step reads its cache once and is bound by
-// that: 32 x 4 heads of 4004 slots of 128, 262 MB in 59 us (4.4 TB/s), 5 us for the join of its splits.
+// Bound by matrix products, the exponentials beside them and, in dK and dV of 64 columns, the reads of tiles from LDS.  Measured,
+// bfloat16: 2 x 16 heads of 128 over 8192 rows, window 1000, O in 213 us (590 TFLOP/s of visible pairs); 8 ragged sequences of
+// up to 2000 rows, 8 query heads of 64 on 2 key heads, window 300: O 36, dQ 55, dK and dV 60, those of 4 sinks 11 + 7 us.  The
+// step reads its cache once and is bound by that: 32 x 4 heads of 4004 slots of 128, 262 MB in 59 us (4.5 TB/s), 5 us for the
+// join of its splits.  (Passes in a row; the comparisons beside the choices below were taken in turn on a card that had just been
+// idle, where the same kernels are up to a sixth slower.)
 //
 // A row outside a key's window must not feel what that key holds.  Scores are replaced, not multiplied, where the mask
 // says so.  Where a partly visible tile holds an infinity or a NaN, which the matrix product would multiply by zero, it is
 // taken out of the tile once the scores are formed.  A visible one still reaches its rows: through a weight that its own
 // score has made NaN, or, where no score depends on it (V in O, dO in dV) or the score may be minus infinity and its weight
-// zero (K in dQ), by a pass over the block's outputs at its end, which costs a block that meets one milliseconds and the
-// others nothing.
+// zero (K in dQ), by a pass over the block's outputs at its end, which costs a block that meets one a walk over its
+// window (0.6 ms at 1000 rows, 6 ms at 8192) and the others nothing.
 
 #include <mutex>
 #include <type_traits>
@@ -1034,7 +1036,7 @@ int check_rows(const int64_t* strides) {
 
 }  // namespace
 
-// The float32 tiles of 65 and more columns use more than 64 KB of LDS: opt in once per device.
+// The tiles of 33 and more columns of float32, 65 and more of bfloat16, use more than 64 KB of LDS: opt in once per device.
 int ensure_window_attention_attrs() {
     static std::mutex mu;
     static bool done[64] = {false};
