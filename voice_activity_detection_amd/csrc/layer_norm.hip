@@ -547,7 +547,7 @@ int run_backward(const void* x, const void* dy, int64_t rows, int64_t cols, int6
 
 extern "C" size_t vad_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    // rows of more than one value a vector and thread may be too long for registers: their means' remainders as well
+    // rows of more than 2048 values may be too long for registers: what is left of their means as well, a float a row
     const size_t left = cols > vad::kMaxVecs * vad::kThreads ? (size_t)rows : 0;
     return ((size_t)(rows < vad::kMaxParts ? rows : vad::kMaxParts) * 2 * (size_t)cols + left) * sizeof(float);
 }
